@@ -58,7 +58,8 @@ enum { UMT_WARP_CV2_FIXED_POINT = 0, UMT_WARP_FLOAT = 1, UMT_WARP_CV2_FIXED_POIN
 enum { UMT_WARP_NO_DEPTH_CHECK = 0x100 };
 
 const char* umt_last_error(void);
-/* bumped on every signature change; bindings compare it with the value they were written for */
+/* bumped when a signature changes; bindings compare it with the value they were written for.  Functions that are only
+ * added leave it as it is: a binding that needs one finds out when it looks the symbol up */
 #define UMT_ABI_VERSION 4
 int umt_abi_version(void);
 
@@ -75,8 +76,11 @@ enum {
   UMT_STATUS_BAD_SAMPLE_RANGE = 4,         /* sample_range row outside [0, n] or not 1 or 2 views: the sample's outputs
                                               are NaN */
   UMT_STATUS_NONFINITE_OUTPUT = 8,         /* a regressor output row was not finite: its decoded outputs are NaN */
-  UMT_STATUS_BAD_BONE_INDEX = 16           /* umt_fk_landmarks: a landmark's bone index outside [0, 16] (IndexError in
+  UMT_STATUS_BAD_BONE_INDEX = 16,          /* umt_fk_landmarks: a landmark's bone index outside [0, 16] (IndexError in
                                               the reference); that landmark is NaN */
+  UMT_STATUS_BAD_ROW = 32,                 /* umt_rows_*: a row number outside the cache, or a fork of a free row: nothing
+                                              is done for it */
+  UMT_STATUS_NO_FREE_ROW = 64              /* umt_rows_fork: fewer free rows than forks; the forks left over get row -1 */
 };
 
 /* ---- model handle: replaces load_pretrained_model, lib/models/model_loader.py:53-88 ---- */
@@ -274,6 +278,81 @@ int umt_metric_partials(const float* gt, const float* pred, const uint8_t* valid
 #define UMT_METRIC_STATIC_MAX_HAND_FRAMES 524288
 int umt_metric_partials_static(const float* gt, const float* pred, const uint8_t* valid, int n_rec, int t,
                                double* partials, void* stream);
+
+/* ---- gated linear recurrence over recordings, no counterpart in the reference (whose only sequence state is the
+ * temporal module).  Per row (one hand track) and feature, with a = sigmoid(gate):
+ *     h[t] = a[t] * h[t-1] + (1 - a[t]) * x[t]                        h[-1] = h0, or 0 where h0 is NULL
+ * use_memory[t,row] == 0 drops the memory (h[t] = x[t], whatever h[t-1] holds), valid[t,row] == 0 skips the frame
+ * (h[t] = h[t-1]; x and gate of that frame may hold anything, NaN included); both 0 leave h[t] = 0.  Either mask may
+ * be NULL (all ones).  A non-finite x, gate or state that no mask excludes makes its feature non-finite (NaN) until the
+ * memory is dropped.  The state is float32 whatever the dtype; h is rounded once, to nearest even.
+ *
+ * features = groups * share: `share` consecutive features use one gate (a landmark's 3 coordinates, a hand's 63, 1).
+ * Element (t, row, feature) of x lies at t * x_t + row * x_row + feature, and so on: strides in elements, not negative,
+ * 0 allowed for what is read.  h and dx share out_t / out_row.  What is written must not overlap itself.
+ * h0, h_last, dh0, dh_last: dev f32 (rows, features), contiguous.                                                  */
+enum { UMT_VALUES_F32 = 0, UMT_VALUES_BF16 = 1 };
+typedef struct {
+  int dtype;                       /* UMT_VALUES_*: x, gate, h and their gradients */
+  int t, rows, groups, share;
+  int64_t x_t, x_row, gate_t, gate_row, out_t, out_row;
+  int64_t use_t, use_row, valid_t, valid_row;
+  int64_t dh_t, dh_row, dgate_t, dgate_row;      /* backward only */
+} umt_gated_shape;
+/* float32 states the backward pass starts its stretches from: (ceil(t / UMT_GATED_KEEP), rows * features), the state
+ * before every UMT_GATED_KEEP-th step; kept may be NULL where no backward pass follows */
+#define UMT_GATED_KEEP 16
+int64_t umt_gated_scan_workspace_bytes(const umt_gated_shape* shape);
+int umt_gated_scan(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
+                   const uint8_t* valid, const float* h0, void* h, float* h_last, float* kept, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+/* Gradients of umt_gated_scan for dh (t, rows, features) and dh_last (NULL: zero).  x, gate, the masks and kept as in the
+ * forward call.  dx, dgate (t, rows, groups) and dh0 are written whole; any of them may be NULL.  Skipped frames get
+ * dx = dgate = 0, a dropped memory dgate = 0 and no gradient to what lies before it.                              */
+int64_t umt_gated_scan_backward_workspace_bytes(const umt_gated_shape* shape);
+int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
+                            const uint8_t* valid, const float* kept, const void* dh, const float* dh_last, void* dx,
+                            void* dgate, float* dh0, void* workspace, int64_t workspace_bytes, void* stream);
+/* One frame of the recurrence for `batch` samples over a cache of rows, in place: sample b advances row memory_idx[b] of
+ * state (cache_rows, groups * share; f32) and out (batch, features; dtype) receives the rounded new state.  memory_idx
+ * NULL: sample b is row b.  x (batch, features) and gate (batch, groups) are contiguous; use_memory and valid (batch) or
+ * NULL.  Duplicates in memory_idx all read the same previous row and the highest batch index writes it, as
+ * umt_temporal_step; an index outside the cache runs without memory, writes no row and raises
+ * UMT_STATUS_BAD_MEMORY_IDX in *status (dev int32[1] or NULL).  Rows that no sample names are left as they are.     */
+int64_t umt_gated_step_workspace_bytes(int batch, int cache_rows);
+int umt_gated_step(int dtype, const void* x, const void* gate, const int64_t* memory_idx, const uint8_t* use_memory,
+                   const uint8_t* valid, int batch, int groups, int share, float* state, int cache_rows, void* out,
+                   int32_t* status, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- rows of state caches: the temporal memory of a model handle (umt_model_memory_buffers) and any caches of the
+ * caller that hold one row per hand track (umt_gated_step's state, ...).  The buffers of one call have `rows` rows each
+ * and move together.  buffers is a host array of n_buffers <= UMT_ROW_BUFFERS_MAX entries whose data is dev memory;
+ * they must not overlap.  Row numbers are dev int64; status is dev int32[1] or NULL (UMT_STATUS_BAD_ROW,
+ * UMT_STATUS_NO_FREE_ROW are OR-ed in).  live: dev uint8 (rows), non-zero = in use.                                */
+#define UMT_ROW_BUFFERS_MAX 8
+typedef struct {
+  void* data;                      /* dev, row r at data + r * row_bytes */
+  int64_t row_bytes;
+} umt_row_buffer;
+/* the handle's memory features and previous extrinsics (2 entries; valid until the memory grows) and their rows */
+int umt_model_memory_buffers(const umt_model* m, umt_row_buffer buffers[2], int* rows);
+/* row dst[i] = row src[i] as it was before the call, i < n; of several writes to one row the highest i counts */
+int64_t umt_rows_copy_workspace_bytes(const umt_row_buffer* buffers, int n_buffers, int rows, int n);
+int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int rows, const int64_t* src, const int64_t* dst, int n,
+                  int32_t* status, void* workspace, int64_t workspace_bytes, void* stream);
+/* the sources, in order, take the lowest free rows, in order: ids[i] = the new row (now live) that is a copy of live row
+ * src[i], or -1 (src[i] is not a live row, or no free row is left) */
+int64_t umt_rows_fork_workspace_bytes(int rows, int n);
+int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int rows, uint8_t* live, const int64_t* src, int n,
+                  int64_t* ids, int32_t* status, void* workspace, int64_t workspace_bytes, void* stream);
+/* live[row_ids[i]] = 0; the rows' content stays until a fork or a step overwrites it */
+int umt_rows_free(uint8_t* live, int rows, const int64_t* row_ids, int n, int32_t* status, void* stream);
+/* closes the cache up: with c live rows, the k-th free row below c receives the k-th live row at or above c, so rows
+ * 0..c-1 are the live ones and only the rows that have to move do.  now[r] = the row that holds what row r held, -1 for
+ * a free one; *count = c; live is updated.  Rows at or above c keep their content. */
+int64_t umt_rows_compact_workspace_bytes(int rows);
+int umt_rows_compact(const umt_row_buffer* buffers, int n_buffers, int rows, uint8_t* live, int64_t* now, int64_t* count,
+                     void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,15 +24,35 @@ STATUS_BITS = {1: "use_memory on a memory row whose previous extrinsics are sing
                2: "memory_idx outside the reserved memory rows",
                4: "sample_range row outside [0, n] or not 1 or 2 views",
                8: "a regressor output row was not finite (NaN/inf in the crop, the weights or the state)",
-               16: "a landmark bone index outside [0, 16]"}
+               16: "a landmark bone index outside [0, 16]",
+               32: "a row number outside the cache, or a fork of a free row",
+               64: "no free row left in the cache for a fork"}
 
 STATUS_NONFINITE_OUTPUT = 8
+STATUS_BAD_MEMORY_IDX, STATUS_BAD_ROW, STATUS_NO_FREE_ROW = 2, 32, 64
 # the conditions under which the reference itself raises (torch.inverse on a singular matrix, index errors); a
 # non-finite regressor row is returned as NaN there and the run goes on
 STATUS_RAISING = 1 | 2 | 4 | 16
 
 _ERR_NAMES = {1: "invalid argument", 2: "bad state", 3: "state_dict key", 4: "HIP runtime",
               5: "workspace", 6: "unsupported"}
+
+VALUES_F32, VALUES_BF16 = 0, 1
+GATED_KEEP = 16
+ROW_BUFFERS_MAX = 8
+
+
+class GatedShape(ctypes.Structure):
+    """umt_gated_shape"""
+    _fields_ = ([(n, c_int) for n in ("dtype", "t", "rows", "groups", "share")]
+                + [(n, c_int64) for n in ("x_t", "x_row", "gate_t", "gate_row", "out_t", "out_row", "use_t", "use_row", "valid_t",
+                                          "valid_row", "dh_t", "dh_row", "dgate_t", "dgate_row")])
+
+
+class RowBuffer(ctypes.Structure):
+    """umt_row_buffer"""
+    _fields_ = [("data", c_void_p), ("row_bytes", c_int64)]
+
 
 # name -> (restype, argtypes); kept in the order of include/umetrack_hip.h
 _P = c_void_p
@@ -75,6 +95,20 @@ SIGNATURES = {
     "umt_metric_workspace_bytes": (c_int64, [c_int, c_int]),
     "umt_metric_partials": (c_int, [_P, _P, _P, c_int, c_int, _P, _P, c_int64, _P]),
     "umt_metric_partials_static": (c_int, [_P, _P, _P, c_int, c_int, _P, _P]),
+    "umt_gated_scan_workspace_bytes": (c_int64, [POINTER(GatedShape)]),
+    "umt_gated_scan": (c_int, [POINTER(GatedShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]),
+    "umt_gated_scan_backward_workspace_bytes": (c_int64, [POINTER(GatedShape)]),
+    "umt_gated_scan_backward": (c_int, [POINTER(GatedShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]),
+    "umt_gated_step_workspace_bytes": (c_int64, [c_int, c_int]),
+    "umt_gated_step": (c_int, [c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_int, _P, _P, _P, c_int64, _P]),
+    "umt_model_memory_buffers": (c_int, [_P, POINTER(RowBuffer), POINTER(c_int)]),
+    "umt_rows_copy_workspace_bytes": (c_int64, [POINTER(RowBuffer), c_int, c_int, c_int]),
+    "umt_rows_copy": (c_int, [POINTER(RowBuffer), c_int, c_int, _P, _P, c_int, _P, _P, c_int64, _P]),
+    "umt_rows_fork_workspace_bytes": (c_int64, [c_int, c_int]),
+    "umt_rows_fork": (c_int, [POINTER(RowBuffer), c_int, c_int, _P, _P, c_int, _P, _P, _P, c_int64, _P]),
+    "umt_rows_free": (c_int, [_P, c_int, _P, c_int, _P, _P]),
+    "umt_rows_compact_workspace_bytes": (c_int64, [c_int]),
+    "umt_rows_compact": (c_int, [POINTER(RowBuffer), c_int, c_int, _P, _P, _P, _P, c_int64, _P]),
 }
 METRIC_STATIC_MAX_HAND_FRAMES = 524288
 

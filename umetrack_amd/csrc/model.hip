@@ -1024,6 +1024,14 @@ extern "C" int umt_model_memory_rows(const umt_model* m, int* rows) {
   return 0;
 }
 
+extern "C" int umt_model_memory_buffers(const umt_model* m, umt_row_buffer buffers[2], int* rows) {
+  UMT_REQUIRE(m && buffers && rows, UMT_ERR_INVALID, "null argument");
+  buffers[0] = {m->mem, 18 * 36 * (int64_t)sizeof(float)};
+  buffers[1] = {m->prev_ext, 16 * (int64_t)sizeof(float)};
+  *rows = m->mem_rows;
+  return 0;
+}
+
 extern "C" int umt_model_clear_memory(umt_model* m) {
   UMT_REQUIRE(m, UMT_ERR_INVALID, "null model handle");
   m->mem_rows = 0;   // capacity is kept; rows are re-zeroed when reserved again

@@ -156,6 +156,18 @@ class UmeTrackModel:
             nat.check(L.umt_model_read_memory(self._h, nat.ptr(mem), nat.ptr(prev), nat.stream_ptr(self._device)))
         return mem, prev
 
+    def reserve_memory(self, rows: int) -> None:
+        """At least `rows` temporal memory rows; those added start at zero (temporal.py:102-120)."""
+        with torch.cuda.device(self._device):
+            nat.check(nat.lib().umt_model_reserve_memory(self._h, rows, nat.stream_ptr(self._device)), "umt_model_reserve_memory")
+
+    def memory_buffers(self):
+        """(the handle's two memory buffers as umt_row_buffer entries, rows): what row_cache moves for this model.  The
+        addresses hold until the memory grows."""
+        arr, rows = (nat.RowBuffer * 2)(), ctypes.c_int()
+        nat.check(nat.lib().umt_model_memory_buffers(self._h, arr, ctypes.byref(rows)), "umt_model_memory_buffers")
+        return arr, rows.value
+
     def status(self, clear: bool = True) -> int:
         """The UMT_STATUS_* bits the kernels of this model have raised (one 4-byte copy + stream sync)."""
         word = ctypes.c_int32(0)

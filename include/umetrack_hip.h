@@ -284,7 +284,8 @@ int umt_metric_partials_static(const float* gt, const float* pred, const uint8_t
  *     h[t] = a[t] * h[t-1] + (1 - a[t]) * x[t]                        h[-1] = h0, or 0 where h0 is NULL
  * use_memory[t,row] == 0 drops the memory (h[t] = x[t], whatever h[t-1] holds), valid[t,row] == 0 skips the frame
  * (h[t] = h[t-1]; x and gate of that frame may hold anything, NaN included); both 0 leave h[t] = 0.  Either mask may
- * be NULL (all ones).  A non-finite x, gate or state that no mask excludes makes its feature non-finite (NaN) until the
+ * be NULL (all ones).  Long axes are worked on in stretches, so equal states of different stretches may differ in the
+ * last bits of a float32.  A non-finite x, gate or state that no mask excludes makes its feature non-finite (NaN) until the
  * memory is dropped.  The state is float32 whatever the dtype; h is rounded once, to nearest even.
  *
  * features = groups * share: `share` consecutive features use one gate (a landmark's 3 coordinates, a hand's 63, 1).

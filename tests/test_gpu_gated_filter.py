@@ -87,7 +87,8 @@ def slack(x, gate, h0, valid, T):
 
 SHAPES = [(1, 1, 1, 1), (1, 3, 21, 3), (2, 2, 22, 1), (15, 2, 21, 3), (16, 1, 1, 63), (17, 5, 7, 9), (31, 2, 1, 64), (33, 3, 5, 13),
           (64, 128, 21, 3), (65, 2, 2, 65), (100, 1, 18, 36), (257, 3, 1, 130), (640, 2, 21, 3), (1500, 1, 1, 2), (1025, 2, 3, 5),
-          (48, 700, 63, 2), (5000, 2, 21, 3)]
+          (48, 700, 63, 2), (5000, 2, 21, 3), (33, 100, 1, 1), (2000, 40, 1, 1), (70, 90, 5, 1), (9000, 1, 1, 70), (300, 300, 21, 3),
+          (40, 30, 6, 400)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -143,7 +144,10 @@ def test_every_mask_combination_and_what_lies_under_it():
     got = np64(h)
     assert np.isfinite(got).all() and (np.abs(got - want) <= eh + 2 * U * np.abs(want)).all()
     assert torch.equal(h[:, 0], h0[0].expand(T, 3, 5)) and torch.equal(h[:, 1], x[:, 1])
-    assert bool((h[:, 2] == 0).all()) and torch.equal(h[20:, 6], h[19:20, 6].expand(20, 3, 5)) and torch.equal(last[6], h[19, 6])
+    assert bool((h[:, 2] == 0).all()) and torch.equal(last[6], h[-1, 6])
+    # A skipped frame's exact value is its predecessor's.  Two frames of different stretches reach it by different orders of the
+    # same steps, each within eh of it, so they lie within 2 eh of each other; within a stretch they are the same bits.
+    assert float((h[20:, 6] - h[19:20, 6]).abs().max()) <= 2 * eh and torch.equal(h[32:, 6], h[32:33, 6].expand(8, 3, 5))
 
 
 def test_gates_at_their_ends_and_a_poisoned_memory():
@@ -239,7 +243,7 @@ def test_strides_offsets_and_broadcast_gates():
         h, _ = _gf().gated_scan(y, one.expand(T, R, 1))
         dh = torch.randn(T, R, G, K, device="cuda").to(dt)
         (got,) = torch.autograd.grad(h, one, dh)
-        *_, want, _, s = oracle(np64(y).reshape(T, R, 1, G * K), np.full((T, R, 1), float(one)), None, None, None,
+        *_, want, _, s = oracle(np64(y).reshape(T, R, 1, G * K), np.full((T, R, 1), float(one.detach())), None, None, None,
                                 np64(dh).reshape(T, R, 1, G * K))
         # T R slopes rounded to the type, then summed by torch and rounded again
         tol = 2 * torch.finfo(dt).eps * np.abs(want).sum() + 40 * U * np.abs(want).sum() + 2.0 ** -16 * T * R
@@ -252,7 +256,10 @@ def test_only_the_gradients_that_are_asked_for():
     h, last = _gf().gated_scan(xg, gate, h0, use, valid)
     (a,) = torch.autograd.grad(last.sum(), xg, retain_graph=True)
     (b,) = torch.autograd.grad(h[-1].sum(), xg)
-    assert torch.equal(a, b)
+    # the same gradient, which enters the last stretch from behind or at its last step: two orders of the same steps, each
+    # within 6 u S K + 4 u S of it, and S = 1 here
+    _, _, kk = slack(x, gate, h0, valid, 70)
+    assert float((a - b).abs().max()) <= 2 * (6 * U * kk + 4 * U)
     h, last, kept = _gf().gated_scan(x, gate, h0, use, valid, keep=True)
     dh = torch.randn_like(h)
     full = _gf().gated_scan_backward(x, gate, kept, dh, None, use, valid)
@@ -289,6 +296,59 @@ def test_offsets_past_32_bits():
     h, last = _gf().gated_scan(x, gate)
     ref, rl = _gf().gated_scan(vals, gate)
     assert torch.equal(h, ref) and torch.equal(last, rl)
+
+
+def test_rows_further_apart_than_32_bits():
+    """Rows 2^30 + 5 elements apart, their features two wide: a wave holds values of all three rows."""
+    far = (1 << 30) + 5
+    big = torch.empty(2 * far + 4096, dtype=torch.float32, device="cuda")
+    for T in (5, 900):
+        x = big.as_strided((T, 3, 2), (2, far, 1))
+        vals = torch.randn(T, 3, 2, device="cuda")
+        x.copy_(vals)
+        gate, valid = torch.randn(T, 3, 2, device="cuda"), torch.rand(T, 3, device="cuda") > 0.3
+        h, last, kept = _gf().gated_scan(x, gate, valid=valid, keep=True)
+        ref, rl, rk = _gf().gated_scan(vals, gate, valid=valid, keep=True)
+        assert torch.equal(h, ref) and torch.equal(last, rl) and torch.equal(kept, rk)
+        dh = torch.randn(T, 3, 2, device="cuda")
+        for a, b in zip(_gf().gated_scan_backward(x, gate, kept, dh, valid=valid), _gf().gated_scan_backward(vals, gate, rk, dh, valid=valid)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [700, 6000, 20011])
+def test_masks_across_stretches_and_segments(T):
+    """Long runs of skipped frames, a memory dropped once in a long while, NaN memory dropped late, NaN below every mask."""
+    R, G, K = 4, 5, 3
+    x, gate, h0, _, _ = make(T, R, G, K, "fp32", T, masks=False)
+    gate += 3
+    gate[:, 2] = 12.0
+    use, valid = (torch.ones(T, R, dtype=torch.bool, device="cuda") for _ in range(2))
+    valid[T // 7:T - 5, 0] = False
+    use[[0, T // 3, T // 3 + 1, T - 1], 1] = False
+    valid[::3, 2] = False
+    use[T // 2, 3] = False
+    valid[T // 2 + 1:, 3] = False
+    use[1, 2] = False
+    h0[1] = float("nan")
+    h0[2] = float("inf")
+    valid[0, 2], use[0, 2] = False, False
+    x[~valid] = float("nan")
+    gate[~valid] = float("nan")
+    for t in (x, gate, h0):
+        t.requires_grad_(True)
+    g = torch.Generator().manual_seed(1)
+    dh, dl = torch.randn(T, R, G, K, generator=g).cuda(), torch.randn(R, G, K, generator=g).cuda()
+    h, last = _gf().gated_scan(x, gate, h0, use, valid)
+    got = (h, last) + torch.autograd.grad((h, last), (x, gate, h0), (dh, dl))
+    h0d = np.nan_to_num(np64(h0), nan=0, posinf=0)
+    ref = oracle(np64(x), np64(gate), h0d, np64(use), np64(valid), np64(dh), np64(dl))
+    eh, M, kk = slack(x, gate, torch.from_numpy(h0d), valid, T)
+    S = np.abs(ref[5]).max()
+    es = 6 * U * S * kk
+    tols = (eh, eh, es + 4 * U * S, K * 0.25 * (S * (eh + 4 * U * M) + 2 * M * es + 12 * U * S * 2 * M), es)
+    for name, a, b, tol in zip(("h", "last", "dx", "dgate", "dh0"), got, ref, tols):
+        a = np64(a)
+        assert np.isfinite(a).all() and (np.abs(a - b) <= tol + 2 * U * np.abs(b)).all(), name
 
 
 def test_other_stream_and_graph_replays():

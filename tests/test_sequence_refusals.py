@@ -49,6 +49,8 @@ def test_scan_pointers_and_workspaces():
     assert need > 0
     assert L.umt_gated_scan_backward(wide, P, P, None, None, P, P, None, P, P, None, P, need - 1, None) == 5
     assert L.umt_gated_scan_backward(wide, P, P, None, None, P, P, None, P, P, None, None, need, None) == 5
+    for empty in (dict(t=0), dict(rows=0), dict(t=0, rows=0)):
+        assert L.umt_gated_scan_workspace_bytes(shape(**empty)) == 0 and L.umt_gated_scan_backward_workspace_bytes(shape(**empty)) == 0
     assert L.umt_gated_scan(shape(rows=0), None, None, None, None, None, None, None, None, None, 0, None) == 0
 
 

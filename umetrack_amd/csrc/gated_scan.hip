@@ -2,106 +2,341 @@
 //
 //   h[t] = a h[t-1] + c x[t],   a = sigmoid(gate), c = 1 - a = sigmoid(-gate)
 //
-// One lane owns one (row, feature) and walks the time axis in stretches of UMT_GATED_KEEP steps whose loads are all in
-// flight together; neighbouring lanes are neighbouring features, so every load of a wave is one run of memory.  There is
-// nothing to reuse: the passes are bound by HBM once enough loads are in flight.
+// One lane owns one (row, feature); a wave loads UMT_GATED_KEEP steps of its 64 lanes at once, so neighbouring lanes read
+// neighbouring features and 32 loads are in flight.  Where there are many lanes a wave walks the whole axis alone.  Where
+// there are few, the waves of a workgroup take successive stretches of a tile (the recurrence over a stretch is itself a
+// step, see join()), and beyond that the axis is cut into segments that workgroups of their own run, whose steps a first
+// launch finds.  No order of arrival enters a result.
 //
 // Arithmetic.  With e = exp(-|gate|) the smaller of (a, c) is m = e / (1 + e), which keeps its relative precision however
 // small it gets, and the larger one is 1 - m.  A step is base + m (other - base), where base is what the larger weight
 // belongs to: one fma, and neither a slow decay (a near 1) nor the remainder of an old outlier (a near 0) is lost in
-// 1 - m.  The sign bit of the stored m says which one the base is (set: the input).  m = 0 returns the base itself, so
-// a masked frame or a dropped memory passes through exactly, whatever the other operand holds.
+// 1 - m.  The sign bit of the stored m says which one the base is (set: the input).  A frame that is skipped is the step
+// (x, m) = (0, +0), a dropped memory is m = -0 with the memory read as 0, so what lies under a mask enters nowhere.
 #include "umt_internal.h"
+
+#include <type_traits>
 
 namespace umt {
 
 constexpr int KEEP = UMT_GATED_KEEP;
 constexpr int GT = 256;
 
+__device__ __forceinline__ float as_value(float v) { return v; }
+__device__ __forceinline__ float as_value(__bf16 v) { return (float)v; }
 __device__ __forceinline__ float load_value(const float* p) { return *p; }
 __device__ __forceinline__ float load_value(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_value(__bf16* p, float v) { *p = (__bf16)v; }   // one rounding, to nearest even
 
-// exp(-|g|) as exp2 of a product in two pieces: the first product's rounding, up to |g| 2^-24 of the result, is put back
+// The stored m of a gate.  exp2 of the rounded product |gate| log2(e) is off by up to |gate| + 2 units of 2^-24 relative,
+// and as m <= exp(-|gate|) that is at most 1.5 such units absolute: less than the rounding of the state in the same step.
 __device__ __forceinline__ float gate_step(float g) {
-  const float n = -fabsf(g);
-  const float p = n * 1.44269504f;
-  const float rest = fmaf(n, 1.44269504f, -p) + n * 1.925963e-8f;      // log2(e) = 1.44269504 + 1.9e-8
-  const float e0 = __builtin_amdgcn_exp2f(p);
-  const float e = e0 > 0.f ? fmaf(e0 * 0.6931472f, rest, e0) : e0;     // gate = +-inf or far: rest may be NaN
+  const float e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
   return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
 
 __device__ __forceinline__ float advance(float h, float x, float m) {
   const bool from_x = __float_as_uint(m) >> 31;
-  const float am = fabsf(m), base = from_x ? x : h, other = from_x ? h : x;
-  return am == 0.f ? base : fmaf(am, other - base, base);
+  const float base = from_x ? x : h, other = from_x ? h : x;
+  return fmaf(fabsf(m), other - base, base);
 }
 
-// the step a mask asks for: hold = (x 0, m +0), drop = (x, m -0), both = (0, -0)
-__device__ __forceinline__ void masked(bool use, bool valid, float& x, float& m) {
-  x = valid ? x : 0.f;
-  m = use ? (valid ? m : 0.f) : -0.f;
+// all ones where bit j is set
+__device__ __forceinline__ unsigned bit_mask(unsigned bits, int j) { return (unsigned)((int)(bits << (31 - j)) >> 31); }
+__device__ __forceinline__ float masked_value(float v, unsigned mask) { return __uint_as_float(__float_as_uint(v) & mask); }
+// the m of a masked step: keeps its value, +0 (skipped) or -0 (memory dropped)
+__device__ __forceinline__ float masked_step(float m, unsigned use, unsigned valid) {
+  return __uint_as_float((__float_as_uint(m) & valid & use) | (~use & 0x80000000u));
 }
 
-// backward factors of a step: c s, a s and c a for the stored m (masks folded in: m = +-0)
-__device__ __forceinline__ float times_c(float m, float s) { return __float_as_uint(m) >> 31 ? fmaf(m, s, s) : m * s; }
-__device__ __forceinline__ float times_a(float m, float s) { return __float_as_uint(m) >> 31 ? -m * s : fmaf(-m, s, s); }
+// backward factors of a step: c s and a s for the stored m
+__device__ __forceinline__ float times_c(float m, float s) {
+  const float p = fabsf(m) * s;
+  return __float_as_uint(m) >> 31 ? s - p : p;
+}
+__device__ __forceinline__ float times_a(float m, float s) {
+  const float p = fabsf(m) * s;
+  return __float_as_uint(m) >> 31 ? p : s - p;
+}
 
 struct Masks {
   const uint8_t* use;
   const uint8_t* valid;
 };
 
-// bits of one lane's stretch: bit j = mask[(t0 + j), row], steps past the end read as the last one
-__device__ __forceinline__ unsigned mask_bits(const uint8_t* p, int64_t st, int t0, int T) {
-  unsigned bits = 0;
-#pragma unroll
-  for (int j = 0; j < KEEP; ++j) {
-    const int t = min(t0 + j, T - 1);
-    bits |= (p[t * st] ? 1u : 0u) << j;
-  }
-  return bits;
+// A stretch of steps is a step itself: h_out = p + a h_in, with q = 1 - a carried on its own (the stretch's response to a
+// memory of 0 and inputs of 1), because 1 - a of a rounded a has lost a slow decay.
+struct Stretch {
+  float a, q, p;
+};
+__device__ __forceinline__ float join(float h, const Stretch& s) {
+  const float slow = h + fmaf(-s.q, h, s.p), fast = fmaf(s.a, h, s.p);
+  return s.a == 0.f ? s.p : s.q <= 0.5f ? slow : fast;      // a = 0: the memory was dropped on the way, whatever h holds
+}
+__device__ __forceinline__ Stretch then(const Stretch& f, const Stretch& s) {
+  return Stretch{f.a * s.a, join(f.q, Stretch{s.a, s.q, s.q}), join(f.p, s)};
 }
 
-template <typename V>
-__global__ __launch_bounds__(GT) void gated_scan_kernel(umt_gated_shape S, const V* __restrict__ x, const V* __restrict__ gate,
-                                                        Masks mk, const float* __restrict__ h0, V* __restrict__ h,
-                                                        float* __restrict__ h_last, float* __restrict__ kept) {
-  const int F = S.groups * S.share;
-  const int64_t N = (int64_t)S.rows * F;
-  const int64_t e = (int64_t)blockIdx.x * GT + threadIdx.x;
-  if (e >= N) return;
-  const int64_t row = e / F;
-  const int f = (int)(e - row * F);
-  const V* xp = x + row * S.x_row + f;
-  const V* gp = gate + row * S.gate_row + f / S.share;
-  V* hp = h + row * S.out_row + f;
-  const uint8_t* up = mk.use ? mk.use + row * S.use_row : nullptr;
-  const uint8_t* vp = mk.valid ? mk.valid + row * S.valid_row : nullptr;
-  float cur = h0 ? h0[e] : 0.f;
-  for (int t0 = 0; t0 < S.t; t0 += KEEP) {
-    float xs[KEEP], ms[KEEP];
-#pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-      const int t = min(t0 + j, S.t - 1);
-      xs[j] = load_value(xp + t * S.x_t);
-      ms[j] = load_value(gp + t * S.gate_t);
+// One stream of (t, row, feature) values as a wave addresses it: the step's place is the same in all lanes, a lane adds
+// its distance from the wave's first row (OFF = 32 bits unless the rows lie further apart than that)
+template <typename V, typename OFF>
+struct Lanes {
+  const V* at;             // step 0 of the wave's first row
+  int64_t step;
+  OFF mine;                // in bytes
+  __device__ __forceinline__ V load(int64_t t) const {
+    return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(at + t * step) + mine);
+  }
+};
+
+// Frame masks of KEEP steps, one bit a step.  Lane 16 k + j reads the byte of step j of the wave's row r0 + k and a ballot
+// hands every lane the 16 bits of its own row: one load a stretch where a wave holds up to 4 rows, more only where the
+// rows are shorter than that.
+struct MaskLanes {
+  const uint8_t* p;
+  int64_t st, sr, r0;
+  int rows, span, mine;    // rows of the call, rows of the wave, this lane's row among them
+  __device__ __forceinline__ uint8_t fetch(int t0, int T, int k0) const {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = r0 + k0 + (lane >> 4);
+    const int t = t0 + (lane & 15);
+    return p[(int64_t)(t < T ? t : T - 1) * st + (r < rows ? r : rows - 1) * sr];
+  }
+  // `first` = fetch(t0, T, 0), made ahead
+  __device__ __forceinline__ unsigned bits(uint8_t first, int t0, int T) const {
+    unsigned b = 0;
+    for (int k0 = 0; k0 < span; k0 += 4) {
+      const uint64_t all = __ballot((k0 ? fetch(t0, T, k0) : first) != 0);
+      if ((mine >> 2) == (k0 >> 2)) b = (unsigned)(all >> (16 * (mine & 3))) & 0xffffu;
     }
-    const unsigned ub = up ? mask_bits(up, S.use_t, t0, S.t) : ~0u, vb = vp ? mask_bits(vp, S.valid_t, t0, S.t) : ~0u;
-    if (kept) kept[(int64_t)(t0 / KEEP) * N + e] = cur;
+    return b;
+  }
+};
+
+// What one wave of the forward direction works on
+template <typename V, typename OFF, bool MASK>
+struct Walk {
+  Lanes<V, OFF> x, g;
+  MaskLanes um, vm;
+  bool has_use, has_valid;
+  int T;
+  V rx[KEEP], rg[KEEP];
+  uint8_t ru, rv;
+
+  // e0: first element of the wave, e: this lane's (clamped into the call)
+  __device__ __forceinline__ void place(const umt_gated_shape& S, const V* x_, const V* gate_, const Masks& mk, int64_t row0, int64_t row,
+                                        int f, int gi, int64_t x_t, int64_t x_row) {
+    T = S.t;
+    x = {x_ + row0 * x_row, x_t, (OFF)(((row - row0) * x_row + f) * (int64_t)sizeof(V))};
+    g = {gate_ + row0 * S.gate_row, S.gate_t, (OFF)(((row - row0) * S.gate_row + gi) * (int64_t)sizeof(V))};
+    if (MASK) {
+      const int mine = (int)(row - row0), span = __builtin_amdgcn_readfirstlane(wave_max(mine)) + 1;
+      has_use = mk.use != nullptr;
+      has_valid = mk.valid != nullptr;
+      um = {mk.use, S.use_t, S.use_row, row0, S.rows, span, mine};
+      vm = {mk.valid, S.valid_t, S.valid_row, row0, S.rows, span, mine};
+    }
+  }
+  static __device__ __forceinline__ int wave_max(int v) {
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+    return v;
+  }
+  __device__ __forceinline__ void fetch(int t0) {
+    if (MASK) {
+      if (has_use) ru = um.fetch(t0, T, 0);
+      if (has_valid) rv = vm.fetch(t0, T, 0);
+    }
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-      float m = gate_step(ms[j]);
-      masked(ub >> j & 1, vb >> j & 1, xs[j], m);
-      if (t0 + j < S.t) {
-        cur = advance(cur, xs[j], m);
-        store_value(hp + (t0 + j) * S.out_t, cur);
+      const int t = t0 + j < T ? t0 + j : T - 1;
+      rg[j] = g.load(t);
+      rx[j] = x.load(t);
+    }
+  }
+  // the fetched stretch: inputs, m of each step, mask bits (steps past the end are skipped frames)
+  // back: xs are gradients, which no valid mask covers
+  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP], float (&ms)[KEEP], unsigned& ub, unsigned& vb, bool back) {
+    ub = vb = 0xffffu;
+    if (MASK) {
+      if (has_use) ub = um.bits(ru, t0, T);
+      if (has_valid) vb = vm.bits(rv, t0, T);
+    }
+    const int left = T - t0;
+    unsigned past = 0;
+    if (left < KEEP) {
+      past = left <= 0 ? 0xffffu : 0xffffu << left & 0xffffu;
+      ub |= past;
+      vb &= ~past;
+    }
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      xs[j] = as_value(rx[j]);
+      ms[j] = gate_step(as_value(rg[j]));
+    }
+    if (MASK || left < KEEP) {
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) {
+        const unsigned v = bit_mask(vb, j);
+        xs[j] = masked_value(xs[j], back ? ~bit_mask(past, j) : v);
+        ms[j] = masked_step(ms[j], bit_mask(ub, j), v);
       }
     }
   }
-  if (h_last) h_last[e] = cur;
+};
+
+template <bool MASK>
+__device__ __forceinline__ float memory_of(float h, unsigned ub, int j) {
+  return MASK ? masked_value(h, bit_mask(ub, j)) : h;
+}
+
+// Partners: the W waves of a workgroup take the KEEP-step stretches of a tile in turn; each hands its stretch over in LDS and
+// joins those before it (after it, in the backward direction) to the state that entered the tile.
+template <int W>
+struct Partners {
+  float (*lds)[W][3][64];
+  int turn = 0;
+  // state before this wave's stretch; `through` becomes the state behind the tile
+  template <bool BACK>
+  __device__ __forceinline__ float enter(const Stretch& mine, int tw, int lane, float& through) {
+    float(*b)[3][64] = lds[turn];
+    turn ^= 1;                              // two places: one barrier a tile
+    b[tw][0][lane] = mine.a;
+    b[tw][1][lane] = mine.q;
+    b[tw][2][lane] = mine.p;
+    __syncthreads();
+    float cur = through, own = through;
+    for (int i = 0; i < W; ++i) {
+      const int w = BACK ? W - 1 - i : i;
+      if (w == tw) own = cur;
+      cur = join(cur, Stretch{b[w][0][lane], b[w][1][lane], b[w][2][lane]});
+    }
+    through = cur;
+    return own;
+  }
+};
+
+template <int W>
+constexpr int group_threads() { return W == 1 ? GT : 64 * W; }
+
+// the joined segments before (after) this one, [segment][a, q, p][lane] in `segs`: the waves join a run of them each
+template <int W, bool BACK>
+__device__ __forceinline__ float enter_segment(const float* __restrict__ segs, int seg, int n_segs, int64_t n, int64_t e, int tw, int lane,
+                                               float first, Partners<W>& partners) {
+  const int count = BACK ? n_segs - 1 - seg : seg, per = (count + W - 1) / W;
+  const int a0 = min(count, tw * per), a1 = min(count, a0 + per);
+  Stretch run{1.f, 0.f, 0.f};
+  for (int i = a0; i < a1; ++i) {
+    const float* s = segs + (int64_t)(BACK ? n_segs - 1 - i : i) * 3 * n + e;
+    run = then(run, Stretch{s[0], s[n], s[2 * n]});
+  }
+  float through = first;
+  partners.template enter<false>(run, tw, lane, through);
+  return through;
+}
+
+template <typename V, typename OFF, int W, bool MASK>
+__global__ __launch_bounds__(group_threads<W>()) void gated_scan_kernel(umt_gated_shape S, const V* __restrict__ x, const V* __restrict__ gate,
+                                                                        Masks mk, const float* __restrict__ h0, const float* __restrict__ segs,
+                                                                        int seg_tiles, V* __restrict__ h, float* __restrict__ h_last,
+                                                                        float* __restrict__ kept) {
+  __shared__ float lds[W > 1 ? 2 : 1][W][3][64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int F = S.groups * S.share;
+  const int64_t N = (int64_t)S.rows * F;
+  const int64_t e0 = W == 1 ? ((int64_t)blockIdx.x * (GT / 64) + wv) * 64 : (int64_t)blockIdx.x * 64;
+  const int tw = W == 1 ? 0 : wv;
+  if (W == 1 && e0 >= N) return;
+  const int64_t e = e0 + lane < N ? e0 + lane : N - 1;
+  const bool on = e0 + lane < N;
+  const int64_t row0 = e0 / F, row = e / F;
+  const int f = (int)(e - row * F);
+  Walk<V, OFF, MASK> w;
+  w.place(S, x, gate, mk, row0, row, f, f / S.share, S.x_t, S.x_row);
+  char* hp = reinterpret_cast<char*>(h + row0 * S.out_row);
+  const OFF mine = (OFF)(((row - row0) * S.out_row + f) * (int64_t)sizeof(V));
+  const int tiles = (S.t + KEEP * W - 1) / (KEEP * W);
+  const int tile0 = blockIdx.y * seg_tiles, tile1 = min(tiles, tile0 + seg_tiles);
+  w.fetch((tile0 * W + tw) * KEEP);
+  float cur = h0 ? h0[e] : 0.f;
+  Partners<W> partners{reinterpret_cast<float(*)[W][3][64]>(lds)};
+  if (W > 1 && segs) cur = enter_segment<W, false>(segs, blockIdx.y, gridDim.y, N, e, tw, lane, cur, partners);
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int t0 = (tile * W + tw) * KEEP;
+    float xs[KEEP], ms[KEEP];
+    unsigned ub, vb;
+    w.take(t0, xs, ms, ub, vb, false);
+    if (tile + 1 < tile1) w.fetch(t0 + W * KEEP);
+    float st = cur;
+    if (W > 1) {
+      Stretch own{1.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) {
+        own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
+        own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
+        own.p = advance(memory_of<MASK>(own.p, ub, j), xs[j], ms[j]);
+      }
+      st = partners.template enter<false>(own, tw, lane, cur);
+      if (t0 >= S.t) continue;
+    }
+    if (kept && on) kept[(int64_t)(t0 / KEEP) * N + e] = st;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      st = advance(memory_of<MASK>(st, ub, j), xs[j], ms[j]);
+      if (on && t0 + j < S.t) store_value(reinterpret_cast<V*>(hp + (int64_t)(t0 + j) * S.out_t * (int64_t)sizeof(V) + mine), st);
+    }
+    if (h_last && on && t0 + KEEP >= S.t) h_last[e] = st;
+    if (W == 1) cur = st;
+  }
+}
+
+// The steps that the first segments make of the state (of the gradient that enters from behind, for the last segments):
+// a wave walks its share of the segment alone, the waves' stretches are joined at the end.
+template <typename V, typename OFF, int W, bool MASK, bool BACK>
+__global__ __launch_bounds__(64 * W) void gated_segment_kernel(umt_gated_shape S, const V* __restrict__ v, const V* __restrict__ gate, Masks mk,
+                                                               int seg_tiles, int64_t v_t, int64_t v_row, float* __restrict__ segs) {
+  __shared__ float lds[W][3][64];
+  const int lane = threadIdx.x & 63, tw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int F = S.groups * S.share;
+  const int64_t N = (int64_t)S.rows * F;
+  const int64_t e0 = (int64_t)blockIdx.x * 64;
+  const int64_t e = e0 + lane < N ? e0 + lane : N - 1;
+  const int64_t row0 = e0 / F, row = e / F;
+  const int f = (int)(e - row * F);
+  Walk<V, OFF, MASK> w;
+  w.place(S, v, gate, mk, row0, row, f, f / S.share, v_t, v_row);
+  const int seg = blockIdx.y + (BACK ? 1 : 0);
+  const int c0 = (seg * W + tw) * seg_tiles;               // stretches of this wave: c0 .. c0 + seg_tiles - 1
+  Stretch own{1.f, 0.f, 0.f};
+  w.fetch((BACK ? c0 + seg_tiles - 1 : c0) * KEEP);
+  for (int k = 0; k < seg_tiles; ++k) {
+    const int t0 = (BACK ? c0 + seg_tiles - 1 - k : c0 + k) * KEEP;
+    float xs[KEEP], ms[KEEP];
+    unsigned ub, vb;
+    w.take(t0, xs, ms, ub, vb, BACK);
+    if (k + 1 < seg_tiles) w.fetch(BACK ? t0 - KEEP : t0 + KEEP);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int j = BACK ? KEEP - 1 - i : i;
+      own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
+      own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
+      own.p = BACK ? memory_of<MASK>(times_a(ms[j], xs[j] + own.p), ub, j) : advance(memory_of<MASK>(own.p, ub, j), xs[j], ms[j]);
+    }
+  }
+  lds[tw][0][lane] = own.a;
+  lds[tw][1][lane] = own.q;
+  lds[tw][2][lane] = own.p;
+  __syncthreads();
+  if (tw != 0 || e0 + lane >= N) return;
+  Stretch all{1.f, 0.f, 0.f};
+  for (int i = 0; i < W; ++i) {
+    const int k = BACK ? W - 1 - i : i;
+    all = then(all, Stretch{lds[k][0][lane], lds[k][1][lane], lds[k][2][lane]});
+  }
+  float* o = segs + (int64_t)seg * 3 * N + e;
+  o[0] = all.a;
+  o[N] = all.q;
+  o[2 * N] = all.p;
 }
 
 // Which features the lanes of a backward wave own.  share = 1: 64 in a row.  share <= 64: as many whole groups as fit, so
@@ -135,75 +370,91 @@ __device__ __forceinline__ float group_sum(float v, int pos, int len) {
   return v;
 }
 
-template <typename V>
-__global__ __launch_bounds__(GT) void gated_scan_backward_kernel(umt_gated_shape S, LaneMap L, const V* __restrict__ x,
-                                                                 const V* __restrict__ gate, Masks mk,
-                                                                 const float* __restrict__ kept, const V* __restrict__ dh,
-                                                                 const float* __restrict__ dh_last, V* __restrict__ dx,
-                                                                 V* __restrict__ dgate, float* __restrict__ part,
-                                                                 float* __restrict__ dh0) {
-  const int lane = threadIdx.x & 63;
-  const int64_t wave = (int64_t)blockIdx.x * (GT / 64) + (threadIdx.x >> 6);
+template <typename V, typename OFF, int W, bool MASK>
+__global__ __launch_bounds__(group_threads<W>()) void gated_scan_backward_kernel(
+    umt_gated_shape S, LaneMap L, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
+    const V* __restrict__ dh, const float* __restrict__ dh_last, const float* __restrict__ segs, int seg_tiles, V* __restrict__ dx,
+    V* __restrict__ dgate, float* __restrict__ part, float* __restrict__ dh0) {
+  __shared__ float lds[W > 1 ? 2 : 1][W][3][64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t wave = W == 1 ? (int64_t)blockIdx.x * (GT / 64) + wv : blockIdx.x;
+  const int tw = W == 1 ? 0 : wv;
   if (wave >= L.waves) return;
   const int F = S.groups * S.share;
   const int64_t N = (int64_t)S.rows * F, G = (int64_t)S.rows * S.groups;
-  int64_t group;
-  int pos, len, first;                     // place in the group or piece, its length, feature of the piece's start in the group
+  // the wave's first group, and this lane's place in its group or piece
+  int64_t group0, group;
+  int pos, len, first;                     // place, length, and the feature of the group at which the piece starts
   if (L.pieces > 1) {
-    group = wave / L.pieces;
+    group0 = group = wave / L.pieces;
     first = (int)(wave - group * L.pieces) * L.width;
     len = min(L.width, S.share - first);
     pos = lane;
   } else {
-    group = wave * L.groups_per_wave + lane / S.share;
+    group0 = wave * L.groups_per_wave;
+    group = group0 + lane / S.share;
     first = 0;
     len = S.share;
     pos = lane % S.share;
   }
   const bool on = pos < len && group < G && (L.pieces > 1 || lane < L.groups_per_wave * S.share);
-  group = on ? group : G - 1;
-  const int inner = on ? first + pos : S.share - 1;
-  const int64_t row = group / S.groups;
+  group = on ? group : group0;
+  const int64_t row0 = group0 / S.groups, row = group / S.groups;
   const int gi = (int)(group - row * S.groups);
-  const int f = gi * S.share + inner;
+  const int f = gi * S.share + (on ? first + pos : first);
   const int64_t e = row * F + f;
-  const V* xp = x + row * S.x_row + f;
-  const V* gp = gate + row * S.gate_row + gi;
-  const V* dp = dh + row * S.dh_row + f;
-  V* dxp = dx ? dx + row * S.out_row + f : nullptr;
-  const uint8_t* up = mk.use ? mk.use + row * S.use_row : nullptr;
-  const uint8_t* vp = mk.valid ? mk.valid + row * S.valid_row : nullptr;
+  Walk<V, OFF, MASK> w;
+  w.place(S, x, gate, mk, row0, row, f, gi, S.x_t, S.x_row);
+  const Lanes<V, OFF> d{dh + row0 * S.dh_row, S.dh_t, (OFF)(((row - row0) * S.dh_row + f) * (int64_t)sizeof(V))};
+  char* dxp = dx ? reinterpret_cast<char*>(dx + row0 * S.out_row) : nullptr;
+  const OFF mine = (OFF)(((row - row0) * S.out_row + f) * (int64_t)sizeof(V));
+  const int tiles = (S.t + KEEP * W - 1) / (KEEP * W);
+  const int tile0 = blockIdx.y * seg_tiles, tile1 = min(tiles, tile0 + seg_tiles);
+  Partners<W> partners{reinterpret_cast<float(*)[W][3][64]>(lds)};
   float v = dh_last ? dh_last[e] : 0.f;
-  for (int t0 = (S.t - 1) / KEEP * KEEP; t0 >= 0; t0 -= KEEP) {
+  if (W > 1 && segs) v = enter_segment<W, true>(segs, blockIdx.y, gridDim.y, N, e, tw, lane, v, partners);
+  for (int tile = tile1 - 1; tile >= tile0; --tile) {
+    const int t0 = (tile * W + tw) * KEEP;
     float q[KEEP], ms[KEEP], ds[KEEP];
+    unsigned ub, vb;
+    w.fetch(t0);
+    V rd[KEEP];
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-      const int t = min(t0 + j, S.t - 1);
-      q[j] = load_value(xp + t * S.x_t);
-      ms[j] = load_value(gp + t * S.gate_t);
-      ds[j] = load_value(dp + t * S.dh_t);
+    for (int j = 0; j < KEEP; ++j) rd[j] = d.load(t0 + j < S.t ? t0 + j : S.t - 1);
+    float cur = t0 < S.t ? kept[(int64_t)(t0 / KEEP) * N + e] : 0.f;
+    w.take(t0, q, ms, ub, vb, false);
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {        // the states again; q becomes c a (h[t-1] - x[t]), the slope over the gate
+      const float am = fabsf(ms[j]), xv = q[j];
+      cur = memory_of<MASK>(cur, ub, j);
+      q[j] = fmaf(-am, am, am) * (cur - xv);
+      if (MASK) q[j] = masked_value(q[j], bit_mask(ub & vb, j));
+      cur = advance(cur, xv, ms[j]);
+      ds[j] = t0 + j < S.t ? as_value(rd[j]) : 0.f;
     }
-    const unsigned ub = up ? mask_bits(up, S.use_t, t0, S.t) : ~0u, vb = vp ? mask_bits(vp, S.valid_t, t0, S.t) : ~0u;
-    float cur = kept[(int64_t)(t0 / KEEP) * N + e];
+    float b = v;
+    if (W > 1) {
+      Stretch own{1.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {       // the states again; q becomes c a (h[t-1] - x[t]), the slope over the gate
-      float m = gate_step(ms[j]), xv = q[j];
-      masked(ub >> j & 1, vb >> j & 1, xv, m);
-      const float am = fabsf(m);
-      q[j] = am == 0.f ? 0.f : fmaf(-am, am, am) * (cur - xv);
-      cur = advance(cur, xv, m);
-      ms[j] = m;
+      for (int j = KEEP - 1; j >= 0; --j) {
+        own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
+        own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
+        own.p = memory_of<MASK>(times_a(ms[j], ds[j] + own.p), ub, j);
+      }
+      b = partners.template enter<true>(own, tw, lane, v);
+      if (t0 >= S.t) continue;
     }
 #pragma unroll
     for (int j = KEEP - 1; j >= 0; --j) {
       const int t = t0 + j;
       if (t >= S.t) continue;
-      const float s = ds[j] + v;
-      const float gx = (vb >> j & 1) ? times_c(ms[j], s) : 0.f;
-      v = (ms[j] == 0.f && __float_as_uint(ms[j]) >> 31) ? 0.f : times_a(ms[j], s);
-      if (on && dxp) store_value(dxp + t * S.out_t, gx);
+      const float s = ds[j] + b;
+      const float gx = masked_value(times_c(ms[j], s), MASK ? bit_mask(vb, j) : ~0u);
+      b = memory_of<MASK>(times_a(ms[j], s), ub, j);
+      if (on && dxp) store_value(reinterpret_cast<V*>(dxp + (int64_t)t * S.out_t * (int64_t)sizeof(V) + mine), gx);
       if (dgate) {
-        const float sum = group_sum(on && q[j] != 0.f ? s * q[j] : 0.f, pos, len);
+        const float slope = s * q[j];
+        const float sum = group_sum(on && (!MASK || (ub & vb) >> j & 1) ? slope : 0.f, pos, len);
         if (on && pos == 0) {
           if (L.pieces > 1)
             part[((int64_t)t * G + group) * L.pieces + (wave - group * L.pieces)] = sum;
@@ -212,8 +463,9 @@ __global__ __launch_bounds__(GT) void gated_scan_backward_kernel(umt_gated_shape
         }
       }
     }
+    if (on && dh0 && t0 == 0) dh0[e] = b;
+    if (W == 1) v = b;
   }
-  if (on && dh0) dh0[e] = v;
 }
 
 template <typename V>
@@ -263,10 +515,10 @@ struct StepArgs {
 template <typename V>
 __device__ __forceinline__ float step_one(const StepArgs& A, const V* x, const V* gate, V* out, int b, int f, float prev, bool has_row) {
   const int F = A.groups * A.share;
-  float xv = load_value(x + (int64_t)b * F + f);
-  float m = gate_step(load_value(gate + (int64_t)b * A.groups + f / A.share));
-  masked(has_row && (!A.use || A.use[b]), !A.valid || A.valid[b], xv, m);
-  const float hv = advance(prev, xv, m);
+  const unsigned use = has_row && (!A.use || A.use[b]) ? ~0u : 0u, valid = !A.valid || A.valid[b] ? ~0u : 0u;
+  const float xv = masked_value(load_value(x + (int64_t)b * F + f), valid);
+  const float m = masked_step(gate_step(load_value(gate + (int64_t)b * A.groups + f / A.share)), use, valid);
+  const float hv = advance(masked_value(prev, use), xv, m);
   store_value(out + (int64_t)b * F + f, hv);
   return hv;
 }
@@ -339,29 +591,105 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
   return 0;
 }
 
-template <typename V>
-static int launch_scan(const umt_gated_shape& S, const void* x, const void* gate, Masks mk, const float* h0, void* h,
-                       float* h_last, float* kept, hipStream_t s) {
-  const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  hipLaunchKernelGGL((gated_scan_kernel<V>), dim3((unsigned)((N + GT - 1) / GT)), dim3(GT), 0, s, S, (const V*)x, (const V*)gate,
-                     mk, h0, (V*)h, h_last, kept);
+// How the time axis is shared out.  `waves` = waves that 64 lanes each would make.  A wave that walks alone needs about four
+// others on its CU to keep HBM busy; below that the workgroup's waves take turns, and where even 16 of them per 64 lanes
+// leave CUs empty the axis is cut into segments of whole tiles, at the price of reading the inputs twice.
+struct Split {
+  int w, segs, seg_tiles;
+};
+static Split split_axis(int64_t waves, int t) {
+  const int64_t stretches = t > 0 ? (t + KEEP - 1) / KEEP : 1;
+  Split p{1, 1, 1};
+  if (waves < 1024 && stretches > 1) p.w = waves >= 256 || stretches <= 4 ? 4 : 16;
+  const int64_t tiles = (stretches + p.w - 1) / p.w;
+  int64_t segs = 1;
+  if (p.w == 16 && waves > 0 && waves < 128) segs = 256 / waves;
+  if (segs > tiles / 2) segs = tiles / 2;
+  if (segs < 1) segs = 1;
+  p.seg_tiles = (int)((tiles + segs - 1) / segs);
+  p.segs = (int)((tiles + p.seg_tiles - 1) / p.seg_tiles);
+  return p;
+}
+static int64_t segment_floats(const umt_gated_shape& S, int64_t waves) {
+  const Split p = split_axis(waves, S.t);
+  return p.segs > 1 ? (int64_t)p.segs * 3 * S.rows * S.groups * S.share : 0;
+}
+static int64_t scan_waves(const umt_gated_shape& S) { return ((int64_t)S.rows * S.groups * S.share + 63) / 64; }
+
+// whether a wave's lanes lie within 2^31 bytes of each other in every stream: 64 features are at most 64 rows
+static bool near_rows(const umt_gated_shape& S, int64_t size) {
+  const int F = S.groups * S.share;
+  const int64_t rows = F >= 64 ? 2 : 64 / F + 2;
+  const int64_t st[] = {S.x_row, S.gate_row, S.out_row, S.dh_row};
+  for (int64_t r : st)
+    if (r > ((1LL << 31) / size - F) / rows) return false;
+  return true;
+}
+
+template <typename V, typename OFF, bool MASK>
+static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* h0, V* h, float* h_last, float* kept,
+                       float* segs, hipStream_t s) {
+  const int64_t waves = scan_waves(S);
+  const Split p = split_axis(waves, S.t);
+  const float* entering = p.segs > 1 ? segs : nullptr;
+  if (p.w == 1) {
+    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 1, MASK>), dim3((unsigned)((waves + 3) / 4)), dim3(GT), 0, s, S, x, gate, mk, h0, entering,
+                       p.seg_tiles, h, h_last, kept);
+  } else if (p.w == 4) {
+    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 4, MASK>), dim3((unsigned)waves), dim3(256), 0, s, S, x, gate, mk, h0, entering,
+                       p.seg_tiles, h, h_last, kept);
+  } else {
+    if (p.segs > 1)
+      hipLaunchKernelGGL((gated_segment_kernel<V, OFF, 16, MASK, false>), dim3((unsigned)waves, p.segs - 1), dim3(1024), 0, s, S, x, gate, mk,
+                         p.seg_tiles, S.x_t, S.x_row, segs);
+    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 16, MASK>), dim3((unsigned)waves, p.segs), dim3(1024), 0, s, S, x, gate, mk, h0, entering,
+                       p.seg_tiles, h, h_last, kept);
+  }
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
-template <typename V>
-static int launch_backward(const umt_gated_shape& S, const void* x, const void* gate, Masks mk, const float* kept, const void* dh,
-                           const float* dh_last, void* dx, void* dgate, float* dh0, float* part, hipStream_t s) {
+template <typename V, typename OFF, bool MASK>
+static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* kept, const V* dh,
+                           const float* dh_last, V* dx, V* dgate, float* dh0, float* part, float* segs, hipStream_t s) {
   const LaneMap L = lane_map(S);
-  const int waves = GT / 64;
-  hipLaunchKernelGGL((gated_scan_backward_kernel<V>), dim3((unsigned)((L.waves + waves - 1) / waves)), dim3(GT), 0, s, S, L,
-                     (const V*)x, (const V*)gate, mk, kept, (const V*)dh, dh_last, (V*)dx, (V*)dgate, part, dh0);
+  const Split p = split_axis(L.waves, S.t);
+  const float* entering = p.segs > 1 ? segs : nullptr;
+  if (p.w == 1) {
+    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 1, MASK>), dim3((unsigned)((L.waves + 3) / 4)), dim3(GT), 0, s, S, L, x, gate, mk,
+                       kept, dh, dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+  } else if (p.w == 4) {
+    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 4, MASK>), dim3((unsigned)L.waves), dim3(256), 0, s, S, L, x, gate, mk, kept, dh,
+                       dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+  } else {
+    if (p.segs > 1)
+      hipLaunchKernelGGL((gated_segment_kernel<V, OFF, 16, MASK, true>), dim3((unsigned)scan_waves(S), p.segs - 1), dim3(1024), 0, s, S, dh,
+                         gate, mk, p.seg_tiles, S.dh_t, S.dh_row, segs);
+    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 16, MASK>), dim3((unsigned)L.waves, p.segs), dim3(1024), 0, s, S, L, x, gate, mk,
+                       kept, dh, dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+  }
   if (dgate && L.pieces > 1) {
     const int64_t n = (int64_t)S.t * S.rows * S.groups;
-    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)((n + GT - 1) / GT)), dim3(GT), 0, s, S, L.pieces, part, (V*)dgate);
+    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)((n + GT - 1) / GT)), dim3(GT), 0, s, S, L.pieces, part, dgate);
   }
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
+}
+
+static int64_t part_floats(const umt_gated_shape& S) {
+  const LaneMap L = lane_map(S);
+  return L.pieces > 1 ? (int64_t)S.t * S.rows * S.groups * L.pieces : 0;
+}
+
+// the kernel variants: value type, distance of the rows, masks
+template <typename Call>
+static int by_variant(const umt_gated_shape& S, bool masks, Call call) {
+  const bool near = near_rows(S, S.dtype == UMT_VALUES_BF16 ? 2 : 4);
+  auto typed = [&](auto v) {
+    if (near) return masks ? call(v, (uint32_t)0, std::true_type()) : call(v, (uint32_t)0, std::false_type());
+    return masks ? call(v, (uint64_t)0, std::true_type()) : call(v, (uint64_t)0, std::false_type());
+  };
+  return S.dtype == UMT_VALUES_BF16 ? typed((__bf16)0.f) : typed(0.f);
 }
 
 template <typename V>
@@ -380,7 +708,7 @@ using namespace umt;
 
 extern "C" int64_t umt_gated_scan_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  return 0;
+  return segment_floats(*shape, scan_waves(*shape)) * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -395,17 +723,20 @@ extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const
   UMT_REQUIRE(x && gate && h, UMT_ERR_INVALID, "gated scan: null pointer");
   UMT_REQUIRE(lies_apart(S.out_t, S.out_row, S.t, S.rows, (int64_t)S.groups * S.share), UMT_ERR_INVALID,
               "gated scan: the output's strides %lld, %lld overlap", (long long)S.out_t, (long long)S.out_row);
-  (void)workspace;
-  (void)workspace_bytes;
+  const int64_t need = umt_gated_scan_workspace_bytes(shape);
+  UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated scan: workspace %lld < %lld bytes",
+              (long long)workspace_bytes, (long long)need);
   const Masks mk{use_memory, valid};
-  return S.dtype == UMT_VALUES_BF16 ? launch_scan<__bf16>(S, x, gate, mk, h0, h, h_last, kept, s)
-                                    : launch_scan<float>(S, x, gate, mk, h0, h, h_last, kept, s);
+  return by_variant(S, use_memory || valid, [&](auto v, auto off, auto masked) {
+    using V = decltype(v);
+    return launch_scan<V, decltype(off), decltype(masked)::value>(S, (const V*)x, (const V*)gate, mk, h0, (V*)h, h_last, kept,
+                                                                  (float*)workspace, s);
+  });
 }
 
 extern "C" int64_t umt_gated_scan_backward_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  const LaneMap L = lane_map(*shape);
-  return L.pieces > 1 ? (int64_t)shape->t * shape->rows * shape->groups * L.pieces * (int64_t)sizeof(float) : 0;
+  return (segment_floats(*shape, lane_map(*shape).waves) + part_floats(*shape)) * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -426,9 +757,12 @@ extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void*
   UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated scan backward: workspace %lld < %lld bytes",
               (long long)workspace_bytes, (long long)need);
   const Masks mk{use_memory, valid};
-  return S.dtype == UMT_VALUES_BF16
-             ? launch_backward<__bf16>(S, x, gate, mk, kept, dh, dh_last, dx, dgate, dh0, (float*)workspace, s)
-             : launch_backward<float>(S, x, gate, mk, kept, dh, dh_last, dx, dgate, dh0, (float*)workspace, s);
+  float *part = (float*)workspace, *segs = part + part_floats(S);
+  return by_variant(S, use_memory || valid, [&](auto v, auto off, auto masked) {
+    using V = decltype(v);
+    return launch_backward<V, decltype(off), decltype(masked)::value>(S, (const V*)x, (const V*)gate, mk, kept, (const V*)dh, dh_last, (V*)dx,
+                                                                      (V*)dgate, dh0, part, segs, s);
+  });
 }
 
 extern "C" int64_t umt_gated_step_workspace_bytes(int batch, int cache_rows) {

@@ -4,9 +4,9 @@
 //
 // One lane owns one (row, feature); a wave loads UMT_GATED_KEEP steps of its 64 lanes at once, so neighbouring lanes read
 // neighbouring features and 32 loads are in flight.  Where there are many lanes a wave walks the whole axis alone.  Where
-// there are few, the waves of a workgroup take successive stretches of a tile (the recurrence over a stretch is itself a
-// step, see join()), and beyond that the axis is cut into segments that workgroups of their own run, whose steps a first
-// launch finds.  No order of arrival enters a result.
+// there are fewer, the waves of a workgroup take successive stretches of a tile (the recurrence over a stretch is itself a
+// step, see join()).  Where there are few, the axis is cut into runs, a wave each: a first launch finds the step that each
+// run is, a second one walks the runs from the states they begin with.  No order of arrival enters a result.
 //
 // Arithmetic.  With e = exp(-|gate|) the smaller of (a, c) is m = e / (1 + e), which keeps its relative precision however
 // small it gets, and the larger one is 1 - m.  A step is base + m (other - base), where base is what the larger weight
@@ -21,6 +21,7 @@ namespace umt {
 
 constexpr int KEEP = UMT_GATED_KEEP;
 constexpr int GT = 256;
+constexpr int RUN_WAVES = 4;               // runs of a workgroup
 
 __device__ __forceinline__ float as_value(float v) { return v; }
 __device__ __forceinline__ float as_value(__bf16 v) { return (float)v; }
@@ -35,10 +36,10 @@ __device__ __forceinline__ float gate_step(float g) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
   return copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
 }
+__device__ __forceinline__ bool from_input(float m) { return __float_as_uint(m) >> 31; }
 
 __device__ __forceinline__ float advance(float h, float x, float m) {
-  const bool from_x = __float_as_uint(m) >> 31;
-  const float base = from_x ? x : h, other = from_x ? h : x;
+  const float base = from_input(m) ? x : h, other = from_input(m) ? h : x;
   return fmaf(fabsf(m), other - base, base);
 }
 
@@ -49,26 +50,39 @@ __device__ __forceinline__ float masked_value(float v, unsigned mask) { return _
 __device__ __forceinline__ float masked_step(float m, unsigned use, unsigned valid) {
   return __uint_as_float((__float_as_uint(m) & valid & use) | (~use & 0x80000000u));
 }
+template <bool MASK>
+__device__ __forceinline__ float memory_of(float h, unsigned ub, int j) {
+  return MASK ? masked_value(h, bit_mask(ub, j)) : h;
+}
 
 // backward factors of a step: c s and a s for the stored m
 __device__ __forceinline__ float times_c(float m, float s) {
   const float p = fabsf(m) * s;
-  return __float_as_uint(m) >> 31 ? s - p : p;
+  return from_input(m) ? s - p : p;
 }
 __device__ __forceinline__ float times_a(float m, float s) {
   const float p = fabsf(m) * s;
-  return __float_as_uint(m) >> 31 ? p : s - p;
+  return from_input(m) ? p : s - p;
 }
 
-struct Masks {
-  const uint8_t* use;
-  const uint8_t* valid;
-};
-
-// A stretch of steps is a step itself: h_out = p + a h_in, with q = 1 - a carried on its own (the stretch's response to a
-// memory of 0 and inputs of 1), because 1 - a of a rounded a has lost a slow decay.
+// A stretch of steps is a step itself: h_out = p + a h_in.  q = 1 - a is carried on its own (the stretch's response to a
+// memory of 0 and inputs of 1: sums of positive terms), because 1 - a of a rounded a has lost a slow decay.
 struct Stretch {
   float a, q, p;
+  template <bool MASK>
+  __device__ __forceinline__ void forward(float x, float m, unsigned ub, int j) {
+    const float s = fabsf(m), l = 1.f - s, sa = from_input(m) ? s : l, sc = from_input(m) ? l : s;
+    a *= sa;
+    q = fmaf(sa, q, sc);
+    p = fmaf(sa, memory_of<MASK>(p, ub, j), sc * x);
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void backward(float d, float m, unsigned ub, int j) {
+    const float s = fabsf(m), l = 1.f - s, sa = from_input(m) ? s : l, sc = from_input(m) ? l : s;
+    a *= sa;
+    q = fmaf(sa, q, sc);
+    p = memory_of<MASK>(sa * (d + p), ub, j);
+  }
 };
 __device__ __forceinline__ float join(float h, const Stretch& s) {
   const float slow = h + fmaf(-s.q, h, s.p), fast = fmaf(s.a, h, s.p);
@@ -78,15 +92,55 @@ __device__ __forceinline__ Stretch then(const Stretch& f, const Stretch& s) {
   return Stretch{f.a * s.a, join(f.q, Stretch{s.a, s.q, s.q}), join(f.p, s)};
 }
 
-// One stream of (t, row, feature) values as a wave addresses it: the step's place is the same in all lanes, a lane adds
-// its distance from the wave's first row (OFF = 32 bits unless the rows lie further apart than that)
+struct Masks {
+  const uint8_t* use;
+  const uint8_t* valid;
+};
+
+template <typename P>
+__device__ __forceinline__ P uniform(P p) {                 // into scalar registers: the same in all lanes of the wave
+  const uint64_t v = (uint64_t)p;
+  return (P)(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+             (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// One stream of (t, row, feature) values as a wave addresses it: a step's place is the same in all lanes, a lane adds its
+// distance from the wave's first row (OFF = 32 bits unless the rows lie further apart than that)
 template <typename V, typename OFF>
 struct Lanes {
-  const V* at;             // step 0 of the wave's first row
-  int64_t step;
-  OFF mine;                // in bytes
-  __device__ __forceinline__ V load(int64_t t) const {
-    return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(at + t * step) + mine);
+  char* at;                // step 0 of the wave's first row
+  int64_t step;            // bytes
+  OFF mine;                // bytes
+  __device__ __forceinline__ Lanes(const V* p, int64_t t_stride, int64_t row_stride, int64_t row0, int64_t row, int64_t inner) {
+    at = uniform((char*)(p + row0 * row_stride));
+    step = t_stride * (int64_t)sizeof(V);
+    mine = (OFF)(((row - row0) * row_stride + inner) * (int64_t)sizeof(V));
+  }
+  // steps t0 .. t0 + KEEP - 1; those past the end read the last one
+  __device__ __forceinline__ void load(int t0, int T, V (&r)[KEEP]) const {
+    const char* p = at + (t0 < T ? t0 : T - 1) * step;
+    if (t0 + KEEP <= T) {
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j, p += step) r[j] = *(const V*)(p + mine);
+    } else {
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) {
+        r[j] = *(const V*)(p + mine);
+        p += t0 + j + 1 < T ? step : 0;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(int t0, int T, bool on, const float (&r)[KEEP]) const {
+    char* p = at + t0 * step;
+    if (!on) return;
+    if (t0 + KEEP <= T) {
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j, p += step) store_value((V*)(p + mine), r[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j, p += step)
+        if (t0 + j < T) store_value((V*)(p + mine), r[j]);
+    }
   }
 };
 
@@ -114,61 +168,70 @@ struct MaskLanes {
   }
 };
 
-// What one wave of the forward direction works on
+// The (row, feature) of a lane.  A wave owns `per` consecutive ones, from wave * per on; lanes without one stand in for the
+// wave's first and write nothing.
+template <typename OFF>
+struct Place {
+  using Index = std::conditional_t<sizeof(OFF) == 4, uint32_t, int64_t>;      // 32-bit divisions where they do
+  int64_t e0, e, row0, row;
+  int f, gi;
+  bool on;
+  __device__ __forceinline__ Place(const umt_gated_shape& S, int64_t wave, int per) {
+    const int lane = threadIdx.x & 63;
+    const Index F = (Index)(S.groups * S.share), N = (Index)S.rows * F, first = (Index)wave * (Index)per, i = first + (Index)lane;
+    on = lane < per && i < N;
+    const Index k = on ? i : first, r0 = first / F, r = k / F;
+    e0 = first;
+    e = k;
+    row0 = r0;
+    row = r;
+    f = (int)(k - r * F);
+    gi = f / S.share;
+  }
+};
+
+// The two streams that both directions go by (an input and its gate) with the masks
 template <typename V, typename OFF, bool MASK>
 struct Walk {
   Lanes<V, OFF> x, g;
   MaskLanes um, vm;
-  bool has_use, has_valid;
   int T;
   V rx[KEEP], rg[KEEP];
   uint8_t ru, rv;
 
-  // e0: first element of the wave, e: this lane's (clamped into the call)
-  __device__ __forceinline__ void place(const umt_gated_shape& S, const V* x_, const V* gate_, const Masks& mk, int64_t row0, int64_t row,
-                                        int f, int gi, int64_t x_t, int64_t x_row) {
-    T = S.t;
-    x = {x_ + row0 * x_row, x_t, (OFF)(((row - row0) * x_row + f) * (int64_t)sizeof(V))};
-    g = {gate_ + row0 * S.gate_row, S.gate_t, (OFF)(((row - row0) * S.gate_row + gi) * (int64_t)sizeof(V))};
+  __device__ __forceinline__ Walk(const umt_gated_shape& S, const Place<OFF>& at, const V* x_, int64_t x_t, int64_t x_row, const V* gate_,
+                                  const Masks& mk)
+      : x(x_, x_t, x_row, at.row0, at.row, at.f), g(gate_, S.gate_t, S.gate_row, at.row0, at.row, at.gi), T(S.t) {
     if (MASK) {
-      const int mine = (int)(row - row0), span = __builtin_amdgcn_readfirstlane(wave_max(mine)) + 1;
-      has_use = mk.use != nullptr;
-      has_valid = mk.valid != nullptr;
-      um = {mk.use, S.use_t, S.use_row, row0, S.rows, span, mine};
-      vm = {mk.valid, S.valid_t, S.valid_row, row0, S.rows, span, mine};
+      int span = (int)(at.row - at.row0);
+      const int mine = span;
+      for (int o = 32; o > 0; o >>= 1) span = max(span, __shfl_xor(span, o));
+      span = __builtin_amdgcn_readfirstlane(span) + 1;
+      um = {mk.use, S.use_t, S.use_row, at.row0, S.rows, span, mine};
+      vm = {mk.valid, S.valid_t, S.valid_row, at.row0, S.rows, span, mine};
     }
-  }
-  static __device__ __forceinline__ int wave_max(int v) {
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
-    return v;
   }
   __device__ __forceinline__ void fetch(int t0) {
     if (MASK) {
-      if (has_use) ru = um.fetch(t0, T, 0);
-      if (has_valid) rv = vm.fetch(t0, T, 0);
+      if (um.p) ru = um.fetch(t0, T, 0);
+      if (vm.p) rv = vm.fetch(t0, T, 0);
     }
-#pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-      const int t = t0 + j < T ? t0 + j : T - 1;
-      rg[j] = g.load(t);
-      rx[j] = x.load(t);
-    }
+    g.load(t0, T, rg);
+    x.load(t0, T, rx);
   }
-  // the fetched stretch: inputs, m of each step, mask bits (steps past the end are skipped frames)
-  // back: xs are gradients, which no valid mask covers
-  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP], float (&ms)[KEEP], unsigned& ub, unsigned& vb, bool back) {
+  // The fetched stretch: inputs, m of each step, mask bits.  Steps past the end are skipped frames.  BACK: the inputs are
+  // gradients, which no valid mask covers.
+  template <bool BACK>
+  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP], float (&ms)[KEEP], unsigned& ub, unsigned& vb) {
     ub = vb = 0xffffu;
     if (MASK) {
-      if (has_use) ub = um.bits(ru, t0, T);
-      if (has_valid) vb = vm.bits(rv, t0, T);
+      if (um.p) ub = um.bits(ru, t0, T);
+      if (vm.p) vb = vm.bits(rv, t0, T);
     }
     const int left = T - t0;
-    unsigned past = 0;
-    if (left < KEEP) {
-      past = left <= 0 ? 0xffffu : 0xffffu << left & 0xffffu;
-      ub |= past;
-      vb &= ~past;
-    }
+    const unsigned past = left >= KEEP ? 0u : left <= 0 ? 0xffffu : 0xffffu << left & 0xffffu;
+    ub |= past;
+    vb &= ~past;
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
       xs[j] = as_value(rx[j]);
@@ -178,17 +241,12 @@ struct Walk {
 #pragma unroll
       for (int j = 0; j < KEEP; ++j) {
         const unsigned v = bit_mask(vb, j);
-        xs[j] = masked_value(xs[j], back ? ~bit_mask(past, j) : v);
+        xs[j] = masked_value(xs[j], BACK ? ~bit_mask(past, j) : v);
         ms[j] = masked_step(ms[j], bit_mask(ub, j), v);
       }
     }
   }
 };
-
-template <bool MASK>
-__device__ __forceinline__ float memory_of(float h, unsigned ub, int j) {
-  return MASK ? masked_value(h, bit_mask(ub, j)) : h;
-}
 
 // Partners: the W waves of a workgroup take the KEEP-step stretches of a tile in turn; each hands its stretch over in LDS and
 // joins those before it (after it, in the backward direction) to the state that entered the tile.
@@ -216,268 +274,294 @@ struct Partners {
   }
 };
 
-template <int W>
-constexpr int group_threads() { return W == 1 ? GT : 64 * W; }
+// How a call is shared out (split_axis)
+struct Split {
+  int per;                 // lanes of a wave that own a feature
+  int w;                   // waves that share a tile, 1: a wave walks alone
+  int len;                 // stretches of a run, 0: the axis is not cut
+  int groups;              // workgroups along the axis
+  int64_t waves;           // of `per` lanes
+};
 
-// the joined segments before (after) this one, [segment][a, q, p][lane] in `segs`: the waves join a run of them each
-template <int W, bool BACK>
-__device__ __forceinline__ float enter_segment(const float* __restrict__ segs, int seg, int n_segs, int64_t n, int64_t e, int tw, int lane,
-                                               float first, Partners<W>& partners) {
-  const int count = BACK ? n_segs - 1 - seg : seg, per = (count + W - 1) / W;
-  const int a0 = min(count, tw * per), a1 = min(count, a0 + per);
-  Stretch run{1.f, 0.f, 0.f};
-  for (int i = a0; i < a1; ++i) {
-    const float* s = segs + (int64_t)(BACK ? n_segs - 1 - i : i) * 3 * n + e;
-    run = then(run, Stretch{s[0], s[n], s[2 * n]});
+// Where a wave works: its lanes' wave, its first stretch, how many stretches, the distance between them
+template <int W, bool RUNS>
+struct Part {
+  int64_t wave;
+  int tw, first, count, by;
+  __device__ __forceinline__ Part(const Split& P, int T) {
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), all = (T + KEEP - 1) / KEEP;
+    if (RUNS) {
+      wave = blockIdx.x;
+      tw = wv;
+      first = (blockIdx.y * RUN_WAVES + wv) * P.len;
+      count = max(0, min(P.len, all - first));
+      by = 1;
+    } else {
+      wave = W == 1 ? (int64_t)blockIdx.x * (GT / 64) + wv : blockIdx.x;
+      tw = first = W == 1 ? 0 : wv;
+      count = (all + W - 1) / W;            // the same for all waves of a workgroup, which meet at a barrier a tile
+      by = W;
+    }
   }
-  float through = first;
-  partners.template enter<false>(run, tw, lane, through);
-  return through;
+};
+
+// ws: Stretch of every run [run][3][N], then of every workgroup's runs joined [group][3][N]
+__device__ __forceinline__ float* run_at(float* ws, int64_t N, int run) { return ws + (int64_t)run * 3 * N; }
+__device__ __forceinline__ Stretch load_stretch(const float* s, int64_t N, int64_t e) { return Stretch{s[e], s[N + e], s[2 * N + e]}; }
+__device__ __forceinline__ void store_stretch(float* s, int64_t N, int64_t e, const Stretch& v) {
+  s[e] = v.a;
+  s[N + e] = v.q;
+  s[2 * N + e] = v.p;
 }
 
-template <typename V, typename OFF, int W, bool MASK>
-__global__ __launch_bounds__(group_threads<W>()) void gated_scan_kernel(umt_gated_shape S, const V* __restrict__ x, const V* __restrict__ gate,
-                                                                        Masks mk, const float* __restrict__ h0, const float* __restrict__ segs,
-                                                                        int seg_tiles, V* __restrict__ h, float* __restrict__ h_last,
-                                                                        float* __restrict__ kept) {
-  __shared__ float lds[W > 1 ? 2 : 1][W][3][64];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int F = S.groups * S.share;
-  const int64_t N = (int64_t)S.rows * F;
-  const int64_t e0 = W == 1 ? ((int64_t)blockIdx.x * (GT / 64) + wv) * 64 : (int64_t)blockIdx.x * 64;
-  const int tw = W == 1 ? 0 : wv;
-  if (W == 1 && e0 >= N) return;
-  const int64_t e = e0 + lane < N ? e0 + lane : N - 1;
-  const bool on = e0 + lane < N;
-  const int64_t row0 = e0 / F, row = e / F;
-  const int f = (int)(e - row * F);
-  Walk<V, OFF, MASK> w;
-  w.place(S, x, gate, mk, row0, row, f, f / S.share, S.x_t, S.x_row);
-  char* hp = reinterpret_cast<char*>(h + row0 * S.out_row);
-  const OFF mine = (OFF)(((row - row0) * S.out_row + f) * (int64_t)sizeof(V));
-  const int tiles = (S.t + KEEP * W - 1) / (KEEP * W);
-  const int tile0 = blockIdx.y * seg_tiles, tile1 = min(tiles, tile0 + seg_tiles);
-  w.fetch((tile0 * W + tw) * KEEP);
-  float cur = h0 ? h0[e] : 0.f;
-  Partners<W> partners{reinterpret_cast<float(*)[W][3][64]>(lds)};
-  if (W > 1 && segs) cur = enter_segment<W, false>(segs, blockIdx.y, gridDim.y, N, e, tw, lane, cur, partners);
-  for (int tile = tile0; tile < tile1; ++tile) {
-    const int t0 = (tile * W + tw) * KEEP;
+// The step that each run is (BACK: of the gradient that comes from behind)
+template <typename V, typename OFF, bool MASK, bool BACK>
+__global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_shape S, Split P, const V* __restrict__ v, int64_t v_t, int64_t v_row,
+                                                                    const V* __restrict__ gate, Masks mk, float* __restrict__ ws) {
+  __shared__ float lds[RUN_WAVES][3][64];
+  const int lane = threadIdx.x & 63;
+  const Part<1, true> part(P, S.t);
+  const Place<OFF> at(S, part.wave, P.per);
+  const int64_t N = (int64_t)S.rows * S.groups * S.share;
+  Walk<V, OFF, MASK> w(S, at, v, v_t, v_row, gate, mk);
+  Stretch own{1.f, 0.f, 0.f};
+  const int last = part.first + part.count - 1;
+  if (part.count > 0) w.fetch((BACK ? last : part.first) * KEEP);
+  for (int k = 0; k < part.count; ++k) {
+    const int t0 = (BACK ? last - k : part.first + k) * KEEP;
     float xs[KEEP], ms[KEEP];
     unsigned ub, vb;
-    w.take(t0, xs, ms, ub, vb, false);
-    if (tile + 1 < tile1) w.fetch(t0 + W * KEEP);
+    w.template take<BACK>(t0, xs, ms, ub, vb);
+    if (k + 1 < part.count) w.fetch(BACK ? t0 - KEEP : t0 + KEEP);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int j = BACK ? KEEP - 1 - i : i;
+      if (BACK)
+        own.template backward<MASK>(xs[j], ms[j], ub, j);
+      else
+        own.template forward<MASK>(xs[j], ms[j], ub, j);
+    }
+  }
+  lds[part.tw][0][lane] = own.a;
+  lds[part.tw][1][lane] = own.q;
+  lds[part.tw][2][lane] = own.p;
+  if (at.on) store_stretch(run_at(ws, N, blockIdx.y * RUN_WAVES + part.tw), N, at.e, own);
+  __syncthreads();
+  if (part.tw != 0 || !at.on) return;
+  Stretch all{1.f, 0.f, 0.f};
+  for (int i = 0; i < RUN_WAVES; ++i) {
+    const int k = BACK ? RUN_WAVES - 1 - i : i;
+    all = then(all, Stretch{lds[k][0][lane], lds[k][1][lane], lds[k][2][lane]});
+  }
+  store_stretch(run_at(ws, N, P.groups * RUN_WAVES + blockIdx.y), N, at.e, all);
+}
+
+// State with which this wave's run begins: the workgroups before it (BACK: behind it) are joined by the waves, a quarter
+// each, then the runs before it in its own
+template <bool BACK>
+__device__ __forceinline__ float enter_run(const float* ws, const Split& P, int64_t N, int64_t e, int tw, int lane, float first,
+                                           Partners<RUN_WAVES>& partners) {
+  const int group = blockIdx.y, count = BACK ? P.groups - 1 - group : group, each = (count + RUN_WAVES - 1) / RUN_WAVES;
+  const int i0 = min(count, tw * each), i1 = min(count, i0 + each);
+  const float* joined = ws + (int64_t)P.groups * RUN_WAVES * 3 * N;
+  Stretch run{1.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = i0; i < i1; ++i) run = then(run, load_stretch(joined + (int64_t)(BACK ? P.groups - 1 - i : i) * 3 * N, N, e));
+  Stretch near[RUN_WAVES];
+#pragma unroll
+  for (int k = 0; k < RUN_WAVES; ++k) near[k] = load_stretch(ws + (int64_t)(group * RUN_WAVES + k) * 3 * N, N, e);
+  float h = first;
+  partners.template enter<false>(run, tw, lane, h);
+#pragma unroll
+  for (int i = 0; i < RUN_WAVES; ++i) {
+    const int k = BACK ? RUN_WAVES - 1 - i : i;
+    if (BACK ? k > tw : k < tw) h = join(h, near[k]);
+  }
+  return h;
+}
+
+template <int W, bool RUNS>
+constexpr int partner_waves() { return RUNS ? RUN_WAVES : W; }
+template <int W, bool RUNS>
+constexpr int group_threads() { return RUNS ? 64 * RUN_WAVES : W == 1 ? GT : 64 * W; }
+
+template <typename V, typename OFF, int W, bool MASK, bool RUNS>
+__global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(umt_gated_shape S, Split P, const V* __restrict__ x,
+                                                                              const V* __restrict__ gate, Masks mk,
+                                                                              const float* __restrict__ h0, const float* __restrict__ ws,
+                                                                              V* __restrict__ h, float* __restrict__ h_last,
+                                                                              float* __restrict__ kept) {
+  constexpr int PW = partner_waves<W, RUNS>();
+  __shared__ float lds[PW > 1 ? 2 : 1][PW][3][64];
+  const int lane = threadIdx.x & 63;
+  const Part<W, RUNS> part(P, S.t);
+  if (W == 1 && !RUNS && part.wave >= P.waves) return;
+  const Place<OFF> at(S, part.wave, P.per);
+  const int64_t N = (int64_t)S.rows * S.groups * S.share;
+  Walk<V, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  const Lanes<V, OFF> out(h, S.out_t, S.out_row, at.row0, at.row, at.f);
+  if (part.count > 0) w.fetch(part.first * KEEP);
+  Partners<PW> partners{reinterpret_cast<float(*)[PW][3][64]>(lds)};
+  float cur = h0 ? h0[at.e] : 0.f;
+  if constexpr (RUNS) cur = enter_run<false>(ws, P, N, at.e, part.tw, lane, cur, partners);
+  for (int k = 0; k < part.count; ++k) {
+    const int c = part.first + k * part.by, t0 = c * KEEP;
+    float xs[KEEP], ms[KEEP];
+    unsigned ub, vb;
+    w.template take<false>(t0, xs, ms, ub, vb);
+    if (k + 1 < part.count) w.fetch(t0 + part.by * KEEP);
     float st = cur;
     if (W > 1) {
       Stretch own{1.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j) {
-        own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
-        own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
-        own.p = advance(memory_of<MASK>(own.p, ub, j), xs[j], ms[j]);
-      }
-      st = partners.template enter<false>(own, tw, lane, cur);
+      for (int j = 0; j < KEEP; ++j) own.template forward<MASK>(xs[j], ms[j], ub, j);
+      st = partners.template enter<false>(own, part.tw, lane, cur);
       if (t0 >= S.t) continue;
     }
-    if (kept && on) kept[(int64_t)(t0 / KEEP) * N + e] = st;
+    if (kept && at.on) kept[(int64_t)c * N + at.e] = st;
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-      st = advance(memory_of<MASK>(st, ub, j), xs[j], ms[j]);
-      if (on && t0 + j < S.t) store_value(reinterpret_cast<V*>(hp + (int64_t)(t0 + j) * S.out_t * (int64_t)sizeof(V) + mine), st);
-    }
-    if (h_last && on && t0 + KEEP >= S.t) h_last[e] = st;
+    for (int j = 0; j < KEEP; ++j) xs[j] = st = advance(memory_of<MASK>(st, ub, j), xs[j], ms[j]);
+    out.store(t0, S.t, at.on, xs);
+    if (h_last && at.on && t0 + KEEP >= S.t) h_last[at.e] = st;
     if (W == 1) cur = st;
   }
 }
 
-// The steps that the first segments make of the state (of the gradient that enters from behind, for the last segments):
-// a wave walks its share of the segment alone, the waves' stretches are joined at the end.
-template <typename V, typename OFF, int W, bool MASK, bool BACK>
-__global__ __launch_bounds__(64 * W) void gated_segment_kernel(umt_gated_shape S, const V* __restrict__ v, const V* __restrict__ gate, Masks mk,
-                                                               int seg_tiles, int64_t v_t, int64_t v_row, float* __restrict__ segs) {
-  __shared__ float lds[W][3][64];
-  const int lane = threadIdx.x & 63, tw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int F = S.groups * S.share;
-  const int64_t N = (int64_t)S.rows * F;
-  const int64_t e0 = (int64_t)blockIdx.x * 64;
-  const int64_t e = e0 + lane < N ? e0 + lane : N - 1;
-  const int64_t row0 = e0 / F, row = e / F;
-  const int f = (int)(e - row * F);
-  Walk<V, OFF, MASK> w;
-  w.place(S, v, gate, mk, row0, row, f, f / S.share, v_t, v_row);
-  const int seg = blockIdx.y + (BACK ? 1 : 0);
-  const int c0 = (seg * W + tw) * seg_tiles;               // stretches of this wave: c0 .. c0 + seg_tiles - 1
-  Stretch own{1.f, 0.f, 0.f};
-  w.fetch((BACK ? c0 + seg_tiles - 1 : c0) * KEEP);
-  for (int k = 0; k < seg_tiles; ++k) {
-    const int t0 = (BACK ? c0 + seg_tiles - 1 - k : c0 + k) * KEEP;
-    float xs[KEEP], ms[KEEP];
-    unsigned ub, vb;
-    w.take(t0, xs, ms, ub, vb, BACK);
-    if (k + 1 < seg_tiles) w.fetch(BACK ? t0 - KEEP : t0 + KEEP);
+// ---------------------------------------------------------------- backward
+// Sums over the features of a gate.  A wave's lanes hold consecutive features, so a gate's are a run of lanes.  The KEEP
+// steps' products go through the wave's own LDS rows; lane 16 k + j adds up step j: whole gates k, k + 4, ... where the
+// wave holds many, a quarter of each where it holds few.  A gate that reaches into other waves leaves its part in `part`, and
+// a second launch adds the parts in order.
+constexpr int SUM_ROW = 65;                // floats of a step's row: the 16 steps of a read lie in different banks
+
+struct GateSums {
+  int64_t G, group0;       // gates of a step, the wave's first
+  int count, lead, per;    // gates that the wave holds, features of the first that lie before it, lanes
+  int slots;
+};
+
+template <typename V>
+__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, int64_t wave, float* rows, const float (&v)[KEEP], bool on,
+                                          int t0, V* __restrict__ dgate, float* __restrict__ part) {
+  const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4, t = t0 + j;
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int j = BACK ? KEEP - 1 - i : i;
-      own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
-      own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
-      own.p = BACK ? memory_of<MASK>(times_a(ms[j], xs[j] + own.p), ub, j) : advance(memory_of<MASK>(own.p, ub, j), xs[j], ms[j]);
+  for (int i = 0; i < KEEP; ++i) rows[i * SUM_ROW + lane] = on ? v[i] : 0.f;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const float* row = rows + j * SUM_ROW;
+  const bool many = A.count > 6;
+  for (int k = many ? k0 : 0; k < A.count; k += many ? 4 : 1) {
+    const int lo = max(0, k * S.share - A.lead), hi = min(A.per, (k + 1) * S.share - A.lead), n = hi - lo;
+    float s = 0.f;
+    if (many) {
+      for (int i = lo; i < hi; ++i) s += row[i];
+    } else {
+      const int each = (n + 3) >> 2, i1 = min(hi, lo + (k0 + 1) * each);
+      for (int i = lo + k0 * each; i < i1; ++i) s += row[i];
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+    }
+    const int64_t group = A.group0 + k;
+    if (t < S.t && group < A.G && (many || k0 == 0)) {
+      if (n == S.share) {
+        const int64_t r = group / S.groups;
+        store_value(dgate + t * S.dgate_t + r * S.dgate_row + (group - r * S.groups), s);
+      } else {
+        part[((int64_t)t * A.G + group) * A.slots + (wave - group * S.share / A.per)] = s;
+      }
     }
   }
-  lds[tw][0][lane] = own.a;
-  lds[tw][1][lane] = own.q;
-  lds[tw][2][lane] = own.p;
-  __syncthreads();
-  if (tw != 0 || e0 + lane >= N) return;
-  Stretch all{1.f, 0.f, 0.f};
-  for (int i = 0; i < W; ++i) {
-    const int k = BACK ? W - 1 - i : i;
-    all = then(all, Stretch{lds[k][0][lane], lds[k][1][lane], lds[k][2][lane]});
-  }
-  float* o = segs + (int64_t)seg * 3 * N + e;
-  o[0] = all.a;
-  o[N] = all.q;
-  o[2 * N] = all.p;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
-// Which features the lanes of a backward wave own.  share = 1: 64 in a row.  share <= 64: as many whole groups as fit, so
-// that the sum over a group stays in its wave (21 landmarks of 3 coordinates: 63 lanes).  share > 64: one of `pieces` equal
-// parts of one group; the parts' sums are added by a second launch in part order, so no order of arrival is in the result.
-struct LaneMap {
-  int pieces, width, groups_per_wave;     // pieces > 1: width = features of a piece
-  int64_t waves;
-};
-static LaneMap lane_map(const umt_gated_shape& S) {
-  LaneMap m{1, S.share, 1, 0};
+template <typename V>
+__global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int per, int slots, const float* __restrict__ part,
+                                                        V* __restrict__ dgate) {
   const int64_t G = (int64_t)S.rows * S.groups;
-  if (S.share > 64) {
-    m.pieces = (S.share + 63) / 64;
-    m.width = (S.share + m.pieces - 1) / m.pieces;
-    m.waves = G * m.pieces;
-  } else {
-    m.groups_per_wave = 64 / S.share;
-    m.waves = (G + m.groups_per_wave - 1) / m.groups_per_wave;
-  }
-  return m;
+  const int64_t k = (int64_t)blockIdx.x * GT + threadIdx.x;
+  if (k >= G * S.t) return;
+  const int64_t t = k / G, g = k - t * G, row = g / S.groups;
+  const int n = (int)(((g + 1) * S.share - 1) / per - g * S.share / per) + 1;
+  if (n == 1) return;
+  float s = 0.f;
+  for (int p = 0; p < n; ++p) s += part[k * slots + p];
+  store_value(dgate + t * S.dgate_t + row * S.dgate_row + (g - row * S.groups), s);
 }
 
-// sum of the `len` lanes from this one on within its group or piece (`pos` = place in it): log2(len) exchanges in a fixed
-// order, the group's first lane holds the whole sum
-__device__ __forceinline__ float group_sum(float v, int pos, int len) {
-  for (int o = 1; o < len; o <<= 1) {
-    const float w = __shfl_down(v, o);
-    v += pos + o < len ? w : 0.f;
-  }
-  return v;
-}
-
-template <typename V, typename OFF, int W, bool MASK>
-__global__ __launch_bounds__(group_threads<W>()) void gated_scan_backward_kernel(
-    umt_gated_shape S, LaneMap L, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
-    const V* __restrict__ dh, const float* __restrict__ dh_last, const float* __restrict__ segs, int seg_tiles, V* __restrict__ dx,
-    V* __restrict__ dgate, float* __restrict__ part, float* __restrict__ dh0) {
-  __shared__ float lds[W > 1 ? 2 : 1][W][3][64];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t wave = W == 1 ? (int64_t)blockIdx.x * (GT / 64) + wv : blockIdx.x;
-  const int tw = W == 1 ? 0 : wv;
-  if (wave >= L.waves) return;
-  const int F = S.groups * S.share;
-  const int64_t N = (int64_t)S.rows * F, G = (int64_t)S.rows * S.groups;
-  // the wave's first group, and this lane's place in its group or piece
-  int64_t group0, group;
-  int pos, len, first;                     // place, length, and the feature of the group at which the piece starts
-  if (L.pieces > 1) {
-    group0 = group = wave / L.pieces;
-    first = (int)(wave - group * L.pieces) * L.width;
-    len = min(L.width, S.share - first);
-    pos = lane;
-  } else {
-    group0 = wave * L.groups_per_wave;
-    group = group0 + lane / S.share;
-    first = 0;
-    len = S.share;
-    pos = lane % S.share;
-  }
-  const bool on = pos < len && group < G && (L.pieces > 1 || lane < L.groups_per_wave * S.share);
-  group = on ? group : group0;
-  const int64_t row0 = group0 / S.groups, row = group / S.groups;
-  const int gi = (int)(group - row * S.groups);
-  const int f = gi * S.share + (on ? first + pos : first);
-  const int64_t e = row * F + f;
-  Walk<V, OFF, MASK> w;
-  w.place(S, x, gate, mk, row0, row, f, gi, S.x_t, S.x_row);
-  const Lanes<V, OFF> d{dh + row0 * S.dh_row, S.dh_t, (OFF)(((row - row0) * S.dh_row + f) * (int64_t)sizeof(V))};
-  char* dxp = dx ? reinterpret_cast<char*>(dx + row0 * S.out_row) : nullptr;
-  const OFF mine = (OFF)(((row - row0) * S.out_row + f) * (int64_t)sizeof(V));
-  const int tiles = (S.t + KEEP * W - 1) / (KEEP * W);
-  const int tile0 = blockIdx.y * seg_tiles, tile1 = min(tiles, tile0 + seg_tiles);
-  Partners<W> partners{reinterpret_cast<float(*)[W][3][64]>(lds)};
-  float v = dh_last ? dh_last[e] : 0.f;
-  if (W > 1 && segs) v = enter_segment<W, true>(segs, blockIdx.y, gridDim.y, N, e, tw, lane, v, partners);
-  for (int tile = tile1 - 1; tile >= tile0; --tile) {
-    const int t0 = (tile * W + tw) * KEEP;
+template <typename V, typename OFF, int W, bool MASK, bool RUNS>
+__global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backward_kernel(
+    umt_gated_shape S, Split P, int slots, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
+    const V* __restrict__ dh, const float* __restrict__ dh_last, const float* __restrict__ ws, V* __restrict__ dx, V* __restrict__ dgate,
+    float* __restrict__ parts, float* __restrict__ dh0) {
+  constexpr int PW = partner_waves<W, RUNS>(), GW = group_threads<W, RUNS>() / 64;
+  __shared__ float lds[PW > 1 ? 2 : 1][PW][3][64];
+  __shared__ float sums[GW][KEEP * SUM_ROW];
+  const int lane = threadIdx.x & 63;
+  const Part<W, RUNS> part(P, S.t);
+  if (W == 1 && !RUNS && part.wave >= P.waves) return;
+  const Place<OFF> at(S, part.wave, P.per);
+  const int64_t N = (int64_t)S.rows * S.groups * S.share;
+  Walk<V, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  const Lanes<V, OFF> d(dh, S.dh_t, S.dh_row, at.row0, at.row, at.f), out(dx, S.out_t, S.out_row, at.row0, at.row, at.f);
+  const Lanes<V, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
+  GateSums A;
+  A.G = (int64_t)S.rows * S.groups;
+  A.group0 = at.e0 / S.share;
+  A.lead = (int)(at.e0 - A.group0 * S.share);
+  A.per = P.per;
+  A.slots = slots;
+  A.count = (A.lead + P.per + S.share - 1) / S.share;
+  Partners<PW> partners{reinterpret_cast<float(*)[PW][3][64]>(lds)};
+  float v = dh_last ? dh_last[at.e] : 0.f;
+  if constexpr (RUNS) v = enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
+  for (int k = part.count - 1; k >= 0; --k) {
+    const int c = part.first + k * part.by, t0 = c * KEEP;
     float q[KEEP], ms[KEEP], ds[KEEP];
     unsigned ub, vb;
-    w.fetch(t0);
     V rd[KEEP];
-#pragma unroll
-    for (int j = 0; j < KEEP; ++j) rd[j] = d.load(t0 + j < S.t ? t0 + j : S.t - 1);
-    float cur = t0 < S.t ? kept[(int64_t)(t0 / KEEP) * N + e] : 0.f;
-    w.take(t0, q, ms, ub, vb, false);
+    w.fetch(t0);
+    d.load(t0, S.t, rd);
+    float cur = t0 < S.t ? kept[(int64_t)c * N + at.e] : 0.f;
+    w.template take<false>(t0, q, ms, ub, vb);
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {        // the states again; q becomes c a (h[t-1] - x[t]), the slope over the gate
       const float am = fabsf(ms[j]), xv = q[j];
       cur = memory_of<MASK>(cur, ub, j);
       q[j] = fmaf(-am, am, am) * (cur - xv);
-      if (MASK) q[j] = masked_value(q[j], bit_mask(ub & vb, j));
       cur = advance(cur, xv, ms[j]);
-      ds[j] = t0 + j < S.t ? as_value(rd[j]) : 0.f;
+      ds[j] = as_value(rd[j]);
     }
+    if (t0 + KEEP > S.t)
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j) ds[j] = t0 + j < S.t ? ds[j] : 0.f;
     float b = v;
     if (W > 1) {
       Stretch own{1.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = KEEP - 1; j >= 0; --j) {
-        own.a *= (__float_as_uint(ms[j]) >> 31) ? fabsf(ms[j]) : 1.f - ms[j];
-        own.q = advance(memory_of<MASK>(own.q, ub, j), 1.f, ms[j]);
-        own.p = memory_of<MASK>(times_a(ms[j], ds[j] + own.p), ub, j);
-      }
-      b = partners.template enter<true>(own, tw, lane, v);
+      for (int j = KEEP - 1; j >= 0; --j) own.template backward<MASK>(ds[j], ms[j], ub, j);
+      b = partners.template enter<true>(own, part.tw, lane, v);
       if (t0 >= S.t) continue;
     }
 #pragma unroll
     for (int j = KEEP - 1; j >= 0; --j) {
-      const int t = t0 + j;
-      if (t >= S.t) continue;
       const float s = ds[j] + b;
-      const float gx = masked_value(times_c(ms[j], s), MASK ? bit_mask(vb, j) : ~0u);
+      q[j] *= s;
+      if (MASK) q[j] = masked_value(q[j], bit_mask(ub & vb, j));
+      ds[j] = times_c(ms[j], s);
+      if (MASK) ds[j] = masked_value(ds[j], bit_mask(vb, j));
       b = memory_of<MASK>(times_a(ms[j], s), ub, j);
-      if (on && dxp) store_value(reinterpret_cast<V*>(dxp + (int64_t)t * S.out_t * (int64_t)sizeof(V) + mine), gx);
-      if (dgate) {
-        const float slope = s * q[j];
-        const float sum = group_sum(on && (!MASK || (ub & vb) >> j & 1) ? slope : 0.f, pos, len);
-        if (on && pos == 0) {
-          if (L.pieces > 1)
-            part[((int64_t)t * G + group) * L.pieces + (wave - group * L.pieces)] = sum;
-          else
-            store_value(dgate + t * S.dgate_t + row * S.dgate_row + gi, sum);
-        }
-      }
     }
-    if (on && dh0 && t0 == 0) dh0[e] = b;
+    if (dx) out.store(t0, S.t, at.on, ds);
+    if (dgate) {
+      if (S.share == 1)
+        single.store(t0, S.t, at.on, q);
+      else
+        sum_gates(S, A, part.wave, sums[threadIdx.x >> 6], q, at.on, t0, dgate, parts);
+    }
+    if (dh0 && at.on && t0 == 0) dh0[at.e] = b;
     if (W == 1) v = b;
   }
-}
-
-template <typename V>
-__global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int pieces, const float* __restrict__ part,
-                                                        V* __restrict__ dgate) {
-  const int64_t G = (int64_t)S.rows * S.groups;
-  const int64_t k = (int64_t)blockIdx.x * GT + threadIdx.x;
-  if (k >= G * S.t) return;
-  float s = 0.f;
-  for (int p = 0; p < pieces; ++p) s += part[k * pieces + p];
-  const int64_t t = k / G, g = k - t * G, row = g / S.groups;
-  store_value(dgate + t * S.dgate_t + row * S.dgate_row + (g - row * S.groups), s);
 }
 
 // ---------------------------------------------------------------- one frame over a cache of rows
@@ -591,94 +675,97 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
   return 0;
 }
 
-// How the time axis is shared out.  `waves` = waves that 64 lanes each would make.  A wave that walks alone needs about four
-// others on its CU to keep HBM busy; below that the workgroup's waves take turns, and where even 16 of them per 64 lanes
-// leave CUs empty the axis is cut into segments of whole tiles, at the price of reading the inputs twice.
-struct Split {
-  int w, segs, seg_tiles;
-};
-static Split split_axis(int64_t waves, int t) {
-  const int64_t stretches = t > 0 ? (t + KEEP - 1) / KEEP : 1;
-  Split p{1, 1, 1};
-  if (waves < 1024 && stretches > 1) p.w = waves >= 256 || stretches <= 4 ? 4 : 16;
-  const int64_t tiles = (stretches + p.w - 1) / p.w;
-  int64_t segs = 1;
-  if (p.w == 16 && waves > 0 && waves < 128) segs = 256 / waves;
-  if (segs > tiles / 2) segs = tiles / 2;
-  if (segs < 1) segs = 1;
-  p.seg_tiles = (int)((tiles + segs - 1) / segs);
-  p.segs = (int)((tiles + p.seg_tiles - 1) / p.seg_tiles);
+// `waves` = waves of `per` lanes.  A wave that walks alone needs about four others on its CU to keep HBM busy; below that the
+// waves of a workgroup take turns.  Fewer than 64 x 8 waves leave most of the GPU empty: an axis of more than two such
+// tiles is cut into runs then, at the price of reading the inputs twice.
+static Split split_axis(const umt_gated_shape& S, int per) {
+  const int64_t N = (int64_t)S.rows * S.groups * S.share;
+  const int all = S.t > 0 ? (S.t + KEEP - 1) / KEEP : 1;
+  Split p{per, 1, 0, 1, (N + per - 1) / per};
+  if (p.waves >= 1024 || all == 1) return p;
+  if (p.waves >= 64 || all <= 16) {
+    p.w = p.waves >= 256 || all <= 4 ? 4 : 8;
+    return p;
+  }
+  const int64_t runs = p.waves > 0 ? (1536 + p.waves - 1) / p.waves : 1;
+  p.len = (int)((all + runs - 1) / runs);
+  p.groups = (all + p.len * RUN_WAVES - 1) / (p.len * RUN_WAVES);
   return p;
 }
-static int64_t segment_floats(const umt_gated_shape& S, int64_t waves) {
-  const Split p = split_axis(waves, S.t);
-  return p.segs > 1 ? (int64_t)p.segs * 3 * S.rows * S.groups * S.share : 0;
+static int64_t run_floats(const umt_gated_shape& S, const Split& p) {
+  return p.len ? (int64_t)p.groups * (RUN_WAVES + 1) * 3 * S.rows * S.groups * S.share : 0;
 }
-static int64_t scan_waves(const umt_gated_shape& S) { return ((int64_t)S.rows * S.groups * S.share + 63) / 64; }
+// Lanes of a backward wave that own a feature: 64, or as many whole gates as fit (21 landmarks of 3 coordinates: 63 lanes)
+// where that leaves at most 4 lanes idle, so that their sums need no second launch.
+static int backward_lanes(const umt_gated_shape& S) {
+  const int whole = S.share <= 64 ? 64 / S.share * S.share : 0;
+  return whole >= 60 ? whole : 64;
+}
+// parts of a gate's sum: waves that its features may lie in, 0 where they always lie in one
+static int gate_slots(const umt_gated_shape& S, int per) { return per % S.share == 0 ? 0 : (S.share + per - 2) / per + 1; }
+static int64_t part_floats(const umt_gated_shape& S, int per) { return (int64_t)S.t * S.rows * S.groups * gate_slots(S, per); }
 
-// whether a wave's lanes lie within 2^31 bytes of each other in every stream: 64 features are at most 64 rows
+// whether 32 bits address a wave's lanes from its first row in every stream (64 features are at most 64 rows), and
+// count the features of the call
 static bool near_rows(const umt_gated_shape& S, int64_t size) {
   const int F = S.groups * S.share;
   const int64_t rows = F >= 64 ? 2 : 64 / F + 2;
-  const int64_t st[] = {S.x_row, S.gate_row, S.out_row, S.dh_row};
+  const int64_t st[] = {S.x_row, S.gate_row, S.out_row, S.dh_row, S.dgate_row};
   for (int64_t r : st)
     if (r > ((1LL << 31) / size - F) / rows) return false;
-  return true;
+  return (int64_t)S.rows * F < (1LL << 31) - 64;
 }
 
 template <typename V, typename OFF, bool MASK>
 static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* h0, V* h, float* h_last, float* kept,
-                       float* segs, hipStream_t s) {
-  const int64_t waves = scan_waves(S);
-  const Split p = split_axis(waves, S.t);
-  const float* entering = p.segs > 1 ? segs : nullptr;
-  if (p.w == 1) {
-    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 1, MASK>), dim3((unsigned)((waves + 3) / 4)), dim3(GT), 0, s, S, x, gate, mk, h0, entering,
-                       p.seg_tiles, h, h_last, kept);
+                       float* ws, hipStream_t s) {
+  const Split p = split_axis(S, 64);
+  const unsigned n = (unsigned)p.waves;
+#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                                \
+  hipLaunchKernelGGL((gated_scan_kernel<V, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, x, gate, mk, h0, ws, h, h_last, kept)
+  if (p.len) {
+    hipLaunchKernelGGL((gated_runs_kernel<V, OFF, MASK, false>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, x, S.x_t, S.x_row, gate,
+                       mk, ws);
+    UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
+  } else if (p.w == 1) {
+    UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
   } else if (p.w == 4) {
-    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 4, MASK>), dim3((unsigned)waves), dim3(256), 0, s, S, x, gate, mk, h0, entering,
-                       p.seg_tiles, h, h_last, kept);
+    UMT_SCAN(4, false, dim3(n), 256);
   } else {
-    if (p.segs > 1)
-      hipLaunchKernelGGL((gated_segment_kernel<V, OFF, 16, MASK, false>), dim3((unsigned)waves, p.segs - 1), dim3(1024), 0, s, S, x, gate, mk,
-                         p.seg_tiles, S.x_t, S.x_row, segs);
-    hipLaunchKernelGGL((gated_scan_kernel<V, OFF, 16, MASK>), dim3((unsigned)waves, p.segs), dim3(1024), 0, s, S, x, gate, mk, h0, entering,
-                       p.seg_tiles, h, h_last, kept);
+    UMT_SCAN(8, false, dim3(n), 512);
   }
+#undef UMT_SCAN
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
 template <typename V, typename OFF, bool MASK>
 static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* kept, const V* dh,
-                           const float* dh_last, V* dx, V* dgate, float* dh0, float* part, float* segs, hipStream_t s) {
-  const LaneMap L = lane_map(S);
-  const Split p = split_axis(L.waves, S.t);
-  const float* entering = p.segs > 1 ? segs : nullptr;
-  if (p.w == 1) {
-    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 1, MASK>), dim3((unsigned)((L.waves + 3) / 4)), dim3(GT), 0, s, S, L, x, gate, mk,
-                       kept, dh, dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+                           const float* dh_last, V* dx, V* dgate, float* dh0, float* parts, float* ws, hipStream_t s) {
+  const int per = backward_lanes(S), slots = gate_slots(S, per);
+  const Split p = split_axis(S, per);
+  const unsigned n = (unsigned)p.waves;
+#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                                 \
+  hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, slots, x, gate, mk, kept, dh, \
+                     dh_last, ws, dx, dgate, parts, dh0)
+  if (p.len) {
+    hipLaunchKernelGGL((gated_runs_kernel<V, OFF, MASK, true>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, dh, S.dh_t, S.dh_row, gate,
+                       mk, ws);
+    UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
+  } else if (p.w == 1) {
+    UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
   } else if (p.w == 4) {
-    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 4, MASK>), dim3((unsigned)L.waves), dim3(256), 0, s, S, L, x, gate, mk, kept, dh,
-                       dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+    UMT_SCAN(4, false, dim3(n), 256);
   } else {
-    if (p.segs > 1)
-      hipLaunchKernelGGL((gated_segment_kernel<V, OFF, 16, MASK, true>), dim3((unsigned)scan_waves(S), p.segs - 1), dim3(1024), 0, s, S, dh,
-                         gate, mk, p.seg_tiles, S.dh_t, S.dh_row, segs);
-    hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, 16, MASK>), dim3((unsigned)L.waves, p.segs), dim3(1024), 0, s, S, L, x, gate, mk,
-                       kept, dh, dh_last, entering, p.seg_tiles, dx, dgate, part, dh0);
+    UMT_SCAN(8, false, dim3(n), 512);
   }
-  if (dgate && L.pieces > 1) {
-    const int64_t n = (int64_t)S.t * S.rows * S.groups;
-    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)((n + GT - 1) / GT)), dim3(GT), 0, s, S, L.pieces, part, dgate);
+#undef UMT_SCAN
+  if (dgate && slots) {
+    const int64_t gates = (int64_t)S.t * S.rows * S.groups;
+    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)((gates + GT - 1) / GT)), dim3(GT), 0, s, S, per, slots, parts, dgate);
   }
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
-}
-
-static int64_t part_floats(const umt_gated_shape& S) {
-  const LaneMap L = lane_map(S);
-  return L.pieces > 1 ? (int64_t)S.t * S.rows * S.groups * L.pieces : 0;
 }
 
 // the kernel variants: value type, distance of the rows, masks
@@ -708,7 +795,7 @@ using namespace umt;
 
 extern "C" int64_t umt_gated_scan_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  return segment_floats(*shape, scan_waves(*shape)) * (int64_t)sizeof(float);
+  return run_floats(*shape, split_axis(*shape, 64)) * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -736,7 +823,8 @@ extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const
 
 extern "C" int64_t umt_gated_scan_backward_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  return (segment_floats(*shape, lane_map(*shape).waves) + part_floats(*shape)) * (int64_t)sizeof(float);
+  const int per = backward_lanes(*shape);
+  return (run_floats(*shape, split_axis(*shape, per)) + part_floats(*shape, per)) * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -757,11 +845,11 @@ extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void*
   UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated scan backward: workspace %lld < %lld bytes",
               (long long)workspace_bytes, (long long)need);
   const Masks mk{use_memory, valid};
-  float *part = (float*)workspace, *segs = part + part_floats(S);
+  float *part = (float*)workspace, *runs = part + part_floats(S, backward_lanes(S));
   return by_variant(S, use_memory || valid, [&](auto v, auto off, auto masked) {
     using V = decltype(v);
     return launch_backward<V, decltype(off), decltype(masked)::value>(S, (const V*)x, (const V*)gate, mk, kept, (const V*)dh, dh_last, (V*)dx,
-                                                                      (V*)dgate, dh0, part, segs, s);
+                                                                      (V*)dgate, dh0, part, runs, s);
   });
 }
 

@@ -2,8 +2,9 @@
 //
 //   h[t] = a h[t-1] + c x[t],   a = sigmoid(gate), c = 1 - a = sigmoid(-gate)
 //
-// One lane owns one (row, feature); a wave loads UMT_GATED_KEEP steps of its 64 lanes at once, so neighbouring lanes read
-// neighbouring features and 32 loads are in flight.  Where there are many lanes a wave walks the whole axis alone.  Where
+// One lane owns one (row, feature), or two neighbouring ones of bfloat16 where they can be loaded together (pairs()); a wave
+// loads UMT_GATED_KEEP steps of its 64 lanes at once, so neighbouring lanes read neighbouring features and 32 loads are in
+// flight.  Where there are many lanes a wave walks the whole axis alone.  Where
 // there are fewer, the waves of a workgroup take successive stretches of a tile (the recurrence over a stretch is itself a
 // step, see join()).  Where there are few, the axis is cut into runs, a wave each: a first launch finds the step that each
 // run is, a second one walks the runs from the states they begin with.  No order of arrival enters a result.
@@ -15,6 +16,7 @@
 // (x, m) = (0, +0), a dropped memory is m = -0 with the memory read as 0, so what lies under a mask enters nowhere.
 #include "umt_internal.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace umt {
@@ -23,8 +25,33 @@ constexpr int KEEP = UMT_GATED_KEEP;
 constexpr int GT = 256;
 constexpr int RUN_WAVES = 4;               // runs of a workgroup
 
-__device__ __forceinline__ float as_value(float v) { return v; }
-__device__ __forceinline__ float as_value(__bf16 v) { return (float)v; }
+// E values that a lane loads and stores as one
+template <typename V, int E>
+struct Values;
+template <>
+struct Values<float, 1> {
+  using Raw = float;
+  static __device__ __forceinline__ void open(Raw r, float (&v)[1]) { v[0] = r; }
+  static __device__ __forceinline__ Raw close(const float (&v)[1]) { return v[0]; }
+};
+template <>
+struct Values<__bf16, 1> {
+  using Raw = __bf16;
+  static __device__ __forceinline__ void open(Raw r, float (&v)[1]) { v[0] = (float)r; }
+  static __device__ __forceinline__ Raw close(const float (&v)[1]) { return (__bf16)v[0]; }      // one rounding, to nearest even
+};
+template <>
+struct Values<__bf16, 2> {
+  using Raw = uint32_t;
+  static __device__ __forceinline__ void open(Raw r, float (&v)[2]) {
+    v[0] = __uint_as_float(r << 16);
+    v[1] = __uint_as_float(r & 0xffff0000u);
+  }
+  static __device__ __forceinline__ Raw close(const float (&v)[2]) {
+    const __bf16 a = (__bf16)v[0], b = (__bf16)v[1];
+    return (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+  }
+};
 __device__ __forceinline__ float load_value(const float* p) { return *p; }
 __device__ __forceinline__ float load_value(const __bf16* p) { return (float)*p; }
 __device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
@@ -97,49 +124,47 @@ struct Masks {
   const uint8_t* valid;
 };
 
-template <typename P>
-__device__ __forceinline__ P uniform(P p) {                 // into scalar registers: the same in all lanes of the wave
+using Global = __attribute__((address_space(1))) char*;     // or the integers below would make them generic addresses
+__device__ __forceinline__ Global uniform(const void* p) {  // into scalar registers: the same in all lanes of the wave
   const uint64_t v = (uint64_t)p;
-  return (P)(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-             (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+  return (Global)(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                  (unsigned)__builtin_amdgcn_readfirstlane((int)v));
 }
 
 // One stream of (t, row, feature) values as a wave addresses it: a step's place is the same in all lanes, a lane adds its
 // distance from the wave's first row (OFF = 32 bits unless the rows lie further apart than that)
-template <typename V, typename OFF>
+template <typename V, int E, typename OFF>
 struct Lanes {
-  char* at;                // step 0 of the wave's first row
+  using Raw = typename Values<V, E>::Raw;
+  using At = __attribute__((address_space(1))) Raw*;
+  Global at;               // step 0 of the wave's first row
   int64_t step;            // bytes
   OFF mine;                // bytes
   __device__ __forceinline__ Lanes(const V* p, int64_t t_stride, int64_t row_stride, int64_t row0, int64_t row, int64_t inner) {
-    at = uniform((char*)(p + row0 * row_stride));
+    at = uniform(p + row0 * row_stride);
     step = t_stride * (int64_t)sizeof(V);
     mine = (OFF)(((row - row0) * row_stride + inner) * (int64_t)sizeof(V));
   }
   // steps t0 .. t0 + KEEP - 1; those past the end read the last one
-  __device__ __forceinline__ void load(int t0, int T, V (&r)[KEEP]) const {
-    const char* p = at + (t0 < T ? t0 : T - 1) * step;
-    if (t0 + KEEP <= T) {
+  __device__ __forceinline__ void load(int t0, int T, Raw (&r)[KEEP]) const {
+    Global p = at + (t0 < T ? t0 : T - 1) * step;
+    const int more = T - 1 - t0;            // steps that follow the first
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j, p += step) r[j] = *(const V*)(p + mine);
-    } else {
-#pragma unroll
-      for (int j = 0; j < KEEP; ++j) {
-        r[j] = *(const V*)(p + mine);
-        p += t0 + j + 1 < T ? step : 0;
-      }
+    for (int j = 0; j < KEEP; ++j) {
+      r[j] = *(At)(p + mine);
+      p += j < more ? step : 0;
     }
   }
-  __device__ __forceinline__ void store(int t0, int T, bool on, const float (&r)[KEEP]) const {
-    char* p = at + t0 * step;
+  __device__ __forceinline__ void store(int t0, int T, bool on, const float (&v)[KEEP][E]) const {
+    Global p = at + t0 * step;
     if (!on) return;
     if (t0 + KEEP <= T) {
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j, p += step) store_value((V*)(p + mine), r[j]);
+      for (int j = 0; j < KEEP; ++j, p += step) *(At)(p + mine) = Values<V, E>::close(v[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < KEEP; ++j, p += step)
-        if (t0 + j < T) store_value((V*)(p + mine), r[j]);
+        if (t0 + j < T) *(At)(p + mine) = Values<V, E>::close(v[j]);
     }
   }
 };
@@ -168,18 +193,18 @@ struct MaskLanes {
   }
 };
 
-// The (row, feature) of a lane.  A wave owns `per` consecutive ones, from wave * per on; lanes without one stand in for the
-// wave's first and write nothing.
-template <typename OFF>
+// The (row, feature) of a lane's first value.  A wave owns `per` consecutive values, from wave * per on; lanes without any
+// stand in for the wave's first and write nothing.
+template <int E, typename OFF>
 struct Place {
   using Index = std::conditional_t<sizeof(OFF) == 4, uint32_t, int64_t>;      // 32-bit divisions where they do
   int64_t e0, e, row0, row;
   int f, gi;
   bool on;
   __device__ __forceinline__ Place(const umt_gated_shape& S, int64_t wave, int per) {
-    const int lane = threadIdx.x & 63;
-    const Index F = (Index)(S.groups * S.share), N = (Index)S.rows * F, first = (Index)wave * (Index)per, i = first + (Index)lane;
-    on = lane < per && i < N;
+    const int mine = (threadIdx.x & 63) * E;
+    const Index F = (Index)(S.groups * S.share), N = (Index)S.rows * F, first = (Index)wave * (Index)per, i = first + (Index)mine;
+    on = mine < per && i < N;
     const Index k = on ? i : first, r0 = first / F, r = k / F;
     e0 = first;
     e = k;
@@ -190,16 +215,20 @@ struct Place {
   }
 };
 
-// The two streams that both directions go by (an input and its gate) with the masks
-template <typename V, typename OFF, bool MASK>
+// The two streams that both directions go by (an input and its gate, GE = 2 gates for 2 values, 1 for all) with the masks
+template <typename V, int E, int GE, typename OFF, bool MASK>
 struct Walk {
-  Lanes<V, OFF> x, g;
+  using X = Lanes<V, E, OFF>;
+  using G = Lanes<V, GE, OFF>;
+  X x;
+  G g;
   MaskLanes um, vm;
   int T;
-  V rx[KEEP], rg[KEEP];
+  typename X::Raw rx[KEEP];
+  typename G::Raw rg[KEEP];
   uint8_t ru, rv;
 
-  __device__ __forceinline__ Walk(const umt_gated_shape& S, const Place<OFF>& at, const V* x_, int64_t x_t, int64_t x_row, const V* gate_,
+  __device__ __forceinline__ Walk(const umt_gated_shape& S, const Place<E, OFF>& at, const V* x_, int64_t x_t, int64_t x_row, const V* gate_,
                                   const Masks& mk)
       : x(x_, x_t, x_row, at.row0, at.row, at.f), g(gate_, S.gate_t, S.gate_row, at.row0, at.row, at.gi), T(S.t) {
     if (MASK) {
@@ -222,7 +251,7 @@ struct Walk {
   // The fetched stretch: inputs, m of each step, mask bits.  Steps past the end are skipped frames.  BACK: the inputs are
   // gradients, which no valid mask covers.
   template <bool BACK>
-  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP], float (&ms)[KEEP], unsigned& ub, unsigned& vb) {
+  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP][E], float (&ms)[KEEP][GE], unsigned& ub, unsigned& vb) {
     ub = vb = 0xffffu;
     if (MASK) {
       if (um.p) ub = um.bits(ru, t0, T);
@@ -234,15 +263,19 @@ struct Walk {
     vb &= ~past;
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-      xs[j] = as_value(rx[j]);
-      ms[j] = gate_step(as_value(rg[j]));
+      Values<V, E>::open(rx[j], xs[j]);
+      Values<V, GE>::open(rg[j], ms[j]);
+#pragma unroll
+      for (int i = 0; i < GE; ++i) ms[j][i] = gate_step(ms[j][i]);
     }
     if (MASK || left < KEEP) {
 #pragma unroll
       for (int j = 0; j < KEEP; ++j) {
-        const unsigned v = bit_mask(vb, j);
-        xs[j] = masked_value(xs[j], BACK ? ~bit_mask(past, j) : v);
-        ms[j] = masked_step(ms[j], bit_mask(ub, j), v);
+        const unsigned v = bit_mask(vb, j), u = bit_mask(ub, j);
+#pragma unroll
+        for (int i = 0; i < E; ++i) xs[j][i] = masked_value(xs[j][i], BACK ? ~bit_mask(past, j) : v);
+#pragma unroll
+        for (int i = 0; i < GE; ++i) ms[j][i] = masked_step(ms[j][i], u, v);
       }
     }
   }
@@ -250,37 +283,43 @@ struct Walk {
 
 // Partners: the W waves of a workgroup take the KEEP-step stretches of a tile in turn; each hands its stretch over in LDS and
 // joins those before it (after it, in the backward direction) to the state that entered the tile.
-template <int W>
+template <int W, int E>
 struct Partners {
-  float (*lds)[W][3][64];
+  float (*lds)[W][3 * E][64];
   int turn = 0;
-  // state before this wave's stretch; `through` becomes the state behind the tile
+  // `own`: state before this wave's stretch; `through` becomes the state behind the tile
   template <bool BACK>
-  __device__ __forceinline__ float enter(const Stretch& mine, int tw, int lane, float& through) {
-    float(*b)[3][64] = lds[turn];
+  __device__ __forceinline__ void enter(const Stretch (&mine)[E], int tw, int lane, float (&through)[E], float (&own)[E]) {
+    float(*b)[3 * E][64] = lds[turn];
     turn ^= 1;                              // two places: one barrier a tile
-    b[tw][0][lane] = mine.a;
-    b[tw][1][lane] = mine.q;
-    b[tw][2][lane] = mine.p;
-    __syncthreads();
-    float cur = through, own = through;
-    for (int i = 0; i < W; ++i) {
-      const int w = BACK ? W - 1 - i : i;
-      if (w == tw) own = cur;
-      cur = join(cur, Stretch{b[w][0][lane], b[w][1][lane], b[w][2][lane]});
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      b[tw][3 * i][lane] = mine[i].a;
+      b[tw][3 * i + 1][lane] = mine[i].q;
+      b[tw][3 * i + 2][lane] = mine[i].p;
     }
-    through = cur;
-    return own;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float cur = through[i];
+      own[i] = cur;
+      for (int n = 0; n < W; ++n) {
+        const int w = BACK ? W - 1 - n : n;
+        if (w == tw) own[i] = cur;
+        cur = join(cur, Stretch{b[w][3 * i][lane], b[w][3 * i + 1][lane], b[w][3 * i + 2][lane]});
+      }
+      through[i] = cur;
+    }
   }
 };
 
 // How a call is shared out (split_axis)
 struct Split {
-  int per;                 // lanes of a wave that own a feature
+  int per;                 // values of a wave
   int w;                   // waves that share a tile, 1: a wave walks alone
   int len;                 // stretches of a run, 0: the axis is not cut
   int groups;              // workgroups along the axis
-  int64_t waves;           // of `per` lanes
+  int64_t waves;           // of `per` values
 };
 
 // Where a wave works: its lanes' wave, its first stretch, how many stretches, the distance between them
@@ -315,69 +354,86 @@ __device__ __forceinline__ void store_stretch(float* s, int64_t N, int64_t e, co
 }
 
 // The step that each run is (BACK: of the gradient that comes from behind)
-template <typename V, typename OFF, bool MASK, bool BACK>
+template <typename V, int E, int GE, typename OFF, bool MASK, bool BACK>
 __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_shape S, Split P, const V* __restrict__ v, int64_t v_t, int64_t v_row,
                                                                     const V* __restrict__ gate, Masks mk, float* __restrict__ ws) {
-  __shared__ float lds[RUN_WAVES][3][64];
+  __shared__ float lds[RUN_WAVES][3 * E][64];
   const int lane = threadIdx.x & 63;
   const Part<1, true> part(P, S.t);
-  const Place<OFF> at(S, part.wave, P.per);
+  const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, OFF, MASK> w(S, at, v, v_t, v_row, gate, mk);
-  Stretch own{1.f, 0.f, 0.f};
+  Walk<V, E, GE, OFF, MASK> w(S, at, v, v_t, v_row, gate, mk);
+  Stretch own[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
   const int last = part.first + part.count - 1;
   if (part.count > 0) w.fetch((BACK ? last : part.first) * KEEP);
   for (int k = 0; k < part.count; ++k) {
     const int t0 = (BACK ? last - k : part.first + k) * KEEP;
-    float xs[KEEP], ms[KEEP];
+    float xs[KEEP][E], ms[KEEP][GE];
     unsigned ub, vb;
     w.template take<BACK>(t0, xs, ms, ub, vb);
     if (k + 1 < part.count) w.fetch(BACK ? t0 - KEEP : t0 + KEEP);
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int j = BACK ? KEEP - 1 - i : i;
-      if (BACK)
-        own.template backward<MASK>(xs[j], ms[j], ub, j);
-      else
-        own.template forward<MASK>(xs[j], ms[j], ub, j);
+    for (int n = 0; n < KEEP; ++n) {
+      const int j = BACK ? KEEP - 1 - n : n;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (BACK)
+          own[i].template backward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
+        else
+          own[i].template forward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
+      }
     }
   }
-  lds[part.tw][0][lane] = own.a;
-  lds[part.tw][1][lane] = own.q;
-  lds[part.tw][2][lane] = own.p;
-  if (at.on) store_stretch(run_at(ws, N, blockIdx.y * RUN_WAVES + part.tw), N, at.e, own);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    lds[part.tw][3 * i][lane] = own[i].a;
+    lds[part.tw][3 * i + 1][lane] = own[i].q;
+    lds[part.tw][3 * i + 2][lane] = own[i].p;
+    if (at.on) store_stretch(run_at(ws, N, blockIdx.y * RUN_WAVES + part.tw), N, at.e + i, own[i]);
+  }
   __syncthreads();
   if (part.tw != 0 || !at.on) return;
-  Stretch all{1.f, 0.f, 0.f};
-  for (int i = 0; i < RUN_WAVES; ++i) {
-    const int k = BACK ? RUN_WAVES - 1 - i : i;
-    all = then(all, Stretch{lds[k][0][lane], lds[k][1][lane], lds[k][2][lane]});
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    Stretch all{1.f, 0.f, 0.f};
+    for (int n = 0; n < RUN_WAVES; ++n) {
+      const int k = BACK ? RUN_WAVES - 1 - n : n;
+      all = then(all, Stretch{lds[k][3 * i][lane], lds[k][3 * i + 1][lane], lds[k][3 * i + 2][lane]});
+    }
+    store_stretch(run_at(ws, N, P.groups * RUN_WAVES + blockIdx.y), N, at.e + i, all);
   }
-  store_stretch(run_at(ws, N, P.groups * RUN_WAVES + blockIdx.y), N, at.e, all);
 }
 
 // State with which this wave's run begins: the workgroups before it (BACK: behind it) are joined by the waves, a quarter
 // each, then the runs before it in its own
-template <bool BACK>
-__device__ __forceinline__ float enter_run(const float* ws, const Split& P, int64_t N, int64_t e, int tw, int lane, float first,
-                                           Partners<RUN_WAVES>& partners) {
+template <bool BACK, int E>
+__device__ __forceinline__ void enter_run(const float* ws, const Split& P, int64_t N, int64_t e, int tw, int lane, float (&h)[E],
+                                          Partners<RUN_WAVES, E>& partners) {
   const int group = blockIdx.y, count = BACK ? P.groups - 1 - group : group, each = (count + RUN_WAVES - 1) / RUN_WAVES;
   const int i0 = min(count, tw * each), i1 = min(count, i0 + each);
   const float* joined = ws + (int64_t)P.groups * RUN_WAVES * 3 * N;
-  Stretch run{1.f, 0.f, 0.f};
+  Stretch run[E], near[RUN_WAVES][E];
+#pragma unroll
+  for (int k = 0; k < RUN_WAVES; ++k)
+#pragma unroll
+    for (int i = 0; i < E; ++i) near[k][i] = load_stretch(ws + (int64_t)(group * RUN_WAVES + k) * 3 * N, N, e + i);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    run[i] = {1.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = i0; i < i1; ++i) run = then(run, load_stretch(joined + (int64_t)(BACK ? P.groups - 1 - i : i) * 3 * N, N, e));
-  Stretch near[RUN_WAVES];
-#pragma unroll
-  for (int k = 0; k < RUN_WAVES; ++k) near[k] = load_stretch(ws + (int64_t)(group * RUN_WAVES + k) * 3 * N, N, e);
-  float h = first;
-  partners.template enter<false>(run, tw, lane, h);
-#pragma unroll
-  for (int i = 0; i < RUN_WAVES; ++i) {
-    const int k = BACK ? RUN_WAVES - 1 - i : i;
-    if (BACK ? k > tw : k < tw) h = join(h, near[k]);
+    for (int n = i0; n < i1; ++n) run[i] = then(run[i], load_stretch(joined + (int64_t)(BACK ? P.groups - 1 - n : n) * 3 * N, N, e + i));
   }
-  return h;
+  float unused[E];
+  partners.template enter<false>(run, tw, lane, h, unused);
+#pragma unroll
+  for (int n = 0; n < RUN_WAVES; ++n) {
+    const int k = BACK ? RUN_WAVES - 1 - n : n;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (BACK ? k > tw : k < tw) h[i] = join(h[i], near[k][i]);
+  }
 }
 
 template <int W, bool RUNS>
@@ -385,50 +441,67 @@ constexpr int partner_waves() { return RUNS ? RUN_WAVES : W; }
 template <int W, bool RUNS>
 constexpr int group_threads() { return RUNS ? 64 * RUN_WAVES : W == 1 ? GT : 64 * W; }
 
-template <typename V, typename OFF, int W, bool MASK, bool RUNS>
+template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
 __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(umt_gated_shape S, Split P, const V* __restrict__ x,
-                                                                              const V* __restrict__ gate, Masks mk,
-                                                                              const float* __restrict__ h0, const float* __restrict__ ws,
-                                                                              V* __restrict__ h, float* __restrict__ h_last,
-                                                                              float* __restrict__ kept) {
+                                                                                const V* __restrict__ gate, Masks mk,
+                                                                                const float* __restrict__ h0, const float* __restrict__ ws,
+                                                                                V* __restrict__ h, float* __restrict__ h_last,
+                                                                                float* __restrict__ kept) {
   constexpr int PW = partner_waves<W, RUNS>();
-  __shared__ float lds[PW > 1 ? 2 : 1][PW][3][64];
+  __shared__ float lds[PW > 1 ? 2 : 1][PW][3 * E][64];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
   if (W == 1 && !RUNS && part.wave >= P.waves) return;
-  const Place<OFF> at(S, part.wave, P.per);
+  const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
-  const Lanes<V, OFF> out(h, S.out_t, S.out_row, at.row0, at.row, at.f);
+  Walk<V, E, GE, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  const Lanes<V, E, OFF> out(h, S.out_t, S.out_row, at.row0, at.row, at.f);
   if (part.count > 0) w.fetch(part.first * KEEP);
-  Partners<PW> partners{reinterpret_cast<float(*)[PW][3][64]>(lds)};
-  float cur = h0 ? h0[at.e] : 0.f;
-  if constexpr (RUNS) cur = enter_run<false>(ws, P, N, at.e, part.tw, lane, cur, partners);
+  Partners<PW, E> partners{reinterpret_cast<float(*)[PW][3 * E][64]>(lds)};
+  float cur[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) cur[i] = h0 ? h0[at.e + i] : 0.f;
+  if constexpr (RUNS) enter_run<false>(ws, P, N, at.e, part.tw, lane, cur, partners);
   for (int k = 0; k < part.count; ++k) {
     const int c = part.first + k * part.by, t0 = c * KEEP;
-    float xs[KEEP], ms[KEEP];
+    float xs[KEEP][E], ms[KEEP][GE], st[E];
     unsigned ub, vb;
     w.template take<false>(t0, xs, ms, ub, vb);
     if (k + 1 < part.count) w.fetch(t0 + part.by * KEEP);
-    float st = cur;
     if (W > 1) {
-      Stretch own{1.f, 0.f, 0.f};
+      Stretch own[E];
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j) own.template forward<MASK>(xs[j], ms[j], ub, j);
-      st = partners.template enter<false>(own, part.tw, lane, cur);
+      for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j)
+#pragma unroll
+        for (int i = 0; i < E; ++i) own[i].template forward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
+      partners.template enter<false>(own, part.tw, lane, cur, st);
       if (t0 >= S.t) continue;
-    }
-    if (kept && at.on) kept[(int64_t)c * N + at.e] = st;
+    } else {
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) xs[j] = st = advance(memory_of<MASK>(st, ub, j), xs[j], ms[j]);
+      for (int i = 0; i < E; ++i) st[i] = cur[i];
+    }
+    if (kept && at.on)
+#pragma unroll
+      for (int i = 0; i < E; ++i) kept[(int64_t)c * N + at.e + i] = st[i];
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j)
+#pragma unroll
+      for (int i = 0; i < E; ++i) xs[j][i] = st[i] = advance(memory_of<MASK>(st[i], ub, j), xs[j][i], ms[j][i % GE]);
     out.store(t0, S.t, at.on, xs);
-    if (h_last && at.on && t0 + KEEP >= S.t) h_last[at.e] = st;
-    if (W == 1) cur = st;
+    if (h_last && at.on && t0 + KEEP >= S.t)
+#pragma unroll
+      for (int i = 0; i < E; ++i) h_last[at.e + i] = st[i];
+    if (W == 1)
+#pragma unroll
+      for (int i = 0; i < E; ++i) cur[i] = st[i];
   }
 }
 
 // ---------------------------------------------------------------- backward
-// Sums over the features of a gate.  A wave's lanes hold consecutive features, so a gate's are a run of lanes.  The KEEP
+// Sums over the features of a gate.  A wave's lanes hold consecutive features, so a gate's are a run of lanes (a lane's own
+// two are added first; `share` and `per` count lanes here).  The KEEP
 // steps' products go through the wave's own LDS rows; lane 16 k + j adds up step j: whole gates k, k + 4, ... where the
 // wave holds many, a quarter of each where it holds few.  A gate that reaches into other waves leaves its part in `part`, and
 // a second launch adds the parts in order.
@@ -436,22 +509,22 @@ constexpr int SUM_ROW = 65;                // floats of a step's row: the 16 ste
 
 struct GateSums {
   int64_t G, group0;       // gates of a step, the wave's first
-  int count, lead, per;    // gates that the wave holds, features of the first that lie before it, lanes
-  int slots;
+  int count, lead, per;    // gates that the wave holds, lanes of the first that lie before it, lanes
+  int share, slots;
 };
 
 template <typename V>
-__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, int64_t wave, float* rows, const float (&v)[KEEP], bool on,
+__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, int64_t wave, float* rows, const float (&v)[KEEP][1], bool on,
                                           int t0, V* __restrict__ dgate, float* __restrict__ part) {
   const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4, t = t0 + j;
 #pragma unroll
-  for (int i = 0; i < KEEP; ++i) rows[i * SUM_ROW + lane] = on ? v[i] : 0.f;
+  for (int i = 0; i < KEEP; ++i) rows[i * SUM_ROW + lane] = on ? v[i][0] : 0.f;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   const float* row = rows + j * SUM_ROW;
   const bool many = A.count > 6;
   for (int k = many ? k0 : 0; k < A.count; k += many ? 4 : 1) {
-    const int lo = max(0, k * S.share - A.lead), hi = min(A.per, (k + 1) * S.share - A.lead), n = hi - lo;
+    const int lo = max(0, k * A.share - A.lead), hi = min(A.per, (k + 1) * A.share - A.lead), n = hi - lo;
     float s = 0.f;
     if (many) {
       for (int i = lo; i < hi; ++i) s += row[i];
@@ -463,11 +536,11 @@ __device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSu
     }
     const int64_t group = A.group0 + k;
     if (t < S.t && group < A.G && (many || k0 == 0)) {
-      if (n == S.share) {
+      if (n == A.share) {
         const int64_t r = group / S.groups;
         store_value(dgate + t * S.dgate_t + r * S.dgate_row + (group - r * S.groups), s);
       } else {
-        part[((int64_t)t * A.G + group) * A.slots + (wave - group * S.share / A.per)] = s;
+        part[((int64_t)t * A.G + group) * A.slots + (wave - group * A.share / A.per)] = s;
       }
     }
   }
@@ -489,78 +562,108 @@ __global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int p
   store_value(dgate + t * S.dgate_t + row * S.dgate_row + (g - row * S.groups), s);
 }
 
-template <typename V, typename OFF, int W, bool MASK, bool RUNS>
+template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
 __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backward_kernel(
     umt_gated_shape S, Split P, int slots, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
     const V* __restrict__ dh, const float* __restrict__ dh_last, const float* __restrict__ ws, V* __restrict__ dx, V* __restrict__ dgate,
     float* __restrict__ parts, float* __restrict__ dh0) {
   constexpr int PW = partner_waves<W, RUNS>(), GW = group_threads<W, RUNS>() / 64;
-  __shared__ float lds[PW > 1 ? 2 : 1][PW][3][64];
+  __shared__ float lds[PW > 1 ? 2 : 1][PW][3 * E][64];
   __shared__ float sums[GW][KEEP * SUM_ROW];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
   if (W == 1 && !RUNS && part.wave >= P.waves) return;
-  const Place<OFF> at(S, part.wave, P.per);
+  const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
-  const Lanes<V, OFF> d(dh, S.dh_t, S.dh_row, at.row0, at.row, at.f), out(dx, S.out_t, S.out_row, at.row0, at.row, at.f);
-  const Lanes<V, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
-  GateSums A;
-  A.G = (int64_t)S.rows * S.groups;
-  A.group0 = at.e0 / S.share;
-  A.lead = (int)(at.e0 - A.group0 * S.share);
-  A.per = P.per;
-  A.slots = slots;
-  A.count = (A.lead + P.per + S.share - 1) / S.share;
-  Partners<PW> partners{reinterpret_cast<float(*)[PW][3][64]>(lds)};
-  float v = dh_last ? dh_last[at.e] : 0.f;
-  if constexpr (RUNS) v = enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
+  Walk<V, E, GE, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  const Lanes<V, E, OFF> d(dh, S.dh_t, S.dh_row, at.row0, at.row, at.f), out(dx, S.out_t, S.out_row, at.row0, at.row, at.f);
+  Partners<PW, E> partners{reinterpret_cast<float(*)[PW][3 * E][64]>(lds)};
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = dh_last ? dh_last[at.e + i] : 0.f;
+  if constexpr (RUNS) enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
   for (int k = part.count - 1; k >= 0; --k) {
     const int c = part.first + k * part.by, t0 = c * KEEP;
-    float q[KEEP], ms[KEEP], ds[KEEP];
+    float q[KEEP][E], ms[KEEP][GE], ds[KEEP][E], cur[E];
     unsigned ub, vb;
-    V rd[KEEP];
+    typename Lanes<V, E, OFF>::Raw rd[KEEP];
     w.fetch(t0);
     d.load(t0, S.t, rd);
-    float cur = t0 < S.t ? kept[(int64_t)c * N + at.e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) cur[i] = t0 < S.t ? kept[(int64_t)c * N + at.e + i] : 0.f;
     w.template take<false>(t0, q, ms, ub, vb);
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {        // the states again; q becomes c a (h[t-1] - x[t]), the slope over the gate
-      const float am = fabsf(ms[j]), xv = q[j];
-      cur = memory_of<MASK>(cur, ub, j);
-      q[j] = fmaf(-am, am, am) * (cur - xv);
-      cur = advance(cur, xv, ms[j]);
-      ds[j] = as_value(rd[j]);
+      Values<V, E>::open(rd[j], ds[j]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float m = ms[j][i % GE], am = fabsf(m), xv = q[j][i];
+        cur[i] = memory_of<MASK>(cur[i], ub, j);
+        q[j][i] = fmaf(-am, am, am) * (cur[i] - xv);
+        cur[i] = advance(cur[i], xv, m);
+      }
     }
     if (t0 + KEEP > S.t)
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j) ds[j] = t0 + j < S.t ? ds[j] : 0.f;
-    float b = v;
-    if (W > 1) {
-      Stretch own{1.f, 0.f, 0.f};
+      for (int j = 0; j < KEEP; ++j)
 #pragma unroll
-      for (int j = KEEP - 1; j >= 0; --j) own.template backward<MASK>(ds[j], ms[j], ub, j);
-      b = partners.template enter<true>(own, part.tw, lane, v);
+        for (int i = 0; i < E; ++i) ds[j][i] = t0 + j < S.t ? ds[j][i] : 0.f;
+    float b[E];
+    if (W > 1) {
+      Stretch own[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = KEEP - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = 0; i < E; ++i) own[i].template backward<MASK>(ds[j][i], ms[j][i % GE], ub, j);
+      partners.template enter<true>(own, part.tw, lane, v, b);
       if (t0 >= S.t) continue;
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) b[i] = v[i];
     }
+    float slope[KEEP][GE];
 #pragma unroll
     for (int j = KEEP - 1; j >= 0; --j) {
-      const float s = ds[j] + b;
-      q[j] *= s;
-      if (MASK) q[j] = masked_value(q[j], bit_mask(ub & vb, j));
-      ds[j] = times_c(ms[j], s);
-      if (MASK) ds[j] = masked_value(ds[j], bit_mask(vb, j));
-      b = memory_of<MASK>(times_a(ms[j], s), ub, j);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float m = ms[j][i % GE], s = ds[j][i] + b[i], l = s * q[j][i];
+        if (i < GE)
+          slope[j][i] = l;
+        else
+          slope[j][0] += l;
+        ds[j][i] = times_c(m, s);
+        if (MASK) ds[j][i] = masked_value(ds[j][i], bit_mask(vb, j));
+        b[i] = memory_of<MASK>(times_a(m, s), ub, j);
+      }
+      if (MASK)
+#pragma unroll
+        for (int i = 0; i < GE; ++i) slope[j][i] = masked_value(slope[j][i], bit_mask(ub & vb, j));
     }
     if (dx) out.store(t0, S.t, at.on, ds);
     if (dgate) {
-      if (S.share == 1)
-        single.store(t0, S.t, at.on, q);
-      else
-        sum_gates(S, A, part.wave, sums[threadIdx.x >> 6], q, at.on, t0, dgate, parts);
+      if (S.share == 1) {
+        const Lanes<V, GE, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
+        single.store(t0, S.t, at.on, slope);
+      } else if constexpr (GE == 1) {
+        GateSums A;
+        A.G = (int64_t)S.rows * S.groups;
+        A.share = S.share / E;
+        A.per = P.per / E;
+        A.group0 = at.e0 / S.share;
+        A.lead = (int)(at.e0 - A.group0 * S.share) / E;
+        A.slots = slots;
+        A.count = (A.lead + A.per + A.share - 1) / A.share;
+        sum_gates(S, A, part.wave, sums[threadIdx.x >> 6], slope, at.on, t0, dgate, parts);
+      }
     }
-    if (dh0 && at.on && t0 == 0) dh0[at.e] = b;
-    if (W == 1) v = b;
+    if (dh0 && at.on && t0 == 0)
+#pragma unroll
+      for (int i = 0; i < E; ++i) dh0[at.e + i] = b[i];
+    if (W == 1)
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = b[i];
   }
 }
 
@@ -675,9 +778,9 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
   return 0;
 }
 
-// `waves` = waves of `per` lanes.  A wave that walks alone needs about four others on its CU to keep HBM busy; below that the
-// waves of a workgroup take turns.  Fewer than 64 x 8 waves leave most of the GPU empty: an axis of more than two such
-// tiles is cut into runs then, at the price of reading the inputs twice.
+// How the axis is shared out, for waves of `per` values.  A wave that walks alone needs about four others on its CU to keep
+// HBM busy; below that the waves of a workgroup take turns.  Fewer than 64 x 8 waves leave most of the GPU empty: an axis
+// of more than two such tiles is cut into runs then, at the price of reading the inputs twice.
 static Split split_axis(const umt_gated_shape& S, int per) {
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   const int all = S.t > 0 ? (S.t + KEEP - 1) / KEEP : 1;
@@ -692,40 +795,53 @@ static Split split_axis(const umt_gated_shape& S, int per) {
   p.groups = (all + p.len * RUN_WAVES - 1) / (p.len * RUN_WAVES);
   return p;
 }
-static int64_t run_floats(const umt_gated_shape& S, const Split& p) {
+static int64_t run_floats(const umt_gated_shape& S, int per) {
+  const Split p = split_axis(S, per);
   return p.len ? (int64_t)p.groups * (RUN_WAVES + 1) * 3 * S.rows * S.groups * S.share : 0;
 }
-// Lanes of a backward wave that own a feature: 64, or as many whole gates as fit (21 landmarks of 3 coordinates: 63 lanes)
-// where that leaves at most 4 lanes idle, so that their sums need no second launch.
-static int backward_lanes(const umt_gated_shape& S) {
-  const int whole = S.share <= 64 ? 64 / S.share * S.share : 0;
-  return whole >= 60 ? whole : 64;
+// Values of a backward wave whose lanes hold E: 64 E, or as many whole gates as fit (21 landmarks of 3 coordinates: 63
+// lanes) where that leaves at most 4 lanes idle, so that their sums need no second launch.
+static int backward_values(const umt_gated_shape& S, int E) {
+  const int share = S.share / E, whole = share > 0 && share <= 64 ? 64 / share * share : 0;
+  return (whole >= 60 ? whole : 64) * E;
 }
 // parts of a gate's sum: waves that its features may lie in, 0 where they always lie in one
 static int gate_slots(const umt_gated_shape& S, int per) { return per % S.share == 0 ? 0 : (S.share + per - 2) / per + 1; }
 static int64_t part_floats(const umt_gated_shape& S, int per) { return (int64_t)S.t * S.rows * S.groups * gate_slots(S, per); }
 
-// whether 32 bits address a wave's lanes from its first row in every stream (64 features are at most 64 rows), and
+// Whether lanes can hold two values: they, and the gates where every feature has its own, lie in pairs at even places.
+// 4-byte loads in the place of 2-byte ones: scan_features (512 x 512 x 648) 267 -> %PAIR% us.
+static bool pairable(const umt_gated_shape& S) {
+  return S.dtype == UMT_VALUES_BF16 && S.groups * S.share % 2 == 0 && (S.share == 1 || S.share % 2 == 0);
+}
+static bool even(int64_t a, int64_t b, const void* p) { return a % 2 == 0 && b % 2 == 0 && (uint64_t)p % 4 == 0; }
+static bool pairs(const umt_gated_shape& S, const void* x, const void* gate, const void* out, const void* dh, const void* dgate) {
+  return pairable(S) && even(S.x_t, S.x_row, x) && even(S.out_t, S.out_row, out) && (!dh || even(S.dh_t, S.dh_row, dh)) &&
+         (S.share > 1 || (even(S.gate_t, S.gate_row, gate) && (!dgate || even(S.dgate_t, S.dgate_row, dgate))));
+}
+
+// whether 32 bits address a wave's lanes from its first row in every stream (128 features are at most 128 rows), and
 // count the features of the call
 static bool near_rows(const umt_gated_shape& S, int64_t size) {
   const int F = S.groups * S.share;
-  const int64_t rows = F >= 64 ? 2 : 64 / F + 2;
+  const int64_t rows = F >= 128 ? 2 : 128 / F + 2;
   const int64_t st[] = {S.x_row, S.gate_row, S.out_row, S.dh_row, S.dgate_row};
   for (int64_t r : st)
     if (r > ((1LL << 31) / size - F) / rows) return false;
-  return (int64_t)S.rows * F < (1LL << 31) - 64;
+  return (int64_t)S.rows * F < (1LL << 31) - 128;
 }
 
-template <typename V, typename OFF, bool MASK>
+template <typename V, int E, int GE, typename OFF, bool MASK>
 static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* h0, V* h, float* h_last, float* kept,
                        float* ws, hipStream_t s) {
-  const Split p = split_axis(S, 64);
+  const Split p = split_axis(S, 64 * E);
   const unsigned n = (unsigned)p.waves;
-#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                                \
-  hipLaunchKernelGGL((gated_scan_kernel<V, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, x, gate, mk, h0, ws, h, h_last, kept)
+#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                              \
+  hipLaunchKernelGGL((gated_scan_kernel<V, E, GE, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, x, gate, mk, h0, ws, h, h_last, \
+                     kept)
   if (p.len) {
-    hipLaunchKernelGGL((gated_runs_kernel<V, OFF, MASK, false>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, x, S.x_t, S.x_row, gate,
-                       mk, ws);
+    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, false>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, x, S.x_t, S.x_row,
+                       gate, mk, ws);
     UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
   } else if (p.w == 1) {
     UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
@@ -739,18 +855,19 @@ static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Mask
   return 0;
 }
 
-template <typename V, typename OFF, bool MASK>
+template <typename V, int E, int GE, typename OFF, bool MASK>
 static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* kept, const V* dh,
-                           const float* dh_last, V* dx, V* dgate, float* dh0, float* parts, float* ws, hipStream_t s) {
-  const int per = backward_lanes(S), slots = gate_slots(S, per);
+                           const float* dh_last, V* dx, V* dgate, float* dh0, float* ws, hipStream_t s) {
+  const int per = backward_values(S, E), slots = gate_slots(S, per);
   const Split p = split_axis(S, per);
   const unsigned n = (unsigned)p.waves;
-#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                                 \
-  hipLaunchKernelGGL((gated_scan_backward_kernel<V, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, slots, x, gate, mk, kept, dh, \
-                     dh_last, ws, dx, dgate, parts, dh0)
+  float* parts = ws + run_floats(S, per);
+#define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                               \
+  hipLaunchKernelGGL((gated_scan_backward_kernel<V, E, GE, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, slots, x, gate, mk, kept, \
+                     dh, dh_last, ws, dx, dgate, parts, dh0)
   if (p.len) {
-    hipLaunchKernelGGL((gated_runs_kernel<V, OFF, MASK, true>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, dh, S.dh_t, S.dh_row, gate,
-                       mk, ws);
+    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, true>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, dh, S.dh_t,
+                       S.dh_row, gate, mk, ws);
     UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
   } else if (p.w == 1) {
     UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
@@ -768,15 +885,19 @@ static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, 
   return 0;
 }
 
-// the kernel variants: value type, distance of the rows, masks
+template <int N>
+using Count = std::integral_constant<int, N>;
+// the kernel variants: value type, values and gates of a lane, distance of the rows, masks
 template <typename Call>
-static int by_variant(const umt_gated_shape& S, bool masks, Call call) {
+static int by_variant(const umt_gated_shape& S, bool two, bool masks, Call call) {
   const bool near = near_rows(S, S.dtype == UMT_VALUES_BF16 ? 2 : 4);
-  auto typed = [&](auto v) {
-    if (near) return masks ? call(v, (uint32_t)0, std::true_type()) : call(v, (uint32_t)0, std::false_type());
-    return masks ? call(v, (uint64_t)0, std::true_type()) : call(v, (uint64_t)0, std::false_type());
+  auto typed = [&](auto v, auto e, auto ge) {
+    if (near) return masks ? call(v, e, ge, (uint32_t)0, std::true_type()) : call(v, e, ge, (uint32_t)0, std::false_type());
+    return masks ? call(v, e, ge, (uint64_t)0, std::true_type()) : call(v, e, ge, (uint64_t)0, std::false_type());
   };
-  return S.dtype == UMT_VALUES_BF16 ? typed((__bf16)0.f) : typed(0.f);
+  if (S.dtype == UMT_VALUES_F32) return typed(0.f, Count<1>(), Count<1>());
+  if (!two) return typed((__bf16)0.f, Count<1>(), Count<1>());
+  return S.share == 1 ? typed((__bf16)0.f, Count<2>(), Count<2>()) : typed((__bf16)0.f, Count<2>(), Count<1>());
 }
 
 template <typename V>
@@ -795,7 +916,9 @@ using namespace umt;
 
 extern "C" int64_t umt_gated_scan_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  return run_floats(*shape, split_axis(*shape, 64)) * (int64_t)sizeof(float);
+  int64_t n = run_floats(*shape, 64);                       // whichever way the tensors' places allow
+  if (pairable(*shape)) n = std::max(n, run_floats(*shape, 128));
+  return n * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -814,17 +937,21 @@ extern "C" int umt_gated_scan(const umt_gated_shape* shape, const void* x, const
   UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated scan: workspace %lld < %lld bytes",
               (long long)workspace_bytes, (long long)need);
   const Masks mk{use_memory, valid};
-  return by_variant(S, use_memory || valid, [&](auto v, auto off, auto masked) {
+  return by_variant(S, pairs(S, x, gate, h, nullptr, nullptr), use_memory || valid, [&](auto v, auto e, auto ge, auto off, auto masked) {
     using V = decltype(v);
-    return launch_scan<V, decltype(off), decltype(masked)::value>(S, (const V*)x, (const V*)gate, mk, h0, (V*)h, h_last, kept,
-                                                                  (float*)workspace, s);
+    return launch_scan<V, decltype(e)::value, decltype(ge)::value, decltype(off), decltype(masked)::value>(
+        S, (const V*)x, (const V*)gate, mk, h0, (V*)h, h_last, kept, (float*)workspace, s);
   });
 }
 
 extern "C" int64_t umt_gated_scan_backward_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  const int per = backward_lanes(*shape);
-  return (run_floats(*shape, split_axis(*shape, per)) + part_floats(*shape, per)) * (int64_t)sizeof(float);
+  int64_t n = 0;
+  for (int E = 1; E <= (pairable(*shape) ? 2 : 1); ++E) {
+    const int per = backward_values(*shape, E);
+    n = std::max(n, run_floats(*shape, per) + part_floats(*shape, per));
+  }
+  return n * (int64_t)sizeof(float);
 }
 
 extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
@@ -845,11 +972,10 @@ extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void*
   UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated scan backward: workspace %lld < %lld bytes",
               (long long)workspace_bytes, (long long)need);
   const Masks mk{use_memory, valid};
-  float *part = (float*)workspace, *runs = part + part_floats(S, backward_lanes(S));
-  return by_variant(S, use_memory || valid, [&](auto v, auto off, auto masked) {
+  return by_variant(S, pairs(S, x, gate, dx, dh, dgate), use_memory || valid, [&](auto v, auto e, auto ge, auto off, auto masked) {
     using V = decltype(v);
-    return launch_backward<V, decltype(off), decltype(masked)::value>(S, (const V*)x, (const V*)gate, mk, kept, (const V*)dh, dh_last, (V*)dx,
-                                                                      (V*)dgate, dh0, part, runs, s);
+    return launch_backward<V, decltype(e)::value, decltype(ge)::value, decltype(off), decltype(masked)::value>(
+        S, (const V*)x, (const V*)gate, mk, kept, (const V*)dh, dh_last, (V*)dx, (V*)dgate, dh0, (float*)workspace, s);
   });
 }
 

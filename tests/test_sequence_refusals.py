@@ -82,7 +82,8 @@ def test_row_arguments():
         assert L.umt_rows_copy_workspace_bytes(arr, k, 8, 1) == -1
     assert L.umt_rows_copy(None, 1, 8, P, P, 1, None, P, big, None) == 1
     assert L.umt_rows_copy(good, n, 8, P, P, -1, None, P, big, None) == 1 and L.umt_rows_copy(good, n, 8, None, P, 1, None, P, big, None) == 1
-    assert L.umt_rows_copy(good, n, 8, P, P, 1, None, P, L.umt_rows_copy_workspace_bytes(good, n, 8, 1) - 1, None) == 5
+    assert L.umt_rows_copy(good, n, 8, P, P, 5000, None, P, L.umt_rows_copy_workspace_bytes(good, n, 8, 5000) - 1, None) == 5
+    assert L.umt_rows_copy_workspace_bytes(good, n, 8, 5000) >= 5000 * 80
     assert L.umt_rows_fork(good, n, 8, None, P, 1, P, None, P, big, None) == 1 and L.umt_rows_fork(good, n, 8, P, P, 1, None, None, P, big, None) == 1
     assert L.umt_rows_fork(good, n, 8, P, P, 9, P, None, P, 4, None) == 5
     assert L.umt_rows_compact(good, n, 8, None, P, P, P, big, None) == 1 and L.umt_rows_compact(good, n, 8, P, P, P, P, 20, None) == 5

@@ -169,6 +169,27 @@ def stream_ptr(device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(device):
+    """torch.cuda.device(device), or nothing where it is the current device already (1.5 us of a small call)."""
+    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device) -> int:
+    """The current stream's handle, without the Stream object that `stream_ptr` goes through (2 us of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def dev_tensor(t, dtype, device) -> torch.Tensor:
     """Contiguous tensor of `dtype` on `device` (no copy when it already is)."""
     if not isinstance(t, torch.Tensor):

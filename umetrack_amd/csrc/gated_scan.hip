@@ -669,6 +669,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backwar
 
 // ---------------------------------------------------------------- one frame over a cache of rows
 constexpr int STEP_SEG = 256;              // features one wave advances
+constexpr int STEP_LOOK = 1024;            // samples among which a wave looks for its row's other names itself
 
 // owner[r] = highest sample that names row r, named[r] = how many do; only rows that are named are touched
 __global__ __launch_bounds__(GT) void step_clear_kernel(const int64_t* __restrict__ idx, int batch, int cache_rows,
@@ -695,51 +696,72 @@ struct StepArgs {
   const uint8_t *use, *valid;
   int batch, groups, share, cache_rows, segs;
   float* state;
-  const int32_t *owner, *named;
+  const int32_t *owner, *named;             // null: every wave looks through idx itself
   int32_t* status;
 };
 
+// STEP_SEG features of sample b, from f0 on; prev: the row's values.  -> the new state
 template <typename V>
-__device__ __forceinline__ float step_one(const StepArgs& A, const V* x, const V* gate, V* out, int b, int f, float prev, bool has_row) {
-  const int F = A.groups * A.share;
+__device__ __forceinline__ void step_values(const StepArgs& A, const V* __restrict__ x, const V* __restrict__ gate, V* out, int b, int f0,
+                                            bool has_row, const float (&prev)[STEP_SEG / 64], float (&h)[STEP_SEG / 64]) {
+  const int lane = threadIdx.x & 63, F = A.groups * A.share;
   const unsigned use = has_row && (!A.use || A.use[b]) ? ~0u : 0u, valid = !A.valid || A.valid[b] ? ~0u : 0u;
-  const float xv = masked_value(load_value(x + (int64_t)b * F + f), valid);
-  const float m = masked_step(gate_step(load_value(gate + (int64_t)b * A.groups + f / A.share)), use, valid);
-  const float hv = advance(masked_value(prev, use), xv, m);
-  store_value(out + (int64_t)b * F + f, hv);
-  return hv;
+  float xv[STEP_SEG / 64], gv[STEP_SEG / 64];
+#pragma unroll
+  for (int i = 0; i < STEP_SEG / 64; ++i) {
+    const int f = min(f0 + 64 * i + lane, F - 1);
+    xv[i] = load_value(x + (int64_t)b * F + f);
+    gv[i] = load_value(gate + (int64_t)b * A.groups + f / A.share);
+  }
+#pragma unroll
+  for (int i = 0; i < STEP_SEG / 64; ++i) {
+    h[i] = advance(masked_value(prev[i], use), masked_value(xv[i], valid), masked_step(gate_step(gv[i]), use, valid));
+    if (f0 + 64 * i + lane < F) store_value(out + (int64_t)b * F + f0 + 64 * i + lane, h[i]);
+  }
 }
 
 // One wave per (sample, segment of features).  A row that several samples name is advanced by the wave of the highest one:
-// it reads the row once, computes the other samples' outputs from that, and writes the row last.
+// it reads the row once, computes the other samples' outputs from that, and writes the row last.  Who that is a small batch
+// finds by looking through memory_idx (64 a load, from L2), a large one in the owner table of two launches before.
 template <typename V>
-__global__ __launch_bounds__(GT) void gated_step_kernel(StepArgs A, const V* __restrict__ x, const V* __restrict__ gate,
-                                                        V* __restrict__ out) {
+__global__ __launch_bounds__(GT) void gated_step_kernel(StepArgs A, const V* __restrict__ x, const V* __restrict__ gate, V* out) {
+  constexpr int K = STEP_SEG / 64;
   const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * (GT / 64) + (threadIdx.x >> 6);
+  const int64_t item = (int64_t)blockIdx.x * (GT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = (int)(item / A.segs), f0 = (int)(item - (int64_t)b * A.segs) * STEP_SEG;
   if (b >= A.batch) return;
-  const int F = A.groups * A.share, f1 = min(F, f0 + STEP_SEG);
+  const int F = A.groups * A.share;
   const int64_t r = A.idx ? A.idx[b] : b;
   const bool has_row = r >= 0 && r < A.cache_rows;
-  if (!has_row) {
-    if (A.status && f0 == 0 && lane == 0) atomicOr(A.status, (int)UMT_STATUS_BAD_MEMORY_IDX);
-    for (int f = f0 + lane; f < f1; f += 64) step_one(A, x, gate, out, b, f, 0.f, false);
-    return;
-  }
   bool shared = false;
-  if (A.idx) {
-    if (A.owner[r] != b) return;
-    shared = A.named[r] > 1;
+  if (A.idx && has_row) {
+    if (A.owner) {
+      if (A.owner[r] != b) return;
+      shared = A.named[r] > 1;
+    } else {
+      for (int o = 0; o < A.batch; o += 64) {
+        const uint64_t same = __ballot(o + lane < A.batch && A.idx[min(o + lane, A.batch - 1)] == r);
+        const int at = b - o;                                  // this sample's place among the 64
+        if (at < 0 ? same != 0 : at < 63 && same >> (at + 1) != 0) return;
+        if (same & (at >= 64 ? ~0ull : at <= 0 ? 0ull : (1ull << at) - 1)) shared = true;
+      }
+    }
   }
-  for (int f = f0 + lane; f < f1; f += 64) {
-    float* sp = A.state + r * F + f;
-    const float prev = *sp;
-    if (shared)
-      for (int o = 0; o < b; ++o)
-        if (A.idx[o] == r) step_one(A, x, gate, out, o, f, prev, true);
-    *sp = step_one(A, x, gate, out, b, f, prev, true);
+  if (!has_row && A.status && f0 == 0 && lane == 0) atomicOr(A.status, (int)UMT_STATUS_BAD_MEMORY_IDX);
+  float prev[K] = {}, h[K];
+  float* sp = A.state + (has_row ? r : 0) * F;
+  if (has_row && (shared || !A.use || A.use[b])) {             // a memory that is dropped is not read
+#pragma unroll
+    for (int i = 0; i < K; ++i) prev[i] = sp[min(f0 + 64 * i + lane, F - 1)];
   }
+  if (shared)
+    for (int o = 0; o < b; ++o)
+      if (A.idx[o] == r) step_values(A, x, gate, out, o, f0, true, prev, h);
+  step_values(A, x, gate, out, b, f0, has_row, prev, h);
+  if (!has_row) return;
+#pragma unroll
+  for (int i = 0; i < K; ++i)
+    if (f0 + 64 * i + lane < F) sp[f0 + 64 * i + lane] = h[i];
 }
 
 static int check_shape(const umt_gated_shape* S, bool backward) {
@@ -980,7 +1002,7 @@ extern "C" int umt_gated_scan_backward(const umt_gated_shape* shape, const void*
 }
 
 extern "C" int64_t umt_gated_step_workspace_bytes(int batch, int cache_rows) {
-  return batch > 0 && cache_rows > 0 ? 2 * (int64_t)cache_rows * (int64_t)sizeof(int32_t) : 0;
+  return batch > STEP_LOOK && cache_rows > 0 ? 2 * (int64_t)cache_rows * (int64_t)sizeof(int32_t) : 0;
 }
 
 extern "C" int umt_gated_step(int dtype, const void* x, const void* gate, const int64_t* memory_idx, const uint8_t* use_memory,
@@ -998,8 +1020,8 @@ extern "C" int umt_gated_step(int dtype, const void* x, const void* gate, const 
   const int F = groups * share, segs = (F + STEP_SEG - 1) / STEP_SEG;
   UMT_REQUIRE((int64_t)batch * segs <= (1LL << 32), UMT_ERR_INVALID, "gated step: %d samples of %d features", batch, F);
   hipStream_t s = (hipStream_t)stream;
-  int32_t *owner = (int32_t*)workspace, *named = owner + cache_rows;
-  if (memory_idx && cache_rows > 0) {
+  int32_t *owner = need ? (int32_t*)workspace : nullptr, *named = need ? owner + cache_rows : nullptr;
+  if (need) {
     const dim3 grid((batch + GT - 1) / GT);
     hipLaunchKernelGGL(step_clear_kernel, grid, dim3(GT), 0, s, memory_idx, batch, cache_rows, owner, named);
     hipLaunchKernelGGL(step_claim_kernel, grid, dim3(GT), 0, s, memory_idx, batch, cache_rows, owner, named);

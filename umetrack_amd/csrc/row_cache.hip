@@ -3,100 +3,109 @@
 //
 // The index work (who writes a row last, which rows are free, where a row goes) is integer arithmetic on a few bytes a
 // row; the moves are bound by HBM: 2 x row bytes for every row that changes place, and rows that stay are not touched.
-// A move is cut into pieces of MOVE_BYTES over all buffers, one wave each, so that a few long rows fill the GPU as well as
-// many short ones.
+// A wave moves up to MOVE_BYTES of one buffer's row, all of its loads in flight before its first store, so that a few long
+// rows fill the GPU as well as many short ones; buffers of a few words a row ride along with a row's first piece.
+// Ranks come from per-block counts that every block adds up for itself, in one workgroup where the cache is small.
 #include "umt_internal.h"
 
 namespace umt {
 
 constexpr int RT = 256;
 constexpr int64_t MOVE_BYTES = 4096;       // 64 lanes x 16 bytes x 4 loads in flight
+constexpr int ONE = 1024;                  // threads of a workgroup that ranks rows
+constexpr int BLOCK = 4 * ONE;             // rows it takes at once
+constexpr int SMALL_BYTES = 64 * 1024;     // moves that one workgroup makes itself rather than wait for another launch
 
 struct RowBuffers {
   char* data[UMT_ROW_BUFFERS_MAX];
   int64_t bytes[UMT_ROW_BUFFERS_MAX];      // a row's
   int64_t staged[UMT_ROW_BUFFERS_MAX];     // offset in a staged row
   int unit[UMT_ROW_BUFFERS_MAX];           // 16, 4 or 1: what data and row_bytes are multiples of
-  int piece0[UMT_ROW_BUFFERS_MAX + 1];     // first piece of the buffer in a row
-  int n;
+  int piece0[UMT_ROW_BUFFERS_MAX + 1];     // first piece of long buffer k in a row; [n_long] = pieces of a row
+  int n, n_long;                           // long buffers first; the others have at most one unit a lane
   int64_t staged_bytes;
 };
 
 template <typename U>
-__device__ __forceinline__ void move_units(char* __restrict__ to, const char* __restrict__ from, int n, int lane) {
-  U* t = reinterpret_cast<U*>(to);
+__device__ __forceinline__ void load_units(const char* from, int n, int lane, U (&r)[4]) {
   const U* f = reinterpret_cast<const U*>(from);
-  int i = lane;
-  for (; i + 192 < n; i += 256) {
-    const U a = f[i], b = f[i + 64], c = f[i + 128], d = f[i + 192];
-    t[i] = a;
-    t[i + 64] = b;
-    t[i + 128] = c;
-    t[i + 192] = d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 64 * i < n) r[i] = f[lane + 64 * i];
+}
+template <typename U>
+__device__ __forceinline__ void store_units(char* to, int n, int lane, const U (&r)[4]) {
+  U* t = reinterpret_cast<U*>(to);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 64 * i < n) t[lane + 64 * i] = r[i];
+}
+template <typename U>
+__device__ __forceinline__ void move_units(char* to, const char* from, int n, int lane) {
+  for (int i = 0; i < n; i += 256) {
+    U r[4];
+    load_units<U>(from + (int64_t)i * sizeof(U), n - i, lane, r);
+    store_units<U>(to + (int64_t)i * sizeof(U), n - i, lane, r);
   }
-  for (; i < n; i += 64) t[i] = f[i];
 }
 
-// piece p of a row; `to` / `from` null: the caches' row, else a staged row (16-byte aligned)
-__device__ __forceinline__ void move_piece(const RowBuffers& B, int p, int64_t dst, char* to, int64_t src, const char* from, int lane) {
-  int k = 0;
-  while (k + 1 < B.n && p >= B.piece0[k + 1]) ++k;
-  const int64_t at = (int64_t)(p - B.piece0[k]) * MOVE_BYTES, left = B.bytes[k] - at;
-  const int n = (int)(left < MOVE_BYTES ? left : MOVE_BYTES);
-  char* t = to ? to + B.staged[k] + at : B.data[k] + dst * B.bytes[k] + at;
-  const char* f = from ? from + B.staged[k] + at : B.data[k] + src * B.bytes[k] + at;
-  if (B.unit[k] == 16)
-    move_units<uint4>(t, f, n / 16, lane);
-  else if (B.unit[k] == 4)
-    move_units<uint32_t>(t, f, n / 4, lane);
-  else
-    move_units<uint8_t>(t, f, n, lane);
+// A row's place in buffer k: in the cache, or (staged != null) in a staged row, which is 16-byte aligned
+__device__ __forceinline__ char* place_of(const RowBuffers& B, int k, int64_t row, char* staged) {
+  return staged ? staged + B.staged[k] : B.data[k] + row * B.bytes[k];
+}
+
+// Piece p of a row, by one wave.  Source and target are different rows, and no other wave writes the one or reads the other.
+__device__ __forceinline__ void move_piece(const RowBuffers& B, int p, int64_t dst, char* to, int64_t src, char* from, int lane) {
+  uint32_t word[UMT_ROW_BUFFERS_MAX];
+  uint4 quad[UMT_ROW_BUFFERS_MAX];
+  const bool tiny = p == 0;
+  if (tiny) {
+#pragma unroll
+    for (int k = 0; k < UMT_ROW_BUFFERS_MAX; ++k) {
+      if (k < B.n_long || k >= B.n) continue;
+      const char* f = place_of(B, k, src, from);
+      if (lane * B.unit[k] < B.bytes[k]) {
+        if (B.unit[k] == 16)
+          quad[k] = reinterpret_cast<const uint4*>(f)[lane];
+        else
+          word[k] = B.unit[k] == 4 ? reinterpret_cast<const uint32_t*>(f)[lane] : (uint32_t)reinterpret_cast<const uint8_t*>(f)[lane];
+      }
+    }
+  }
+  if (B.n_long) {
+    int k = 0;
+    while (k + 1 < B.n_long && p >= B.piece0[k + 1]) ++k;
+    const int64_t at = (int64_t)(p - B.piece0[k]) * MOVE_BYTES, left = B.bytes[k] - at;
+    const int n = (int)(left < MOVE_BYTES ? left : MOVE_BYTES);
+    char* t = place_of(B, k, dst, to) + at;
+    const char* f = place_of(B, k, src, from) + at;
+    if (B.unit[k] == 16)
+      move_units<uint4>(t, f, n / 16, lane);
+    else if (B.unit[k] == 4)
+      move_units<uint32_t>(t, f, n / 4, lane);
+    else
+      move_units<uint8_t>(t, f, n, lane);
+  }
+  if (tiny) {
+#pragma unroll
+    for (int k = 0; k < UMT_ROW_BUFFERS_MAX; ++k) {
+      if (k < B.n_long || k >= B.n) continue;
+      char* t = place_of(B, k, dst, to);
+      if (lane * B.unit[k] < B.bytes[k]) {
+        if (B.unit[k] == 16)
+          reinterpret_cast<uint4*>(t)[lane] = quad[k];
+        else if (B.unit[k] == 4)
+          reinterpret_cast<uint32_t*>(t)[lane] = word[k];
+        else
+          reinterpret_cast<uint8_t*>(t)[lane] = (uint8_t)word[k];
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ bool in_cache(int64_t r, int rows) { return r >= 0 && r < rows; }
 
-// ---------------------------------------------------------------- copy
-// last[r] = highest i that writes row r, -1 where none does; only rows that the call names are touched
-__global__ __launch_bounds__(RT) void copy_clear_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
-                                                        int rows, int32_t* __restrict__ last, int32_t* __restrict__ status) {
-  const int i = blockIdx.x * RT + threadIdx.x;
-  if (i >= n) return;
-  if (!in_cache(src[i], rows) || !in_cache(dst[i], rows)) {
-    if (status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
-    return;
-  }
-  last[src[i]] = -1;
-  last[dst[i]] = -1;
-}
-__global__ __launch_bounds__(RT) void copy_claim_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
-                                                        int rows, int32_t* __restrict__ last) {
-  const int i = blockIdx.x * RT + threadIdx.x;
-  if (i < n && in_cache(src[i], rows) && in_cache(dst[i], rows)) atomicMax(last + dst[i], i);
-}
-// phase 0: rows that are read and overwritten by this call go to their staging place; phase 1: every copy, from there
-template <int PHASE>
-__global__ __launch_bounds__(RT) void copy_move_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst,
-                                                       int n, int rows, const int32_t* __restrict__ last, char* __restrict__ stage) {
-  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n];
-  const int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6);
-  const int64_t i = item / pieces;
-  if (i >= n) return;
-  const int p = (int)(item - i * pieces);
-  const int64_t s = src[i], d = dst[i];
-  if (!in_cache(s, rows) || !in_cache(d, rows) || s == d || last[d] != i) return;
-  const bool overwritten = last[s] >= 0;
-  char* place = stage + i * B.staged_bytes;
-  if (PHASE == 0) {
-    if (overwritten) move_piece(B, p, 0, place, s, nullptr, lane);
-  } else {
-    move_piece(B, p, d, nullptr, s, overwritten ? place : nullptr, lane);
-  }
-}
-
-// ---------------------------------------------------------------- fork
-constexpr int ONE = 1024;                  // threads of the single workgroup that ranks rows
-
-// exclusive rank of `flag` among the workgroup's threads, and the count of all
+// exclusive rank of v among the workgroup's ONE threads, in thread order, and the sum of all
 __device__ __forceinline__ int rank_in_group(int v, int* total, int* lds) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   int incl = v;
@@ -116,46 +125,201 @@ __device__ __forceinline__ int rank_in_group(int v, int* total, int* lds) {
   return before + incl - v;
 }
 
-// order[k] = the k-th source that is a live row; the k-th free row becomes its copy
-__global__ __launch_bounds__(ONE) void fork_rows_kernel(uint8_t* __restrict__ live, int rows, const int64_t* __restrict__ src, int n,
-                                                        int64_t* __restrict__ ids, int32_t* __restrict__ order, int32_t* __restrict__ status) {
+// bit i: live[r + i] is set, i < 4; rows at or past `end` are not
+__device__ __forceinline__ int live4(const uint8_t* live, int64_t r, int64_t end) {
+  int b = 0;
+  if (((uint64_t)live & 3) == 0 && r + 4 <= end && (r & 3) == 0) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(live + r);
+    for (int i = 0; i < 4; ++i) b |= (v >> (8 * i) & 0xff ? 1 : 0) << i;
+  } else {
+    for (int i = 0; i < 4; ++i)
+      if (r + i < end) b |= (live[r + i] ? 1 : 0) << i;
+  }
+  return b;
+}
+
+// counts[block] = live rows of the block
+__global__ __launch_bounds__(ONE) void count_rows_kernel(const uint8_t* __restrict__ live, int rows, int32_t* __restrict__ counts) {
   __shared__ int lds[ONE / 64];
-  const int tid = threadIdx.x;
-  int wanted = 0;
-  bool bad = false;
-  for (int i0 = 0; i0 < n; i0 += ONE) {
-    const int i = i0 + tid;
-    bool ok = false;
-    if (i < n) {
-      ok = in_cache(src[i], rows) && live[src[i]] != 0;
-      bad |= !ok;
-      ids[i] = -1;
-    }
-    int all;
-    const int k = rank_in_group(ok, &all, lds);
-    if (ok) order[wanted + k] = i;
-    wanted += all;
+  int all;
+  rank_in_group(__popc(live4(live, (int64_t)blockIdx.x * BLOCK + threadIdx.x * 4, rows)), &all, lds);
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+// sum of counts[0 .. upto) by the whole workgroup, in any order: they are integers
+__device__ __forceinline__ int sum_counts(const int32_t* counts, int upto, int* lds) {
+  int mine = 0, all;
+  for (int i = threadIdx.x; i < upto; i += ONE) mine += counts[i];
+  rank_in_group(mine, &all, lds);
+  return all;
+}
+
+// ---------------------------------------------------------------- copy
+// A few rows: one workgroup holds them all in LDS between reading and writing.
+constexpr int FEW = 256;
+__global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                       int rows, int32_t* __restrict__ status) {
+  extern __shared__ uint4 stage[];
+  __shared__ int64_t to[FEW];
+  __shared__ int64_t from[FEW];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, pieces = B.piece0[B.n_long];
+  for (int i = tid; i < n; i += ONE) {
+    const bool ok = in_cache(src[i], rows) && in_cache(dst[i], rows);
+    if (!ok && status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
+    to[i] = ok ? dst[i] : -1;
+    from[i] = ok ? src[i] : -1;
   }
+  __syncthreads();
+  for (int it = wv; it < n * pieces; it += ONE / 64) {
+    const int i = it / pieces;
+    if (to[i] >= 0) move_piece(B, it - i * pieces, 0, (char*)stage + i * B.staged_bytes, from[i], nullptr, lane);
+  }
+  __syncthreads();
+  for (int it = wv; it < n * pieces; it += ONE / 64) {
+    const int i = it / pieces;
+    if (to[i] < 0) continue;
+    bool last = true;                       // of several writes to one row the highest i counts
+    for (int o = i + 1 + lane; o < n; o += 64) last &= to[o] != to[i];
+    if (__all(last)) move_piece(B, it - i * pieces, to[i], nullptr, 0, (char*)stage + i * B.staged_bytes, lane);
+  }
+}
+
+// last[r] = highest i that writes row r, -1 where none does; only rows that the call names are touched
+__global__ __launch_bounds__(RT) void copy_clear_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                        int rows, int32_t* __restrict__ last, int32_t* __restrict__ todo,
+                                                        int32_t* __restrict__ status) {
+  const int i = blockIdx.x * RT + threadIdx.x;
+  if (i == 0) todo[0] = 0;
+  if (i >= n) return;
+  if (!in_cache(src[i], rows) || !in_cache(dst[i], rows)) {
+    if (status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
+    return;
+  }
+  last[src[i]] = -1;
+  last[dst[i]] = -1;
+}
+__global__ __launch_bounds__(RT) void copy_claim_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                        int rows, int32_t* __restrict__ last) {
+  const int i = blockIdx.x * RT + threadIdx.x;
+  if (i < n && in_cache(src[i], rows) && in_cache(dst[i], rows)) atomicMax(last + dst[i], i);
+}
+__device__ __forceinline__ bool copies(const int32_t* last, int64_t s, int64_t d, int i, int rows) {
+  return in_cache(s, rows) && in_cache(d, rows) && s != d && last[d] == i;
+}
+// todo: [0] how many, then the copies whose source is overwritten by the call (in any order: each has its staging place)
+__global__ __launch_bounds__(RT) void copy_list_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n, int rows,
+                                                       const int32_t* __restrict__ last, int32_t* __restrict__ todo) {
+  const int i = blockIdx.x * RT + threadIdx.x;
+  if (i < n && copies(last, src[i], dst[i], i, rows) && last[src[i]] >= 0) todo[4 + atomicAdd(todo, 1)] = i;
+}
+__global__ __launch_bounds__(RT) void copy_stage_kernel(RowBuffers B, const int64_t* __restrict__ src, const int32_t* __restrict__ todo,
+                                                        char* __restrict__ stage) {
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
+  const int64_t n = (int64_t)todo[0] * pieces, stride = (int64_t)gridDim.x * (RT / 64);
+  for (int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6); item < n; item += stride) {
+    const int64_t k = item / pieces;
+    const int i = todo[4 + k];
+    move_piece(B, (int)(item - k * pieces), 0, stage + i * B.staged_bytes, src[i], nullptr, lane);
+  }
+}
+__global__ __launch_bounds__(RT) void copy_move_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                       int rows, const int32_t* __restrict__ last, char* stage) {
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
+  const int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6);
+  const int64_t i = item / pieces;
+  if (i >= n) return;
+  const int64_t s = src[i], d = dst[i];
+  if (copies(last, s, d, (int)i, rows))
+    move_piece(B, (int)(item - i * pieces), d, nullptr, s, last[s] >= 0 ? stage + i * B.staged_bytes : nullptr, lane);
+}
+
+// ---------------------------------------------------------------- fork
+// order[k] = the k-th source that is a live row; the k-th free row becomes its copy.
+// sources of one block: appends to order from `wanted` on
+__device__ __forceinline__ int order_sources(const uint8_t* live, int rows, const int64_t* src, int n, int64_t i0, int wanted, int64_t* ids,
+                                             int32_t* order, int32_t* status, int* lds) {
+  int ok = 0;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t i = i0 + threadIdx.x * 4 + j;
+    if (i >= n) break;
+    const bool fine = in_cache(src[i], rows) && live[src[i]] != 0;
+    if (!fine && status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
+    ok |= fine << j;
+    ids[i] = -1;
+  }
+  int all, k = wanted + rank_in_group(__popc(ok), &all, lds);
+  for (int j = 0; j < 4; ++j)
+    if (ok >> j & 1) order[k++] = (int)(i0 + threadIdx.x * 4 + j);
+  return all;
+}
+// free rows of one block: hands them to the sources from `found` on
+__device__ __forceinline__ int hand_out_rows(uint8_t* live, int rows, int64_t r0, int found, int wanted, int64_t* ids, const int32_t* order,
+                                             int* lds) {
+  const int64_t r = r0 + threadIdx.x * 4;
+  const int there = (int)max((int64_t)0, min((int64_t)4, rows - r)), gone = ~live4(live, r, rows) & ((1 << there) - 1);
+  int all, k = found + rank_in_group(__popc(gone), &all, lds);
+  for (int j = 0; j < 4; ++j)
+    if (gone >> j & 1) {
+      if (k < wanted) {
+        ids[order[k]] = r + j;
+        live[r + j] = 1;
+      }
+      ++k;
+    }
+  return all;
+}
+
+// everything in one workgroup; `moves`: the copies too
+__global__ __launch_bounds__(ONE) void fork_one_kernel(RowBuffers B, uint8_t* live, int rows, const int64_t* __restrict__ src, int n,
+                                                       int64_t* ids, int32_t* order, int32_t* status, int moves) {
+  __shared__ int lds[ONE / 64];
+  int wanted = 0, found = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += BLOCK) wanted += order_sources(live, rows, src, n, i0, wanted, ids, order, status, lds);
   __syncthreads();                          // order and ids are complete, and no live flag has changed yet
-  int found = 0;
-  for (int r0 = 0; r0 < rows && found < wanted; r0 += ONE) {
-    const int r = r0 + tid;
-    const bool is_free = r < rows && live[r] == 0;
-    int all;
-    const int k = found + rank_in_group(is_free, &all, lds);
-    if (is_free && k < wanted) {
-      ids[order[k]] = r;
-      live[r] = 1;
-    }
-    found += all;
+  for (int64_t r0 = 0; r0 < rows && found < wanted; r0 += BLOCK) found += hand_out_rows(live, rows, r0, found, wanted, ids, order, lds);
+  if (status && threadIdx.x == 0 && found < wanted) atomicOr(status, (int)UMT_STATUS_NO_FREE_ROW);
+  if (!moves) return;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
+  for (int it = threadIdx.x >> 6; it < n * pieces; it += ONE / 64) {
+    const int i = it / pieces;
+    if (ids[i] >= 0) move_piece(B, it - i * pieces, ids[i], nullptr, src[i], nullptr, lane);
   }
-  if (status && bad) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
-  if (status && tid == 0 && found < wanted) atomicOr(status, (int)UMT_STATUS_NO_FREE_ROW);
+}
+// the same in four launches: counts (live rows a block; good sources a block behind them), order, hand out, move
+__global__ __launch_bounds__(ONE) void fork_count_kernel(const uint8_t* __restrict__ live, int rows, const int64_t* __restrict__ src, int n,
+                                                         int row_blocks, int32_t* __restrict__ counts) {
+  __shared__ int lds[ONE / 64];
+  int mine = 0, all;
+  if ((int)blockIdx.x < row_blocks) {
+    mine = __popc(live4(live, (int64_t)blockIdx.x * BLOCK + threadIdx.x * 4, rows));
+  } else {
+    const int64_t i0 = (int64_t)(blockIdx.x - row_blocks) * BLOCK + threadIdx.x * 4;
+    for (int j = 0; j < 4; ++j) mine += i0 + j < n && in_cache(src[i0 + j], rows) && live[src[i0 + j]] != 0;
+  }
+  rank_in_group(mine, &all, lds);
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+__global__ __launch_bounds__(ONE) void fork_order_kernel(const uint8_t* __restrict__ live, int rows, const int64_t* __restrict__ src, int n,
+                                                         const int32_t* __restrict__ counts, int row_blocks, int64_t* __restrict__ ids,
+                                                         int32_t* __restrict__ order, int32_t* __restrict__ status) {
+  __shared__ int lds[ONE / 64];
+  const int before = sum_counts(counts + row_blocks, blockIdx.x, lds);
+  order_sources(live, rows, src, n, (int64_t)blockIdx.x * BLOCK, before, ids, order, status, lds);
+}
+__global__ __launch_bounds__(ONE) void fork_rows_kernel(uint8_t* live, int rows, const int32_t* __restrict__ counts, int row_blocks,
+                                                        int source_blocks, int64_t* ids, const int32_t* __restrict__ order,
+                                                        int32_t* __restrict__ status) {
+  __shared__ int lds[ONE / 64];
+  const int64_t r0 = (int64_t)blockIdx.x * BLOCK;
+  const int found = (int)(r0 - sum_counts(counts, blockIdx.x, lds));       // free rows before this block
+  const int wanted = sum_counts(counts + row_blocks, source_blocks, lds);
+  const int here = found < wanted ? hand_out_rows(live, rows, r0, found, wanted, ids, order, lds) : 0;
+  if (status && blockIdx.x + 1 == gridDim.x && threadIdx.x == 0 && found + here < wanted) atomicOr(status, (int)UMT_STATUS_NO_FREE_ROW);
 }
 
 // sources are live rows and targets were free ones, so no row is both
 __global__ __launch_bounds__(RT) void fork_move_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ ids, int n) {
-  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n];
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
   const int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6);
   const int64_t i = item / pieces;
   if (i >= n || ids[i] < 0) return;
@@ -175,82 +339,108 @@ __global__ __launch_bounds__(RT) void free_rows_kernel(uint8_t* __restrict__ liv
 }
 
 // ---------------------------------------------------------------- compact
-// moves: [0] = how many, then (hole, row) lists of rows entries each
-__global__ __launch_bounds__(ONE) void compact_rows_kernel(uint8_t* __restrict__ live, int rows, int64_t* __restrict__ now,
-                                                           int64_t* __restrict__ count, int32_t* __restrict__ moves) {
+// lists: [0] = live rows c, [1] = moves, from [4] on the holes below c and behind them the live rows from c on, in order.
+// counts may be null in a grid of one block.  live is read only: the launch that moves writes it.
+__global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __restrict__ live, int rows, const int32_t* __restrict__ counts,
+                                                           int64_t* __restrict__ now, int32_t* __restrict__ lists) {
   __shared__ int lds[ONE / 64];
-  const int tid = threadIdx.x;
-  int mine = 0, c;
-  for (int r = tid; r < rows; r += ONE) mine += live[r] != 0;
-  rank_in_group(mine, &c, lds);
-  int32_t *holes = moves + 4, *movers = holes + rows;
-  int n_holes = 0, n_movers = 0;
-  for (int r0 = 0; r0 < rows; r0 += ONE) {
-    const int r = r0 + tid;
-    const bool lv = r < rows && live[r] != 0;
-    const bool hole = r < c && !lv, mover = r >= c && lv;
-    int all;
-    const int k = rank_in_group(hole | (mover << 16), &all, lds);
-    if (hole) holes[n_holes + (k & 0xffff)] = r;
-    if (mover) movers[n_movers + (k >> 16)] = r;
-    n_holes += all & 0xffff;
-    n_movers += all >> 16;
-    if (r < rows) {
-      if (!mover) now[r] = lv ? r : -1;
-      live[r] = r < c;
-    }
+  const int64_t r = (int64_t)blockIdx.x * BLOCK + threadIdx.x * 4;
+  const int mine = live4(live, r, rows);
+  int here, k = rank_in_group(__popc(mine), &here, lds);
+  int c = here, below = 0;                  // live rows in all, before this block
+  if (counts) {
+    c = sum_counts(counts, gridDim.x, lds);
+    below = sum_counts(counts, blockIdx.x, lds);
   }
-  __syncthreads();                          // the lists are complete; n_holes == n_movers
-  for (int k = tid; k < n_movers; k += ONE) now[movers[k]] = holes[k];
-  if (tid == 0) {
-    moves[0] = n_movers;
-    *count = c;
+  // live rows below row c: whole blocks, and the part of the block that row c lies in
+  const int cut = counts ? c / BLOCK : 0;
+  int under;
+  rank_in_group(__popc(live4(live, (int64_t)cut * BLOCK + threadIdx.x * 4, c)), &under, lds);
+  if (counts) under += sum_counts(counts, cut, lds);
+  int32_t *holes = lists + 4, *movers = holes + rows;
+  k += below;                               // live rows before row r
+  for (int i = 0; i < 4; ++i) {
+    if (r + i >= rows) break;
+    const bool lv = mine >> i & 1;
+    if (r + i < c) {
+      if (!lv) holes[r + i - k] = (int32_t)(r + i);
+      now[r + i] = lv ? r + i : -1;
+    } else if (lv) {
+      movers[k - under] = (int32_t)(r + i);
+    } else {
+      now[r + i] = -1;
+    }
+    k += lv;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    lists[0] = c;
+    lists[1] = c - under;
   }
 }
 
 // rows at or above the live count move to free rows below it: no row is both
-__global__ __launch_bounds__(RT) void compact_move_kernel(RowBuffers B, const int32_t* __restrict__ moves, int rows) {
-  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n];
-  const int64_t n = (int64_t)moves[0] * pieces, stride = (int64_t)gridDim.x * (RT / 64);
-  const int32_t *holes = moves + 4, *movers = holes + rows;
+__global__ __launch_bounds__(RT) void compact_move_kernel(RowBuffers B, const int32_t* __restrict__ lists, int rows, uint8_t* __restrict__ live,
+                                                          int64_t* __restrict__ now, int64_t* __restrict__ count) {
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long], c = lists[0], moves = lists[1];
+  const int64_t n = (int64_t)moves * pieces, stride = (int64_t)gridDim.x * (RT / 64), all = (int64_t)gridDim.x * RT;
+  const int32_t *holes = lists + 4, *movers = holes + rows;
+  for (int64_t r = (int64_t)blockIdx.x * RT + threadIdx.x; r < rows; r += all) {
+    live[r] = r < c;
+    if (r < moves) now[movers[r]] = holes[r];
+    if (r == 0) *count = c;
+  }
   for (int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6); item < n; item += stride) {
     const int64_t k = item / pieces;
     move_piece(B, (int)(item - k * pieces), holes[k], nullptr, movers[k], nullptr, lane);
   }
 }
+__global__ void compact_nothing_kernel(int64_t* count) { *count = 0; }
 
 static int row_buffers(const char* what, const umt_row_buffer* buffers, int n, int rows, RowBuffers* B) {
   UMT_REQUIRE(n > 0 && n <= UMT_ROW_BUFFERS_MAX && buffers && rows >= 0, UMT_ERR_INVALID, "%s: %d buffers of %d rows", what, n, rows);
+  *B = RowBuffers{};
   B->n = n;
-  int64_t pieces = 0, off = 0;
   for (int k = 0; k < n; ++k) {
     const umt_row_buffer& b = buffers[k];
     UMT_REQUIRE((b.data || rows == 0) && b.row_bytes > 0 && b.row_bytes <= (1LL << 40), UMT_ERR_INVALID,
                 "%s: buffer %d is null or its rows have %lld bytes", what, k, (long long)b.row_bytes);
-    const uint64_t lo = (uint64_t)b.data, both = lo | (uint64_t)b.row_bytes;
+    const uint64_t lo = (uint64_t)b.data;
     for (int j = 0; j < k && rows > 0; ++j) {
       const uint64_t o = (uint64_t)buffers[j].data;
       UMT_REQUIRE(o + (uint64_t)buffers[j].row_bytes * rows <= lo || lo + (uint64_t)b.row_bytes * rows <= o, UMT_ERR_INVALID,
                   "%s: buffers %d and %d overlap", what, j, k);
     }
-    B->data[k] = (char*)b.data;
-    B->bytes[k] = b.row_bytes;
-    B->unit[k] = both % 16 == 0 ? 16 : both % 4 == 0 ? 4 : 1;
-    B->staged[k] = off;
-    off += round_up64(b.row_bytes, 16);
-    B->piece0[k] = (int)pieces;
-    pieces += (b.row_bytes + MOVE_BYTES - 1) / MOVE_BYTES;
-    UMT_REQUIRE(pieces < (1 << 30), UMT_ERR_INVALID, "%s: rows of %lld bytes", what, (long long)b.row_bytes);
   }
-  B->piece0[n] = (int)pieces;
+  int64_t pieces = 0, off = 0;
+  int at = 0;
+  for (int tiny = 0; tiny < 2; ++tiny)      // long buffers first
+    for (int k = 0; k < n; ++k) {
+      const umt_row_buffer& b = buffers[k];
+      const uint64_t both = (uint64_t)b.data | (uint64_t)b.row_bytes;
+      const int unit = both % 16 == 0 ? 16 : both % 4 == 0 ? 4 : 1;
+      if ((b.row_bytes <= 64 * unit) != (tiny == 1)) continue;
+      B->data[at] = (char*)b.data;
+      B->bytes[at] = b.row_bytes;
+      B->unit[at] = unit;
+      B->staged[at] = off;
+      off += round_up64(b.row_bytes, 16);
+      if (!tiny) {
+        B->piece0[at] = (int)pieces;
+        pieces += (b.row_bytes + MOVE_BYTES - 1) / MOVE_BYTES;
+        UMT_REQUIRE(pieces < (1 << 30), UMT_ERR_INVALID, "%s: rows of %lld bytes", what, (long long)b.row_bytes);
+        B->n_long = at + 1;
+      }
+      ++at;
+    }
+  B->piece0[B->n_long] = pieces > 0 ? (int)pieces : 1;
   B->staged_bytes = off;
   return 0;
 }
 
 // workgroups of a move of n rows, a wave per piece
 static int move_grid(const char* what, const RowBuffers& B, int64_t n, unsigned* grid) {
-  const int64_t wg = (n * B.piece0[B.n] + RT / 64 - 1) / (RT / 64);
-  UMT_REQUIRE(wg < (1LL << 31), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n, B.piece0[B.n]);
+  const int64_t wg = (n * B.piece0[B.n_long] + RT / 64 - 1) / (RT / 64);
+  UMT_REQUIRE(wg < (1LL << 31), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n, B.piece0[B.n_long]);
   *grid = (unsigned)wg;
   return 0;
 }
@@ -264,10 +454,13 @@ static int need_workspace(const char* what, const void* ws, int64_t have, int64_
 
 using namespace umt;
 
+static bool few_rows(const RowBuffers& B, int n) { return n <= FEW && n * B.staged_bytes <= SMALL_BYTES - 16 * FEW; }
+static int blocks_of(int64_t n) { return (int)((n + BLOCK - 1) / BLOCK); }
+
 extern "C" int64_t umt_rows_copy_workspace_bytes(const umt_row_buffer* buffers, int n_buffers, int rows, int n) {
   RowBuffers B;
   if (n < 0 || row_buffers("rows copy", buffers, n_buffers, rows, &B) != 0) return -1;
-  return n == 0 || rows == 0 ? 0 : round_up64((int64_t)rows * 4, 16) + n * B.staged_bytes;
+  return n == 0 || rows == 0 || few_rows(B, n) ? 0 : round_up64((int64_t)rows * 4, 16) + round_up64(16 + (int64_t)n * 4, 16) + n * B.staged_bytes;
 }
 
 extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int rows, const int64_t* src, const int64_t* dst, int n,
@@ -276,22 +469,34 @@ extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int r
   UMT_TRY(row_buffers("rows copy", buffers, n_buffers, rows, &B));
   UMT_REQUIRE(n >= 0 && (n == 0 || (src && dst)), UMT_ERR_INVALID, "rows copy: n=%d or null pointer", n);
   if (n == 0) return 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (few_rows(B, n)) {
+    hipLaunchKernelGGL(copy_few_kernel, dim3(1), dim3(ONE), (size_t)(n * B.staged_bytes), s, B, src, dst, n, rows, status);
+    UMT_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
   UMT_TRY(need_workspace("rows copy", workspace, workspace_bytes, umt_rows_copy_workspace_bytes(buffers, n_buffers, rows, n)));
   unsigned grid = 0;
   UMT_TRY(move_grid("rows copy", B, n, &grid));
-  hipStream_t s = (hipStream_t)stream;
   int32_t* last = (int32_t*)workspace;
-  char* stage = (char*)workspace + round_up64((int64_t)rows * 4, 16);
+  int32_t* todo = (int32_t*)((char*)workspace + round_up64((int64_t)rows * 4, 16));
+  char* stage = (char*)todo + round_up64(16 + (int64_t)n * 4, 16);
   const dim3 per_pair((n + RT - 1) / RT);
-  hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, status);
+  hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo, status);
   hipLaunchKernelGGL(copy_claim_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last);
-  hipLaunchKernelGGL(copy_move_kernel<0>, dim3(grid), dim3(RT), 0, s, B, src, dst, n, rows, last, stage);
-  hipLaunchKernelGGL(copy_move_kernel<1>, dim3(grid), dim3(RT), 0, s, B, src, dst, n, rows, last, stage);
+  hipLaunchKernelGGL(copy_list_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo);
+  hipLaunchKernelGGL(copy_stage_kernel, dim3(grid < 2048 ? grid : 2048), dim3(RT), 0, s, B, src, todo, stage);
+  hipLaunchKernelGGL(copy_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, dst, n, rows, last, stage);
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }
 
-extern "C" int64_t umt_rows_fork_workspace_bytes(int rows, int n) { return rows < 0 || n < 0 ? -1 : (int64_t)n * 4; }
+// one workgroup ranks this many rows or sources in the time of the other launches' start
+static bool one_group(int rows, int n) { return rows <= 4 * BLOCK && n <= BLOCK; }
+
+extern "C" int64_t umt_rows_fork_workspace_bytes(int rows, int n) {
+  return rows < 0 || n < 0 ? -1 : n == 0 ? 0 : (int64_t)n * 4 + (one_group(rows, n) ? 0 : (blocks_of(rows) + blocks_of(n)) * 4);
+}
 
 extern "C" int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int rows, uint8_t* live, const int64_t* src, int n,
                              int64_t* ids, int32_t* status, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -303,8 +508,18 @@ extern "C" int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int r
   unsigned grid = 0;
   UMT_TRY(move_grid("rows fork", B, n, &grid));
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(fork_rows_kernel, dim3(1), dim3(ONE), 0, s, live, rows, src, n, ids, (int32_t*)workspace, status);
-  hipLaunchKernelGGL(fork_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, ids, n);
+  int32_t *order = (int32_t*)workspace, *counts = order + n;
+  if (one_group(rows, n)) {
+    const int moves = n <= FEW && n * B.staged_bytes <= SMALL_BYTES;
+    hipLaunchKernelGGL(fork_one_kernel, dim3(1), dim3(ONE), 0, s, B, live, rows, src, n, ids, order, status, moves);
+    if (!moves) hipLaunchKernelGGL(fork_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, ids, n);
+  } else {
+    const int rb = blocks_of(rows), sb = blocks_of(n);
+    hipLaunchKernelGGL(fork_count_kernel, dim3(rb + sb), dim3(ONE), 0, s, live, rows, src, n, rb, counts);
+    hipLaunchKernelGGL(fork_order_kernel, dim3(sb), dim3(ONE), 0, s, live, rows, src, n, counts, rb, ids, order, status);
+    if (rb) hipLaunchKernelGGL(fork_rows_kernel, dim3(rb), dim3(ONE), 0, s, live, rows, counts, rb, sb, ids, order, status);
+    hipLaunchKernelGGL(fork_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, ids, n);
+  }
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -317,22 +532,27 @@ extern "C" int umt_rows_free(uint8_t* live, int rows, const int64_t* row_ids, in
   return 0;
 }
 
-extern "C" int64_t umt_rows_compact_workspace_bytes(int rows) { return rows < 0 ? -1 : 16 + 8 * (int64_t)rows; }
+extern "C" int64_t umt_rows_compact_workspace_bytes(int rows) { return rows < 0 ? -1 : 16 + 8 * (int64_t)rows + 4 * (int64_t)blocks_of(rows); }
 
 extern "C" int umt_rows_compact(const umt_row_buffer* buffers, int n_buffers, int rows, uint8_t* live, int64_t* now, int64_t* count,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
   RowBuffers B;
   UMT_TRY(row_buffers("rows compact", buffers, n_buffers, rows, &B));
   UMT_REQUIRE((live && now && count) || (rows == 0 && count), UMT_ERR_INVALID, "rows compact: null pointer");
-  UMT_TRY(need_workspace("rows compact", workspace, workspace_bytes, umt_rows_compact_workspace_bytes(rows)));
   hipStream_t s = (hipStream_t)stream;
-  int32_t* moves = (int32_t*)workspace;
-  hipLaunchKernelGGL(compact_rows_kernel, dim3(1), dim3(ONE), 0, s, live, rows, now, count, moves);
-  if (rows > 1) {                           // at most half of the rows move
-    unsigned grid = 0;
-    UMT_TRY(move_grid("rows compact", B, rows / 2, &grid));
-    hipLaunchKernelGGL(compact_move_kernel, dim3(grid < 4096 ? grid : 4096), dim3(RT), 0, s, B, moves, rows);
+  if (rows == 0) {
+    hipLaunchKernelGGL(compact_nothing_kernel, dim3(1), dim3(1), 0, s, count);
+    UMT_CHECK_HIP(hipGetLastError());
+    return 0;
   }
+  UMT_TRY(need_workspace("rows compact", workspace, workspace_bytes, umt_rows_compact_workspace_bytes(rows)));
+  unsigned grid = 0;
+  UMT_TRY(move_grid("rows compact", B, rows / 2 + 1, &grid));              // at most half of the rows move
+  int32_t *lists = (int32_t*)workspace, *counts = lists + 4 + 2 * (int64_t)rows;
+  const int blocks = blocks_of(rows);
+  if (blocks > 1) hipLaunchKernelGGL(count_rows_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counts);
+  hipLaunchKernelGGL(compact_list_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, blocks > 1 ? counts : (int32_t*)nullptr, now, lists);
+  hipLaunchKernelGGL(compact_move_kernel, dim3(grid < 4096 ? grid : 4096), dim3(RT), 0, s, B, lists, rows, live, now, count);
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }

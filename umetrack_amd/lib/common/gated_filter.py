@@ -20,8 +20,9 @@ _DTYPES = {torch.float32: nat.VALUES_F32, torch.bfloat16: nat.VALUES_BF16}
 def _split(name: str, x: torch.Tensor, gate: torch.Tensor, lead: int) -> Tuple[int, int]:
     """(groups, share) of features x.shape[lead:] under gates gate.shape[lead:]: the gate's dimensions are the first of the
     feature's, up to dimensions of size 1 behind them; the features behind share a gate."""
-    feat, g = tuple(x.shape[lead:]), tuple(gate.shape[lead:])
-    if tuple(x.shape[:lead]) != tuple(gate.shape[:lead]):
+    xs, gs = tuple(x.shape), tuple(gate.shape)
+    feat, g = xs[lead:], gs[lead:]
+    if xs[:lead] != gs[:lead]:
         raise ValueError(f"{name}: x is {tuple(x.shape)} and gate {tuple(gate.shape)}: the first {lead} dimensions differ")
     while g and (len(g) > len(feat) or g[-1] == 1 != feat[len(g) - 1]):
         if g[-1] != 1:
@@ -37,33 +38,32 @@ def _check_values(name: str, x, gate) -> torch.device:
         raise TypeError(f"{name}: x and gate are tensors")
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         raise TypeError(f"{name}: x and gate are both float32 or both bfloat16, got {x.dtype} and {gate.dtype}")
-    dev = nat.require_gpu(x.device if x.is_cuda else None)
-    if x.device != dev or gate.device != dev:
+    dev = x.device
+    if dev.type != "cuda":
+        nat.require_gpu()
+    if dev.type != "cuda" or gate.device != dev:
         raise ValueError(f"{name}: x is on {x.device} and gate on {gate.device}: both have to be on one GPU")
     return dev
 
 
 def _rows_of(t: torch.Tensor, n: int) -> torch.Tensor:
     """[T, R, ...] as [T, R, n] whose last axis is contiguous; the first two keep their strides (0 included) where they can."""
-    v = t
+    if t.is_contiguous():
+        return t                                           # only the address and the first two strides are read
     if n == 1:
-        v = t.reshape(t.shape[0], t.shape[1], 1)
-    elif t.dim() != 3 or t.stride(2) != 1:
-        inner, want = t.shape[2:], 1
-        dense = True
-        for size, stride in zip(reversed(inner), reversed(t.stride()[2:])):
-            if size != 1 and stride != want:
-                dense = False
-            want *= size
-        v = t.as_strided((t.shape[0], t.shape[1], n), (t.stride(0), t.stride(1), 1)) if dense \
-            else t.contiguous().view(t.shape[0], t.shape[1], n)
-    return v
+        return t.reshape(t.shape[0], t.shape[1], 1)
+    want = 1
+    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+        if size != 1 and stride != want:
+            return t.contiguous()
+        want *= size
+    return t
 
 
 def _mask(name: str, m, shape, dev) -> Optional[torch.Tensor]:
     if m is None:
         return None
-    if not isinstance(m, torch.Tensor) or m.dtype not in (torch.bool, torch.uint8) or tuple(m.shape) != tuple(shape) or m.device != dev:
+    if not isinstance(m, torch.Tensor) or m.dtype not in (torch.bool, torch.uint8) or m.shape != shape or m.device != dev:
         raise ValueError(f"{name}: expected a bool tensor {tuple(shape)} on {dev}")
     return m
 
@@ -71,7 +71,7 @@ def _mask(name: str, m, shape, dev) -> Optional[torch.Tensor]:
 def _state(name: str, s, shape, dev) -> Optional[torch.Tensor]:
     if s is None:
         return None
-    if not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or tuple(s.shape) != tuple(shape) or s.device != dev:
+    if not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or s.shape != shape or s.device != dev:
         raise ValueError(f"{name}: expected a float32 tensor {tuple(shape)} on {dev}")
     return s.contiguous()
 
@@ -89,13 +89,10 @@ def _raw(t: Optional[torch.Tensor]):
 
 
 def _shape(x, gate, use, valid, groups, share, out) -> nat.GatedShape:
-    s = nat.GatedShape(_DTYPES[x.dtype], x.shape[0], x.shape[1], groups, share, x.stride(0), x.stride(1), gate.stride(0),
-                       gate.stride(1), out.stride(0), out.stride(1))
-    if use is not None:
-        s.use_t, s.use_row = use.stride()
-    if valid is not None:
-        s.valid_t, s.valid_row = valid.stride()
-    return s
+    T, R = x.shape[:2]
+    xs, gs, os = x.stride(), gate.stride(), out.stride()
+    us, vs = (0, 0) if use is None else use.stride(), (0, 0) if valid is None else valid.stride()
+    return nat.GatedShape(_DTYPES[x.dtype], T, R, groups, share, xs[0], xs[1], gs[0], gs[1], os[0], os[1], us[0], us[1], vs[0], vs[1])
 
 
 def _workspace(nbytes: int, dev):
@@ -104,24 +101,46 @@ def _workspace(nbytes: int, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _scan(x, gate, h0, use, valid, keep: bool):
-    """-> (h, h_last, kept).  Shapes are checked by the callers."""
+def _scan(x, gate, h0, use, valid, groups: int, share: int, keep: bool):
+    """-> (h, h_last, kept).  Arguments are checked by the caller."""
     dev = x.device
-    groups, share = _split("gated_scan", x, gate, 2)
-    feat = tuple(x.shape[2:])
-    xs, gs = _rows_of(x, groups * share), _rows_of(gate, groups)
-    h = _like(x, feat)
-    last = torch.empty((x.shape[1],) + feat, dtype=torch.float32, device=dev)
+    feat = x.shape[2:]
     T, R = x.shape[:2]
-    kept = torch.empty((-(-T // nat.GATED_KEEP), R * groups * share), dtype=torch.float32, device=dev) if keep else None
-    if h.numel() or last.numel():
+    n = groups * share
+    xs, gs = _rows_of(x, n), _rows_of(gate, groups)
+    h = _like(x, feat)
+    last = torch.empty(x.shape[1:], dtype=torch.float32, device=dev)
+    kept = torch.empty((-(-T // nat.GATED_KEEP), R * n), dtype=torch.float32, device=dev) if keep else None
+    if R * n:
         shape = _shape(xs, gs, use, valid, groups, share, h)
         L = nat.lib()
-        with torch.cuda.device(dev):
+        with nat.on_device(dev):
             ws = _workspace(L.umt_gated_scan_workspace_bytes(shape), dev)
-            nat.check(L.umt_gated_scan(shape, _raw(xs), _raw(gs), _raw(use), _raw(valid), _raw(h0), _raw(h), _raw(last), _raw(kept),
-                                       _raw(ws), 0 if ws is None else ws.numel(), nat.stream_ptr(dev)), "umt_gated_scan")
+            nat.check(L.umt_gated_scan(shape, xs.data_ptr(), gs.data_ptr(), _raw(use), _raw(valid), _raw(h0), h.data_ptr(), last.data_ptr(),
+                                       _raw(kept), _raw(ws), 0 if ws is None else ws.numel(), nat.raw_stream(dev)), "umt_gated_scan")
     return h, last, kept
+
+
+def _backward(x, gate, kept, dh, dh_last, use, valid, groups: int, share: int, need):
+    """-> (dx, dgate, dh0), None where not needed.  Arguments are checked by the caller."""
+    dev = x.device
+    R, n = x.shape[1], groups * share
+    xs, gs, ds = _rows_of(x, n), _rows_of(gate, groups), _rows_of(dh, n)
+    dx = _like(x, x.shape[2:]) if need[0] else None
+    dgate = _like(x, gate.shape[2:]) if need[1] else None
+    dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=dev) if need[2] else None
+    if R * n and any(need):
+        shape = _shape(xs, gs, use, valid, groups, share, xs if dx is None else dx)
+        shape.dh_t, shape.dh_row = ds.stride()[:2]
+        if dgate is not None:
+            shape.dgate_t, shape.dgate_row = dgate.stride()[:2]
+        L = nat.lib()
+        with nat.on_device(dev):
+            ws = _workspace(L.umt_gated_scan_backward_workspace_bytes(shape), dev)
+            nat.check(L.umt_gated_scan_backward(shape, xs.data_ptr(), gs.data_ptr(), _raw(use), _raw(valid), kept.data_ptr(), ds.data_ptr(),
+                                                _raw(dh_last), _raw(dx), _raw(dgate), _raw(dh0), _raw(ws), 0 if ws is None else ws.numel(),
+                                                nat.raw_stream(dev)), "umt_gated_scan_backward")
+    return dx, dgate, dh0
 
 
 def gated_scan_backward(x: torch.Tensor, gate: torch.Tensor, kept: torch.Tensor, dh: torch.Tensor,
@@ -135,49 +154,37 @@ def gated_scan_backward(x: torch.Tensor, gate: torch.Tensor, kept: torch.Tensor,
         raise ValueError(f"gated_scan_backward: x is [T, R, ...], got {tuple(x.shape)}")
     groups, share = _split("gated_scan_backward", x, gate, 2)
     T, R = x.shape[:2]
-    feat, n = tuple(x.shape[2:]), groups * share
     use, ok = _mask("use_memory", use_memory, (T, R), dev), _mask("valid", valid, (T, R), dev)
-    if tuple(dh.shape) != tuple(x.shape) or dh.dtype != x.dtype or dh.device != dev:
+    if not isinstance(dh, torch.Tensor) or dh.shape != x.shape or dh.dtype != x.dtype or dh.device != dev:
         raise ValueError(f"gated_scan_backward: dh is {x.dtype} {tuple(x.shape)} on {dev}")
-    kept = _state("kept", kept, (-(-T // nat.GATED_KEEP), R * n), dev)
+    kept = _state("kept", kept, (-(-T // nat.GATED_KEEP), R * groups * share), dev)
     if kept is None:
         raise ValueError("gated_scan_backward: kept is what gated_scan(..., keep=True) returned")
-    dh_last = _state("dh_last", dh_last, (R,) + feat, dev)
-    xs, gs, ds = _rows_of(x, n), _rows_of(gate, groups), _rows_of(dh, n)
-    dx = _like(x, feat) if need[0] else None
-    dgate = _like(x, tuple(gate.shape[2:])) if need[1] else None
-    dh0 = torch.empty((R,) + feat, dtype=torch.float32, device=dev) if need[2] else None
-    if R * n and any(need):
-        shape = _shape(xs, gs, use, ok, groups, share, dx if dx is not None else xs)
-        shape.dh_t, shape.dh_row = ds.stride(0), ds.stride(1)
-        if dgate is not None:
-            shape.dgate_t, shape.dgate_row = dgate.stride(0), dgate.stride(1)
-        L = nat.lib()
-        with torch.cuda.device(dev):
-            ws = _workspace(L.umt_gated_scan_backward_workspace_bytes(shape), dev)
-            nat.check(L.umt_gated_scan_backward(shape, _raw(xs), _raw(gs), _raw(use), _raw(ok), _raw(kept), _raw(ds), _raw(dh_last),
-                                                _raw(dx), _raw(dgate), _raw(dh0), _raw(ws), 0 if ws is None else ws.numel(),
-                                                nat.stream_ptr(dev)), "umt_gated_scan_backward")
-    return dx, dgate, dh0
+    dh_last = _state("dh_last", dh_last, x.shape[1:], dev)
+    with torch.no_grad():
+        return _backward(x, gate, kept, dh, dh_last, use, ok, groups, share, need)
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, h0, use, valid):
-        h, last, kept = _scan(x, gate, h0, use, valid, keep=True)
+    def forward(ctx, x, gate, h0, use, valid, groups, share):
+        h, last, kept = _scan(x, gate, h0, use, valid, groups, share, keep=True)
         ctx.save_for_backward(x, gate, kept, use, valid)
         ctx.set_materialize_grads(False)
+        ctx.split = groups, share
         return h, last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dh_last):
-        x, gate, kept, use, valid = ctx.saved_tensors
         if dh is None and dh_last is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None, None
+        x, gate, kept, use, valid = ctx.saved_tensors
         if dh is None:
             dh = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
-        return gated_scan_backward(x, gate, kept, dh, dh_last, use, valid, ctx.needs_input_grad[:3]) + (None, None)
+        if dh_last is not None:
+            dh_last = dh_last.contiguous()
+        return _backward(x, gate, kept, dh, dh_last, use, valid, *ctx.split, ctx.needs_input_grad) + (None, None, None, None)
 
 
 def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: Optional[torch.Tensor] = None,
@@ -196,14 +203,15 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: Optional[torch.Tensor] =
     dev = _check_values("gated_scan", x, gate)
     if x.dim() < 2:
         raise ValueError(f"gated_scan: x is [T, R, ...features], got {tuple(x.shape)}")
-    _split("gated_scan", x, gate, 2)
-    T, R = x.shape[:2]
-    h0 = _state("h0", h0, (R,) + tuple(x.shape[2:]), dev)
-    use, ok = _mask("use_memory", use_memory, (T, R), dev), _mask("valid", valid, (T, R), dev)
-    if not keep and torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(x, gate, h0, use, ok)
-    with torch.no_grad():
-        h, last, kept = _scan(x, gate, h0, use, ok, keep)
+    groups, share = _split("gated_scan", x, gate, 2)
+    h0 = _state("h0", h0, x.shape[1:], dev)
+    use, ok = _mask("use_memory", use_memory, x.shape[:2], dev), _mask("valid", valid, x.shape[:2], dev)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
+        if not keep:
+            return _GatedScan.apply(x, gate, h0, use, ok, groups, share)
+        with torch.no_grad():
+            return _scan(x, gate, h0, use, ok, groups, share, True)
+    h, last, kept = _scan(x, gate, h0, use, ok, groups, share, keep)
     return (h, last, kept) if keep else (h, last)
 
 
@@ -225,7 +233,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
         raise nat.UmtError("gated_step is not differentiable: use gated_scan, or call it under torch.no_grad()")
     rows = state.shape[0]
     if memory_idx is not None:
-        if memory_idx.dtype != torch.int64 or tuple(memory_idx.shape) != (B,) or memory_idx.device != dev:
+        if not isinstance(memory_idx, torch.Tensor) or memory_idx.dtype != torch.int64 or tuple(memory_idx.shape) != (B,) or memory_idx.device != dev:
             raise ValueError(f"gated_step: memory_idx is an int64 tensor ({B},) on {dev}")
         memory_idx = memory_idx.contiguous()
     elif B > rows:
@@ -242,9 +250,9 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
         return out
     x, gate = x.contiguous(), gate.contiguous()
     L = nat.lib()
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         ws = _workspace(L.umt_gated_step_workspace_bytes(B, rows) if memory_idx is not None else 0, dev)
-        nat.check(L.umt_gated_step(_DTYPES[x.dtype], _raw(x), _raw(gate), _raw(memory_idx), _raw(use), _raw(ok), B, groups, share,
-                                   _raw(state), rows, _raw(out), _raw(status), _raw(ws), 0 if ws is None else ws.numel(),
-                                   nat.stream_ptr(dev)), "umt_gated_step")
+        nat.check(L.umt_gated_step(_DTYPES[x.dtype], x.data_ptr(), gate.data_ptr(), _raw(memory_idx), _raw(use), _raw(ok), B, groups, share,
+                                   state.data_ptr(), rows, out.data_ptr(), _raw(status), _raw(ws), 0 if ws is None else ws.numel(),
+                                   nat.raw_stream(dev)), "umt_gated_step")
     return out

@@ -94,9 +94,9 @@ def copy_rows(buffers: Sequence, src: torch.Tensor, dst: torch.Tensor, status: O
     if n == 0:
         return
     L = nat.lib()
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         ws, p, size = _work(L.umt_rows_copy_workspace_bytes(arr, n_buf, rows, n), dev)
-        nat.check(L.umt_rows_copy(arr, n_buf, rows, src.data_ptr(), dst.data_ptr(), n, st, p, size, nat.stream_ptr(dev)), "umt_rows_copy")
+        nat.check(L.umt_rows_copy(arr, n_buf, rows, src.data_ptr(), dst.data_ptr(), n, st, p, size, nat.raw_stream(dev)), "umt_rows_copy")
 
 
 def fork_rows(buffers: Sequence, live: torch.Tensor, src: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -111,10 +111,10 @@ def fork_rows(buffers: Sequence, live: torch.Tensor, src: torch.Tensor, status: 
     if n == 0:
         return ids
     L = nat.lib()
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         ws, p, size = _work(L.umt_rows_fork_workspace_bytes(rows, n), dev)
         nat.check(L.umt_rows_fork(arr, n_buf, rows, live.data_ptr(), src.data_ptr(), n, ids.data_ptr(), st, p, size,
-                                  nat.stream_ptr(dev)), "umt_rows_fork")
+                                  nat.raw_stream(dev)), "umt_rows_fork")
     return ids
 
 
@@ -127,8 +127,8 @@ def free_rows(live: torch.Tensor, rows: torch.Tensor, status: Optional[torch.Ten
     st = _status(status, dev)
     if rows.shape[0] == 0:
         return
-    with torch.cuda.device(dev):
-        nat.check(nat.lib().umt_rows_free(live.data_ptr(), live.shape[0], rows.data_ptr(), rows.shape[0], st, nat.stream_ptr(dev)),
+    with nat.on_device(dev):
+        nat.check(nat.lib().umt_rows_free(live.data_ptr(), live.shape[0], rows.data_ptr(), rows.shape[0], st, nat.raw_stream(dev)),
                   "umt_rows_free")
 
 
@@ -142,8 +142,8 @@ def compact_rows(buffers: Sequence, live: torch.Tensor) -> Tuple[torch.Tensor, t
     now = torch.empty(rows, dtype=torch.int64, device=dev)
     count = torch.empty(1, dtype=torch.int64, device=dev)
     L = nat.lib()
-    with torch.cuda.device(dev):
+    with nat.on_device(dev):
         ws, p, size = _work(L.umt_rows_compact_workspace_bytes(rows), dev)
         nat.check(L.umt_rows_compact(arr, n_buf, rows, live.data_ptr(), now.data_ptr(), count.data_ptr(), p, size,
-                                     nat.stream_ptr(dev)), "umt_rows_compact")
+                                     nat.raw_stream(dev)), "umt_rows_compact")
     return now, count

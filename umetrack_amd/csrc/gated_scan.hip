@@ -23,7 +23,7 @@ namespace umt {
 
 constexpr int KEEP = UMT_GATED_KEEP;
 constexpr int GT = 256;
-constexpr int RUN_WAVES = 4;               // runs of a workgroup
+constexpr int RUN_WAVES = 8;               // runs of a workgroup
 
 // E values that a lane loads and stores as one
 template <typename V, int E>
@@ -406,34 +406,27 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
   }
 }
 
-// State with which this wave's run begins: the workgroups before it (BACK: behind it) are joined by the waves, a quarter
-// each, then the runs before it in its own
+// State with which this wave's run begins: the workgroups before it (BACK: behind it) are joined by the waves, an equal
+// share each, then the runs before it in its own
 template <bool BACK, int E>
 __device__ __forceinline__ void enter_run(const float* ws, const Split& P, int64_t N, int64_t e, int tw, int lane, float (&h)[E],
                                           Partners<RUN_WAVES, E>& partners) {
   const int group = blockIdx.y, count = BACK ? P.groups - 1 - group : group, each = (count + RUN_WAVES - 1) / RUN_WAVES;
   const int i0 = min(count, tw * each), i1 = min(count, i0 + each);
   const float* joined = ws + (int64_t)P.groups * RUN_WAVES * 3 * N;
-  Stretch run[E], near[RUN_WAVES][E];
-#pragma unroll
-  for (int k = 0; k < RUN_WAVES; ++k)
-#pragma unroll
-    for (int i = 0; i < E; ++i) near[k][i] = load_stretch(ws + (int64_t)(group * RUN_WAVES + k) * 3 * N, N, e + i);
+  Stretch run[E], own[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
+    own[i] = load_stretch(ws + (int64_t)(group * RUN_WAVES + tw) * 3 * N, N, e + i);
     run[i] = {1.f, 0.f, 0.f};
 #pragma unroll 4
     for (int n = i0; n < i1; ++n) run[i] = then(run[i], load_stretch(joined + (int64_t)(BACK ? P.groups - 1 - n : n) * 3 * N, N, e + i));
   }
-  float unused[E];
+  float unused[E], begin[E];
   partners.template enter<false>(run, tw, lane, h, unused);
+  partners.template enter<BACK>(own, tw, lane, h, begin);
 #pragma unroll
-  for (int n = 0; n < RUN_WAVES; ++n) {
-    const int k = BACK ? RUN_WAVES - 1 - n : n;
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (BACK ? k > tw : k < tw) h[i] = join(h[i], near[k][i]);
-  }
+  for (int i = 0; i < E; ++i) h[i] = begin[i];
 }
 
 template <int W, bool RUNS>
@@ -508,13 +501,14 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
 constexpr int SUM_ROW = 65;                // floats of a step's row: the 16 steps of a read lie in different banks
 
 struct GateSums {
-  int64_t G, group0;       // gates of a step, the wave's first
+  int64_t G, group0, row0; // gates of a step, the wave's first, its row
+  int gi0;                 // and its place in the row
   int count, lead, per;    // gates that the wave holds, lanes of the first that lie before it, lanes
-  int share, slots;
+  int share, slots, slot0; // slot0: waves that hold the first gate before this one
 };
 
 template <typename V>
-__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, int64_t wave, float* rows, const float (&v)[KEEP][1], bool on,
+__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, float* rows, const float (&v)[KEEP][1], bool on,
                                           int t0, V* __restrict__ dgate, float* __restrict__ part) {
   const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4, t = t0 + j;
 #pragma unroll
@@ -537,10 +531,14 @@ __device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSu
     const int64_t group = A.group0 + k;
     if (t < S.t && group < A.G && (many || k0 == 0)) {
       if (n == A.share) {
-        const int64_t r = group / S.groups;
-        store_value(dgate + t * S.dgate_t + r * S.dgate_row + (group - r * S.groups), s);
+        unsigned gi = A.gi0 + k, row = 0;   // at most 64 gates on: one row further where rows have that many
+        if (gi >= (unsigned)S.groups) {
+          row = S.groups >= 64 ? 1 : gi / (unsigned)S.groups;
+          gi -= row * S.groups;
+        }
+        store_value(dgate + t * S.dgate_t + (A.row0 + row) * S.dgate_row + gi, s);
       } else {
-        part[((int64_t)t * A.G + group) * A.slots + (wave - group * A.share / A.per)] = s;
+        part[((int64_t)t * A.G + group) * A.slots + (k == 0 ? A.slot0 : 0)] = s;
       }
     }
   }
@@ -552,14 +550,16 @@ template <typename V>
 __global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int per, int slots, const float* __restrict__ part,
                                                         V* __restrict__ dgate) {
   const int64_t G = (int64_t)S.rows * S.groups;
-  const int64_t k = (int64_t)blockIdx.x * GT + threadIdx.x;
-  if (k >= G * S.t) return;
-  const int64_t t = k / G, g = k - t * G, row = g / S.groups;
+  const int64_t g = (int64_t)blockIdx.x * GT + threadIdx.x;
+  if (g >= G) return;
   const int n = (int)(((g + 1) * S.share - 1) / per - g * S.share / per) + 1;
   if (n == 1) return;
-  float s = 0.f;
-  for (int p = 0; p < n; ++p) s += part[k * slots + p];
-  store_value(dgate + t * S.dgate_t + row * S.dgate_row + (g - row * S.groups), s);
+  const int64_t row = g / S.groups, at = row * S.dgate_row + (g - row * S.groups);
+  for (int64_t t = blockIdx.y; t < S.t; t += gridDim.y) {
+    float s = 0.f;
+    for (int p = 0; p < n; ++p) s += part[(t * G + g) * slots + p];
+    store_value(dgate + t * S.dgate_t + at, s);
+  }
 }
 
 template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
@@ -577,18 +577,32 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backwar
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   Walk<V, E, GE, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
   const Lanes<V, E, OFF> d(dh, S.dh_t, S.dh_row, at.row0, at.row, at.f), out(dx, S.out_t, S.out_row, at.row0, at.row, at.f);
+  GateSums A;
+  A.G = (int64_t)S.rows * S.groups;
+  A.share = S.share / E;
+  A.per = P.per / E;
+  A.row0 = at.row0;
+  A.gi0 = (int)(at.e0 - at.row0 * (S.groups * S.share)) / S.share;
+  A.group0 = at.row0 * S.groups + A.gi0;
+  A.lead = (int)(at.e0 - A.group0 * S.share) / E;
+  A.slots = slots;
+  A.slot0 = (A.lead + A.per - 1) / A.per;
+  A.count = A.share ? (A.lead + A.per + A.share - 1) / A.share : 0;
   Partners<PW, E> partners{reinterpret_cast<float(*)[PW][3 * E][64]>(lds)};
   float v[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] = dh_last ? dh_last[at.e + i] : 0.f;
   if constexpr (RUNS) enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
+  typename Lanes<V, E, OFF>::Raw rd[KEEP];
+  if (part.count > 0) {
+    const int t1 = (part.first + (part.count - 1) * part.by) * KEEP;
+    w.fetch(t1);
+    d.load(t1, S.t, rd);
+  }
   for (int k = part.count - 1; k >= 0; --k) {
     const int c = part.first + k * part.by, t0 = c * KEEP;
     float q[KEEP][E], ms[KEEP][GE], ds[KEEP][E], cur[E];
     unsigned ub, vb;
-    typename Lanes<V, E, OFF>::Raw rd[KEEP];
-    w.fetch(t0);
-    d.load(t0, S.t, rd);
 #pragma unroll
     for (int i = 0; i < E; ++i) cur[i] = t0 < S.t ? kept[(int64_t)c * N + at.e + i] : 0.f;
     w.template take<false>(t0, q, ms, ub, vb);
@@ -602,6 +616,10 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backwar
         q[j][i] = fmaf(-am, am, am) * (cur[i] - xv);
         cur[i] = advance(cur[i], xv, m);
       }
+    }
+    if (k > 0) {
+      w.fetch(t0 - part.by * KEEP);
+      d.load(t0 - part.by * KEEP, S.t, rd);
     }
     if (t0 + KEEP > S.t)
 #pragma unroll
@@ -647,15 +665,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backwar
         const Lanes<V, GE, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
         single.store(t0, S.t, at.on, slope);
       } else if constexpr (GE == 1) {
-        GateSums A;
-        A.G = (int64_t)S.rows * S.groups;
-        A.share = S.share / E;
-        A.per = P.per / E;
-        A.group0 = at.e0 / S.share;
-        A.lead = (int)(at.e0 - A.group0 * S.share) / E;
-        A.slots = slots;
-        A.count = (A.lead + A.per + A.share - 1) / A.share;
-        sum_gates(S, A, part.wave, sums[threadIdx.x >> 6], slope, at.on, t0, dgate, parts);
+        sum_gates(S, A, sums[threadIdx.x >> 6], slope, at.on, t0, dgate, parts);
       }
     }
     if (dh0 && at.on && t0 == 0)
@@ -801,18 +811,19 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
 }
 
 // How the axis is shared out, for waves of `per` values.  A wave that walks alone needs about four others on its CU to keep
-// HBM busy; below that the waves of a workgroup take turns.  Fewer than 64 x 8 waves leave most of the GPU empty: an axis
-// of more than two such tiles is cut into runs then, at the price of reading the inputs twice.
+// HBM busy; below that the waves of a workgroup take turns.  Fewer than 128 workgroups leave half of the CUs without one: an
+// axis of more than two such tiles is cut into runs then, 2048 waves in all, at the price of reading the inputs twice
+// (4000 x 64 x 63 fp32: backward 270 us in tiles, 106 in runs; 2000 x 200 x 63: 165 in tiles, 225 in runs).
 static Split split_axis(const umt_gated_shape& S, int per) {
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   const int all = S.t > 0 ? (S.t + KEEP - 1) / KEEP : 1;
   Split p{per, 1, 0, 1, (N + per - 1) / per};
   if (p.waves >= 1024 || all == 1) return p;
-  if (p.waves >= 64 || all <= 16) {
+  if (p.waves >= 128 || all <= 16) {
     p.w = p.waves >= 256 || all <= 4 ? 4 : 8;
     return p;
   }
-  const int64_t runs = p.waves > 0 ? (1536 + p.waves - 1) / p.waves : 1;
+  const int64_t runs = p.waves > 0 ? (2048 + p.waves - 1) / p.waves : 1;
   p.len = (int)((all + runs - 1) / runs);
   p.groups = (all + p.len * RUN_WAVES - 1) / (p.len * RUN_WAVES);
   return p;
@@ -900,8 +911,9 @@ static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, 
   }
 #undef UMT_SCAN
   if (dgate && slots) {
-    const int64_t gates = (int64_t)S.t * S.rows * S.groups;
-    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)((gates + GT - 1) / GT)), dim3(GT), 0, s, S, per, slots, parts, dgate);
+    // a thread per gate and a few steps: 4096 workgroups where there are that many
+    const int64_t across = ((int64_t)S.rows * S.groups + GT - 1) / GT, along = std::min<int64_t>(S.t, std::max<int64_t>(1, 4096 / across));
+    hipLaunchKernelGGL((gate_parts_kernel<V>), dim3((unsigned)across, (unsigned)along), dim3(GT), 0, s, S, per, slots, parts, dgate);
   }
   UMT_CHECK_HIP(hipGetLastError());
   return 0;

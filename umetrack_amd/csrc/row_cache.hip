@@ -8,6 +8,8 @@
 // Ranks come from per-block counts that every block adds up for itself, in one workgroup where the cache is small.
 #include "umt_internal.h"
 
+#include <type_traits>
+
 namespace umt {
 
 constexpr int RT = 256;
@@ -26,61 +28,81 @@ struct RowBuffers {
   int64_t staged_bytes;
 };
 
-template <typename U>
-__device__ __forceinline__ void load_units(const char* from, int n, int lane, U (&r)[4]) {
-  const U* f = reinterpret_cast<const U*>(from);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < n) r[i] = f[lane + 64 * i];
+// Bytes in HBM and in LDS: addresses of their own kinds, or every access would be a generic one
+using Global = __attribute__((address_space(1))) char*;
+using Local = __attribute__((address_space(3))) char*;
+template <typename P, typename U>
+__device__ __forceinline__ U load_unit(P p, int i) {
+  if constexpr (std::is_same_v<P, Global>)
+    return ((const __attribute__((address_space(1))) U*)p)[i];
+  else
+    return ((const __attribute__((address_space(3))) U*)p)[i];
 }
-template <typename U>
-__device__ __forceinline__ void store_units(char* to, int n, int lane, const U (&r)[4]) {
-  U* t = reinterpret_cast<U*>(to);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < n) t[lane + 64 * i] = r[i];
+template <typename P, typename U>
+__device__ __forceinline__ void store_unit(P p, int i, U v) {
+  if constexpr (std::is_same_v<P, Global>)
+    ((__attribute__((address_space(1))) U*)p)[i] = v;
+  else
+    ((__attribute__((address_space(3))) U*)p)[i] = v;
 }
-template <typename U>
-__device__ __forceinline__ void move_units(char* to, const char* from, int n, int lane) {
-  for (int i = 0; i < n; i += 256) {
+typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+
+template <typename U, typename TO, typename FROM>
+__device__ __forceinline__ void move_units(TO to, FROM from, int n, int lane) {
+  for (int i0 = 0; i0 < n; i0 += 256) {
     U r[4];
-    load_units<U>(from + (int64_t)i * sizeof(U), n - i, lane, r);
-    store_units<U>(to + (int64_t)i * sizeof(U), n - i, lane, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + lane + 64 * i < n) r[i] = load_unit<FROM, U>(from, i0 + lane + 64 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + lane + 64 * i < n) store_unit<TO, U>(to, i0 + lane + 64 * i, r[i]);
   }
 }
 
-// A row's place in buffer k: in the cache, or (staged != null) in a staged row, which is 16-byte aligned
-__device__ __forceinline__ char* place_of(const RowBuffers& B, int k, int64_t row, char* staged) {
-  return staged ? staged + B.staged[k] : B.data[k] + row * B.bytes[k];
-}
+// Where a row lies: in the caches, or in a staged row (16-byte aligned)
+struct Cached {
+  using P = Global;
+  int64_t row;
+  __device__ __forceinline__ P at(const RowBuffers& B, int k) const { return (Global)(B.data[k] + row * B.bytes[k]); }
+};
+template <typename A>
+struct Staged {
+  using P = A;
+  A base;
+  __device__ __forceinline__ P at(const RowBuffers& B, int k) const { return base + B.staged[k]; }
+};
 
 // Piece p of a row, by one wave.  Source and target are different rows, and no other wave writes the one or reads the other.
-__device__ __forceinline__ void move_piece(const RowBuffers& B, int p, int64_t dst, char* to, int64_t src, char* from, int lane) {
+template <typename TO, typename FROM>
+__device__ __forceinline__ void move_piece(const RowBuffers& B, int p, TO to, FROM from, int lane) {
+  using T = typename TO::P;
+  using F = typename FROM::P;
   uint32_t word[UMT_ROW_BUFFERS_MAX];
-  uint4 quad[UMT_ROW_BUFFERS_MAX];
+  Quad quad[UMT_ROW_BUFFERS_MAX];
   const bool tiny = p == 0;
   if (tiny) {
 #pragma unroll
     for (int k = 0; k < UMT_ROW_BUFFERS_MAX; ++k) {
       if (k < B.n_long || k >= B.n) continue;
-      const char* f = place_of(B, k, src, from);
+      const F f = from.at(B, k);
       if (lane * B.unit[k] < B.bytes[k]) {
         if (B.unit[k] == 16)
-          quad[k] = reinterpret_cast<const uint4*>(f)[lane];
+          quad[k] = load_unit<F, Quad>(f, lane);
         else
-          word[k] = B.unit[k] == 4 ? reinterpret_cast<const uint32_t*>(f)[lane] : (uint32_t)reinterpret_cast<const uint8_t*>(f)[lane];
+          word[k] = B.unit[k] == 4 ? load_unit<F, uint32_t>(f, lane) : (uint32_t)load_unit<F, uint8_t>(f, lane);
       }
     }
   }
   if (B.n_long) {
     int k = 0;
     while (k + 1 < B.n_long && p >= B.piece0[k + 1]) ++k;
-    const int64_t at = (int64_t)(p - B.piece0[k]) * MOVE_BYTES, left = B.bytes[k] - at;
+    const int64_t off = (int64_t)(p - B.piece0[k]) * MOVE_BYTES, left = B.bytes[k] - off;
     const int n = (int)(left < MOVE_BYTES ? left : MOVE_BYTES);
-    char* t = place_of(B, k, dst, to) + at;
-    const char* f = place_of(B, k, src, from) + at;
+    const T t = to.at(B, k) + off;
+    const F f = from.at(B, k) + off;
     if (B.unit[k] == 16)
-      move_units<uint4>(t, f, n / 16, lane);
+      move_units<Quad>(t, f, n / 16, lane);
     else if (B.unit[k] == 4)
       move_units<uint32_t>(t, f, n / 4, lane);
     else
@@ -90,17 +112,22 @@ __device__ __forceinline__ void move_piece(const RowBuffers& B, int p, int64_t d
 #pragma unroll
     for (int k = 0; k < UMT_ROW_BUFFERS_MAX; ++k) {
       if (k < B.n_long || k >= B.n) continue;
-      char* t = place_of(B, k, dst, to);
+      const T t = to.at(B, k);
       if (lane * B.unit[k] < B.bytes[k]) {
         if (B.unit[k] == 16)
-          reinterpret_cast<uint4*>(t)[lane] = quad[k];
+          store_unit<T, Quad>(t, lane, quad[k]);
         else if (B.unit[k] == 4)
-          reinterpret_cast<uint32_t*>(t)[lane] = word[k];
+          store_unit<T, uint32_t>(t, lane, word[k]);
         else
-          reinterpret_cast<uint8_t*>(t)[lane] = (uint8_t)word[k];
+          store_unit<T, uint8_t>(t, lane, (uint8_t)word[k]);
       }
     }
   }
+}
+
+// the same in all lanes of a wave: row numbers go into scalar registers, and with them every address of the row
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
 }
 
 __device__ __forceinline__ bool in_cache(int64_t r, int rows) { return r >= 0 && r < rows; }
@@ -161,7 +188,7 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
   extern __shared__ uint4 stage[];
   __shared__ int64_t to[FEW];
   __shared__ int64_t from[FEW];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, pieces = B.piece0[B.n_long];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), pieces = B.piece0[B.n_long];
   for (int i = tid; i < n; i += ONE) {
     const bool ok = in_cache(src[i], rows) && in_cache(dst[i], rows);
     if (!ok && status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
@@ -171,7 +198,7 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
   __syncthreads();
   for (int it = wv; it < n * pieces; it += ONE / 64) {
     const int i = it / pieces;
-    if (to[i] >= 0) move_piece(B, it - i * pieces, 0, (char*)stage + i * B.staged_bytes, from[i], nullptr, lane);
+    if (to[i] >= 0) move_piece(B, it - i * pieces, Staged<Local>{(Local)stage + i * B.staged_bytes}, Cached{uniform(from[i])}, lane);
   }
   __syncthreads();
   for (int it = wv; it < n * pieces; it += ONE / 64) {
@@ -179,7 +206,7 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
     if (to[i] < 0) continue;
     bool last = true;                       // of several writes to one row the highest i counts
     for (int o = i + 1 + lane; o < n; o += 64) last &= to[o] != to[i];
-    if (__all(last)) move_piece(B, it - i * pieces, to[i], nullptr, 0, (char*)stage + i * B.staged_bytes, lane);
+    if (__all(last)) move_piece(B, it - i * pieces, Cached{uniform(to[i])}, Staged<Local>{(Local)stage + i * B.staged_bytes}, lane);
   }
 }
 
@@ -211,25 +238,55 @@ __global__ __launch_bounds__(RT) void copy_list_kernel(const int64_t* __restrict
   const int i = blockIdx.x * RT + threadIdx.x;
   if (i < n && copies(last, src[i], dst[i], i, rows) && last[src[i]] >= 0) todo[4 + atomicAdd(todo, 1)] = i;
 }
+// the three of them in one workgroup, for a copy a thread (a CU takes 50 us over the scattered words of 8191)
+constexpr int INDEX_ONE = ONE;
+__global__ __launch_bounds__(ONE) void copy_index_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n, int rows,
+                                                         int32_t* __restrict__ last, int32_t* __restrict__ todo, int32_t* __restrict__ status) {
+  const int tid = threadIdx.x;
+  if (tid == 0) todo[0] = 0;
+  for (int i = tid; i < n; i += ONE) {
+    if (in_cache(src[i], rows) && in_cache(dst[i], rows)) {
+      last[src[i]] = -1;
+      last[dst[i]] = -1;
+    } else if (status) {
+      atomicOr(status, (int)UMT_STATUS_BAD_ROW);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += ONE)
+    if (in_cache(src[i], rows) && in_cache(dst[i], rows)) atomicMax(last + dst[i], i);
+  __threadfence();
+  __syncthreads();
+  for (int i = tid; i < n; i += ONE) {
+    const int64_t s = src[i], d = dst[i];
+    if (!in_cache(s, rows) || !in_cache(d, rows) || s == d) continue;
+    const int ls = __hip_atomic_load(last + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int ld = __hip_atomic_load(last + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (ld == i && ls >= 0) todo[4 + atomicAdd(todo, 1)] = i;
+  }
+}
 __global__ __launch_bounds__(RT) void copy_stage_kernel(RowBuffers B, const int64_t* __restrict__ src, const int32_t* __restrict__ todo,
                                                         char* __restrict__ stage) {
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
-  const int64_t n = (int64_t)todo[0] * pieces, stride = (int64_t)gridDim.x * (RT / 64);
-  for (int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6); item < n; item += stride) {
-    const int64_t k = item / pieces;
+  const unsigned n = (unsigned)todo[0] * (unsigned)pieces, stride = gridDim.x * (RT / 64);
+  for (unsigned item = blockIdx.x * (RT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); item < n; item += stride) {
+    const unsigned k = item / (unsigned)pieces;
     const int i = todo[4 + k];
-    move_piece(B, (int)(item - k * pieces), 0, stage + i * B.staged_bytes, src[i], nullptr, lane);
+    move_piece(B, (int)(item - k * pieces), Staged<Global>{(Global)(stage + i * B.staged_bytes)}, Cached{uniform(src[i])}, lane);
   }
 }
 __global__ __launch_bounds__(RT) void copy_move_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
                                                        int rows, const int32_t* __restrict__ last, char* stage) {
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
-  const int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6);
-  const int64_t i = item / pieces;
+  const unsigned item = blockIdx.x * (RT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = (int)(item / (unsigned)pieces), p = (int)(item - (unsigned)i * (unsigned)pieces);
   if (i >= n) return;
   const int64_t s = src[i], d = dst[i];
-  if (copies(last, s, d, (int)i, rows))
-    move_piece(B, (int)(item - i * pieces), d, nullptr, s, last[s] >= 0 ? stage + i * B.staged_bytes : nullptr, lane);
+  if (!copies(last, s, d, i, rows)) return;
+  if (last[s] >= 0)
+    move_piece(B, p, Cached{uniform(d)}, Staged<Global>{(Global)(stage + i * B.staged_bytes)}, lane);
+  else
+    move_piece(B, p, Cached{uniform(d)}, Cached{uniform(s)}, lane);
 }
 
 // ---------------------------------------------------------------- fork
@@ -280,9 +337,9 @@ __global__ __launch_bounds__(ONE) void fork_one_kernel(RowBuffers B, uint8_t* li
   if (!moves) return;
   __syncthreads();
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
-  for (int it = threadIdx.x >> 6; it < n * pieces; it += ONE / 64) {
+  for (int it = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < n * pieces; it += ONE / 64) {
     const int i = it / pieces;
-    if (ids[i] >= 0) move_piece(B, it - i * pieces, ids[i], nullptr, src[i], nullptr, lane);
+    if (ids[i] >= 0) move_piece(B, it - i * pieces, Cached{uniform(ids[i])}, Cached{uniform(src[i])}, lane);
   }
 }
 // the same in four launches: counts (live rows a block; good sources a block behind them), order, hand out, move
@@ -320,10 +377,10 @@ __global__ __launch_bounds__(ONE) void fork_rows_kernel(uint8_t* live, int rows,
 // sources are live rows and targets were free ones, so no row is both
 __global__ __launch_bounds__(RT) void fork_move_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ ids, int n) {
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
-  const int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6);
-  const int64_t i = item / pieces;
+  const unsigned item = blockIdx.x * (RT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = (int)(item / (unsigned)pieces);
   if (i >= n || ids[i] < 0) return;
-  move_piece(B, (int)(item - i * pieces), ids[i], nullptr, src[i], nullptr, lane);
+  move_piece(B, (int)(item - (unsigned)i * (unsigned)pieces), Cached{uniform(ids[i])}, Cached{uniform(src[i])}, lane);
 }
 
 // ---------------------------------------------------------------- free
@@ -382,16 +439,17 @@ __global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __rest
 __global__ __launch_bounds__(RT) void compact_move_kernel(RowBuffers B, const int32_t* __restrict__ lists, int rows, uint8_t* __restrict__ live,
                                                           int64_t* __restrict__ now, int64_t* __restrict__ count) {
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long], c = lists[0], moves = lists[1];
-  const int64_t n = (int64_t)moves * pieces, stride = (int64_t)gridDim.x * (RT / 64), all = (int64_t)gridDim.x * RT;
+  const unsigned n = (unsigned)moves * (unsigned)pieces, stride = gridDim.x * (RT / 64);
+  const int64_t all = (int64_t)gridDim.x * RT;
   const int32_t *holes = lists + 4, *movers = holes + rows;
   for (int64_t r = (int64_t)blockIdx.x * RT + threadIdx.x; r < rows; r += all) {
     live[r] = r < c;
     if (r < moves) now[movers[r]] = holes[r];
     if (r == 0) *count = c;
   }
-  for (int64_t item = (int64_t)blockIdx.x * (RT / 64) + (threadIdx.x >> 6); item < n; item += stride) {
-    const int64_t k = item / pieces;
-    move_piece(B, (int)(item - k * pieces), holes[k], nullptr, movers[k], nullptr, lane);
+  for (unsigned item = blockIdx.x * (RT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); item < n; item += stride) {
+    const unsigned k = item / (unsigned)pieces;
+    move_piece(B, (int)(item - k * pieces), Cached{uniform(holes[k])}, Cached{uniform(movers[k])}, lane);
   }
 }
 __global__ void compact_nothing_kernel(int64_t* count) { *count = 0; }
@@ -440,7 +498,7 @@ static int row_buffers(const char* what, const umt_row_buffer* buffers, int n, i
 // workgroups of a move of n rows, a wave per piece
 static int move_grid(const char* what, const RowBuffers& B, int64_t n, unsigned* grid) {
   const int64_t wg = (n * B.piece0[B.n_long] + RT / 64 - 1) / (RT / 64);
-  UMT_REQUIRE(wg < (1LL << 31), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n, B.piece0[B.n_long]);
+  UMT_REQUIRE(n * B.piece0[B.n_long] < (1LL << 31), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n, B.piece0[B.n_long]);
   *grid = (unsigned)wg;
   return 0;
 }
@@ -482,9 +540,13 @@ extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int r
   int32_t* todo = (int32_t*)((char*)workspace + round_up64((int64_t)rows * 4, 16));
   char* stage = (char*)todo + round_up64(16 + (int64_t)n * 4, 16);
   const dim3 per_pair((n + RT - 1) / RT);
-  hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo, status);
-  hipLaunchKernelGGL(copy_claim_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last);
-  hipLaunchKernelGGL(copy_list_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo);
+  if (n <= INDEX_ONE) {
+    hipLaunchKernelGGL(copy_index_kernel, dim3(1), dim3(ONE), 0, s, src, dst, n, rows, last, todo, status);
+  } else {
+    hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo, status);
+    hipLaunchKernelGGL(copy_claim_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last);
+    hipLaunchKernelGGL(copy_list_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo);
+  }
   hipLaunchKernelGGL(copy_stage_kernel, dim3(grid < 2048 ? grid : 2048), dim3(RT), 0, s, B, src, todo, stage);
   hipLaunchKernelGGL(copy_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, dst, n, rows, last, stage);
   UMT_CHECK_HIP(hipGetLastError());

@@ -18,6 +18,7 @@ from typing import Optional
 import torch
 
 from . import _native as nat
+from .lib.common.landmark_filter import LandmarkFilter
 from .lib.models.regressor import RegressorOutput
 from .lib.models.umetrack_model import InputSkeletonData, UmeTrackModel
 from .lib.tracker import warp as gpu_warp
@@ -92,3 +93,12 @@ class BulkSequenceRunner:
             prev_ok = valid_t[t]
         return RegressorOutput(ja_t.transpose(0, 1).reshape(self.S, 22), wx_t.transpose(0, 1).reshape(self.S, 4, 4), None,
                                sg_t.transpose(0, 1).reshape(self.S, 21))
+
+    def smooth_landmarks(self, landmarks: torch.Tensor, filt: LandmarkFilter, out: Optional[RegressorOutput] = None,
+                         valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Landmarks [S,21,3] of ``run``'s poses (skin_landmarks) smoothed along every (recording, hand) row in one call; same
+        order and shape.  ``out``: run's outputs, whose sigmas the filter may weigh by; ``valid`` as ``run``'s."""
+        T, R = self.T, self.n_rec * 2
+        sig = None if out is None else out.landmark_uncertainty_sigmas.view(R, T, 21).transpose(0, 1)
+        h, _ = filt(landmarks.view(R, T, 21, 3).transpose(0, 1), None if valid is None else valid.t(), sig)
+        return h.transpose(0, 1).reshape(self.S, 21, 3)

@@ -28,6 +28,7 @@ from . import synthetic
 from .lib.common import camera
 from .lib.common import metric_utils as mu
 from .lib.common.hand import NUM_HANDS, NUM_LANDMARKS_PER_HAND, HandModel, scaled_hand_model
+from .lib.common.landmark_filter import LandmarkFilter, fit_landmark_filter
 from .lib.tracker.perspective_crop import landmarks_from_hand_pose
 from .lib.tracker.tracker import HandTracker, HandTrackerOpts, InputFrame, ViewData
 from .lib.tracker.tracking_result import SingleHandPose
@@ -182,10 +183,32 @@ def load_result(path: str) -> Dict[str, np.ndarray]:
     return d
 
 
+def smooth_result(d: Dict[str, np.ndarray], filt: LandmarkFilter) -> torch.Tensor:
+    """The tracked keypoints of a result [2,T,21,3], filtered along the recording (on the GPU, float32)."""
+    dev = filt.bias.device
+    with torch.no_grad():
+        h, _ = filt(torch.from_numpy(d["tracked_keypoints"]).to(dev, torch.float32).transpose(0, 1),
+                    torch.from_numpy(d["valid_tracking"]).to(dev).t())
+    return h.transpose(0, 1)
+
+
+def fit_smoothing(files: Sequence[str], filt: LandmarkFilter, **kw) -> LandmarkFilter:
+    """Fits a filter's constants to result files that hold labels (gt_keypoints); see fit_landmark_filter."""
+    dev = filt.bias.device
+    recs = []
+    for d in map(load_result, files):
+        if d["valid_tracking"].any():
+            recs.append((torch.from_numpy(d["tracked_keypoints"]).to(dev, torch.float32).transpose(0, 1),
+                         torch.from_numpy(d["gt_keypoints"]).to(dev, torch.float32).transpose(0, 1),
+                         torch.from_numpy(d["valid_tracking"]).to(dev).t()))
+    return fit_landmark_filter(filt, recs, **kw)
+
+
 def aggregate_metrics(output_dir: str, files: Optional[Sequence[str]] = None, reduce_over_ranks: bool = False,
-                      verbose: bool = True) -> Optional[mu.AggregateMetrics]:
+                      verbose: bool = True, landmark_filter: Optional[LandmarkFilter] = None) -> Optional[mu.AggregateMetrics]:
     """load_eval.py:47-89 with the sums computed by the GPU metric kernel.  With
-    ``reduce_over_ranks`` every rank passes its own ``files`` and all ranks get the global result."""
+    ``reduce_over_ranks`` every rank passes its own ``files`` and all ranks get the global result.
+    ``landmark_filter`` scores the recordings' filtered keypoints instead (the files stay as they are)."""
     if files is None:
         files = find_result_files(output_dir)
     total = None
@@ -193,8 +216,8 @@ def aggregate_metrics(output_dir: str, files: Optional[Sequence[str]] = None, re
         d = load_result(f)
         if d["valid_tracking"].shape[1] == 0:
             continue
-        part = mu.metric_partials(torch.from_numpy(d["gt_keypoints"]), torch.from_numpy(d["tracked_keypoints"]),
-                                  torch.from_numpy(d["valid_tracking"]))
+        tracked = torch.from_numpy(d["tracked_keypoints"]) if landmark_filter is None else smooth_result(d, landmark_filter)
+        part = mu.metric_partials(torch.from_numpy(d["gt_keypoints"]), tracked, torch.from_numpy(d["valid_tracking"]))
         total = part.clone() if total is None else total + part.to(total.device)    # lives where the partials live
     if total is None:
         # a rank without files still takes part in the all-reduce, with zeros on the device the collective runs on:
@@ -274,7 +297,12 @@ def main():
     ap.add_argument("--output", required=True, help="e.g. tmp/eval_results_known_skeleton/real")
     ap.add_argument("--weights", required=True)
     ap.add_argument("--calibration-samples", type=int, default=30)
+    ap.add_argument("--smoothing", type=float, default=None, metavar="W",
+                    help="also report the metrics of the keypoints smoothed along each recording, with weight W in [0, 1) on "
+                         "the filtered past")
     args = ap.parse_args()
+    if args.smoothing is not None and not 0 <= args.smoothing < 1:
+        ap.error("--smoothing takes a weight in [0, 1)")
     logging.basicConfig(level=logging.INFO)
     rank, world, local = udist.init_from_env()
     if not torch.cuda.is_available():
@@ -288,6 +316,11 @@ def main():
     m = aggregate_metrics(args.output, files, reduce_over_ranks=True, verbose=rank == 0)
     if rank == 0 and m is None:
         print("no valid frames")
+    if args.smoothing is not None:
+        if rank == 0:
+            print(f"Keypoints smoothed with memory weight {args.smoothing}:")
+        aggregate_metrics(args.output, files, reduce_over_ranks=True, verbose=rank == 0,
+                          landmark_filter=LandmarkFilter(args.smoothing).to(torch.device("cuda", local)))
 
 
 if __name__ == "__main__":

@@ -15,6 +15,7 @@ from ..common import camera
 from ... import _native as nat
 from ..common.hand import NUM_HANDS, HandModel, hand_model_to, scaled_hand_model
 from ..common.hand_skinning import skin_landmarks
+from ..common.landmark_filter import LandmarkFilter
 from ..models.regressor import RegressorOutput
 from ..models.umetrack_model import InputFrameData, InputFrameDesc, InputSkeletonData
 from . import warp as gpu_warp
@@ -51,6 +52,9 @@ class HandTrackerOpts:
     hand_ratio_in_crop: float = 0.95
     min_required_vis_landmarks: int = 19
     warp_mode: int = gpu_warp.MODE_CV2     # OpenCV-compatible fixed-point sampling (see csrc/warp.hip)
+    # smooths the landmarks that the returned poses carry (landmarks_mm), frame by frame on the GPU; the poses themselves
+    # stay as the model gave them.  None (the reference): landmarks as the frame gave them
+    landmark_filter: Optional[LandmarkFilter] = None
 
 
 def _check_view(vi, img):
@@ -147,7 +151,8 @@ class _FrameIO:
 
     _IN = (("src", np.float64, gpu_warp.SRC_CAM_WORDS, "n"), ("dst", np.float64, gpu_warp.DST_CAM_WORDS, "n"),
            ("off", np.int64, 1, "n"), ("sr", np.int64, 2, "bs"), ("midx", np.int64, 1, "bs"), ("hidx", np.int64, 1, "bs"),
-           ("K", np.float32, 9, "n"), ("E", np.float32, 16, "n"), ("pitch", np.int32, 1, "n"), ("use", np.uint8, 1, "bs"))
+           ("K", np.float32, 9, "n"), ("E", np.float32, 16, "n"), ("pitch", np.int32, 1, "n"), ("use", np.uint8, 1, "bs"),
+           ("fuse", np.uint8, 1, "bs"))
     _OUT = (("status", np.int32, 4, "one"), ("angles", np.float32, 22, "bs"), ("wrist", np.float32, 16, "bs"),
             ("sigmas", np.float32, 21, "bs"), ("scales", np.float32, 1, "bs"), ("lm", np.float32, 63, "bs"))
     _TORCH = {np.float64: torch.float64, np.int64: torch.int64, np.float32: torch.float32, np.int32: torch.int32,
@@ -241,11 +246,17 @@ class HandTracker:
         self._hm_dev: Optional[HandModel] = None
         self._skel: Optional[InputSkeletonData] = None
         self._src_rows = {}                          # id(camera) -> (camera, packed row): rig cameras are constant
+        self._filter = opts.landmark_filter
+        if self._filter is not None:
+            self._filter = self._filter.to(self._io.device)
+            self._filter_state = torch.zeros(NUM_HANDS, 21, 3, device=self._io.device)
+        self._filter_history = np.zeros(NUM_HANDS, dtype=bool)       # hands whose filter row is the last frame's and finite
 
     def reset_history(self, clear_model_memory: bool = False) -> None:
         """tracker.py:98-99 clears the tracking history only (the next frame runs with use_memory=False, which
         neutralises the module memory).  ``clear_model_memory`` additionally drops the model's temporal rows."""
         self._valid_tracking_history[:] = False
+        self._filter_history[:] = False
         if clear_model_memory:
             self._model.reset_memory()
 
@@ -371,6 +382,7 @@ class HandTracker:
         hv["midx"][:, 0] = hands
         hv["hidx"][:, 0] = hands
         hv["use"][:, 0] = self._valid_tracking_history[hands]    # enable_memory is stored but unused, as in the reference
+        hv["fuse"][:, 0] = self._filter_history[hands]
         hv["status"][:] = 0
         io.upload("params")
         crops = gpu_warp.warp_crops(io.devt("pixels"), io.devt("off"), io.devt("pitch"), io.devt("src"), io.devt("dst"),
@@ -401,8 +413,12 @@ class HandTracker:
         status_dev = io.devt("status").view(-1)
         if hand_model_mm is not None:       # the landmarks the eval loop asks for next (perspective_crop.py:40-51)
             _, hm_dev = self._device_hand_model(hand_model_mm)
-            skin_landmarks(hm_dev, out.joint_angles, out.wrist_xfs, hand_idx=io.devt("hidx").view(bs), mirror_right=True,
-                           wrist_translation_scale=M_TO_MM, out=io.devt("lm").view(bs, 21, 3), status=status_dev[1:2])
+            lm = skin_landmarks(hm_dev, out.joint_angles, out.wrist_xfs, hand_idx=io.devt("hidx").view(bs), mirror_right=True,
+                                wrist_translation_scale=M_TO_MM, status=status_dev[1:2],
+                                out=io.devt("lm").view(bs, 21, 3) if self._filter is None else None)
+            if self._filter is not None:    # memory as the model's: it counts when the hand was tracked in the frame before
+                self._filter.step(lm, self._filter_state, io.devt("fuse").view(bs).view(torch.bool), io.devt("midx").view(bs),
+                                  sigmas=out.landmark_uncertainty_sigmas, out=io.devt("lm").view(bs, 21, 3))
         self._model.status_to(status_dev[0:1])
         io.download()
         bits = int(io.host("status")[0, 0]) | int(io.host("status")[0, 1])
@@ -427,4 +443,8 @@ class HandTracker:
                 pred_scales[hand_idx] = scales[row]
         for hand_idx in range(NUM_HANDS):
             self._valid_tracking_history[hand_idx] = hand_idx in poses
+        if self._filter is not None:
+            self._filter_history[:] = False
+            if lms is not None:                 # a pose that is not finite would stay in the filter: its memory is dropped
+                self._filter_history[hands] = np.isfinite(lms).all(axis=(1, 2))
         return TrackingResult(hand_poses=poses, num_views=views, predicted_scales=pred_scales)

@@ -92,23 +92,43 @@ __device__ __forceinline__ float times_a(float m, float s) {
   return from_input(m) ? p : s - p;
 }
 
+// Both weights of a gate, a = 1 / (1 + e) and c = e a with e = exp(-gate), each to a few units of 2^-24 of itself.  The
+// exponent stops at 2^126, where c is 1 and a as good as 0.
+struct Weights {
+  float a, c;
+  static __device__ __forceinline__ Weights of_gate(float g) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269504f, 126.f));     // NaN stays NaN
+    const float a = __builtin_amdgcn_rcpf(1.f + e);
+    return {a, e * a};
+  }
+  static __device__ __forceinline__ Weights of_step(float m) {
+    const float s = fabsf(m), l = 1.f - s;
+    return {from_input(m) ? s : l, from_input(m) ? l : s};
+  }
+  // skipped: (1, 0); memory dropped: (0, 1)
+  __device__ __forceinline__ Weights masked(unsigned use, unsigned valid) const {
+    return {__uint_as_float(((__float_as_uint(a) & valid) | (~valid & 0x3f800000u)) & use),
+            __uint_as_float((__float_as_uint(c) & valid & use) | (~use & 0x3f800000u))};
+  }
+};
+
 // A stretch of steps is a step itself: h_out = p + a h_in.  q = 1 - a is carried on its own (the stretch's response to a
-// memory of 0 and inputs of 1: sums of positive terms), because 1 - a of a rounded a has lost a slow decay.
+// memory of 0 and inputs of 1: sums of positive terms), because 1 - a of a rounded a has lost a slow decay.  p and q are
+// made of the same weights, so a constant input keeps its value whatever their rounding.
 struct Stretch {
   float a, q, p;
   template <bool MASK>
-  __device__ __forceinline__ void forward(float x, float m, unsigned ub, int j) {
-    const float s = fabsf(m), l = 1.f - s, sa = from_input(m) ? s : l, sc = from_input(m) ? l : s;
-    a *= sa;
-    q = fmaf(sa, q, sc);
-    p = fmaf(sa, memory_of<MASK>(p, ub, j), sc * x);
+  __device__ __forceinline__ void forward(float x, const Weights& w, unsigned use) {
+    a *= w.a;
+    q = fmaf(w.a, q, w.c);
+    p = fmaf(w.a, MASK ? masked_value(p, use) : p, w.c * x);
   }
   template <bool MASK>
-  __device__ __forceinline__ void backward(float d, float m, unsigned ub, int j) {
-    const float s = fabsf(m), l = 1.f - s, sa = from_input(m) ? s : l, sc = from_input(m) ? l : s;
-    a *= sa;
-    q = fmaf(sa, q, sc);
-    p = memory_of<MASK>(sa * (d + p), ub, j);
+  __device__ __forceinline__ void backward(float d, const Weights& w, unsigned use) {
+    a *= w.a;
+    q = fmaf(w.a, q, w.c);
+    p = w.a * (d + p);
+    if (MASK) p = masked_value(p, use);
   }
 };
 __device__ __forceinline__ float join(float h, const Stretch& s) {
@@ -132,31 +152,33 @@ __device__ __forceinline__ Global uniform(const void* p) {  // into scalar regis
 }
 
 // One stream of (t, row, feature) values as a wave addresses it: a step's place is the same in all lanes, a lane adds its
-// distance from the wave's first row (OFF = 32 bits unless the rows lie further apart than that)
+// distance from the wave's first row (OFF = 32 bits unless steps or rows lie further apart than that)
 template <typename V, int E, typename OFF>
 struct Lanes {
   using Raw = typename Values<V, E>::Raw;
   using At = __attribute__((address_space(1))) Raw*;
   Global at;               // step 0 of the wave's first row
-  int64_t step;            // bytes
-  OFF mine;                // bytes
+  OFF step, mine;          // bytes
   __device__ __forceinline__ Lanes(const V* p, int64_t t_stride, int64_t row_stride, int64_t row0, int64_t row, int64_t inner) {
     at = uniform(p + row0 * row_stride);
-    step = t_stride * (int64_t)sizeof(V);
+    step = (OFF)(t_stride * (int64_t)sizeof(V));
     mine = (OFF)(((row - row0) * row_stride + inner) * (int64_t)sizeof(V));
   }
   // steps t0 .. t0 + KEEP - 1; those past the end read the last one
   __device__ __forceinline__ void load(int t0, int T, Raw (&r)[KEEP]) const {
-    Global p = at + (t0 < T ? t0 : T - 1) * step;
+    Global p = at + (int64_t)(t0 < T ? t0 : T - 1) * (int64_t)step;
     const int more = T - 1 - t0;            // steps that follow the first
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
       r[j] = *(At)(p + mine);
-      p += j < more ? step : 0;
+      p += j < more ? step : (OFF)0;
     }
   }
+  __device__ __forceinline__ void store_one(int t, const float (&v)[E]) const {
+    *(At)(at + (int64_t)t * (int64_t)step + mine) = Values<V, E>::close(v);
+  }
   __device__ __forceinline__ void store(int t0, int T, bool on, const float (&v)[KEEP][E]) const {
-    Global p = at + t0 * step;
+    Global p = at + (int64_t)t0 * (int64_t)step;
     if (!on) return;
     if (t0 + KEEP <= T) {
 #pragma unroll
@@ -173,20 +195,22 @@ struct Lanes {
 // hands every lane the 16 bits of its own row: one load a stretch where a wave holds up to 4 rows, more only where the
 // rows are shorter than that.
 struct MaskLanes {
-  const uint8_t* p;
-  int64_t st, sr, r0;
-  int rows, span, mine;    // rows of the call, rows of the wave, this lane's row among them
-  __device__ __forceinline__ uint8_t fetch(int t0, int T, int k0) const {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = r0 + k0 + (lane >> 4);
-    const int t = t0 + (lane & 15);
-    return p[(int64_t)(t < T ? t : T - 1) * st + (r < rows ? r : rows - 1) * sr];
+  const uint8_t* p;        // this lane's byte of step 0, of row r0 + lane / 16
+  int64_t st, sr;
+  __device__ __forceinline__ MaskLanes() = default;
+  __device__ __forceinline__ MaskLanes(const uint8_t* m, int64_t st_, int64_t sr_, int64_t r0) : st(st_), sr(sr_) {
+    p = m ? m + (r0 + ((threadIdx.x & 63) >> 4)) * sr_ : nullptr;
   }
-  // `first` = fetch(t0, T, 0), made ahead
-  __device__ __forceinline__ unsigned bits(uint8_t first, int t0, int T) const {
+  // rows past the call's last are not read (they have no lanes)
+  __device__ __forceinline__ uint8_t fetch(int t0, int T, int k0, int rows) const {
+    const int lane = threadIdx.x & 63, t = min(t0 + (lane & 15), T - 1);
+    return k0 + (lane >> 4) < rows ? p[(int64_t)t * st + k0 * sr] : 0;
+  }
+  // `first` = fetch(t0, T, 0, rows), made ahead; rows: of the wave, from its first on; mine: this lane's
+  __device__ __forceinline__ unsigned bits(uint8_t first, int t0, int T, int rows, int mine) const {
     unsigned b = 0;
-    for (int k0 = 0; k0 < span; k0 += 4) {
-      const uint64_t all = __ballot((k0 ? fetch(t0, T, k0) : first) != 0);
+    for (int k0 = 0; k0 < rows; k0 += 4) {
+      const uint64_t all = __ballot((k0 ? fetch(t0, T, k0, rows) : first) != 0);
       if ((mine >> 2) == (k0 >> 2)) b = (unsigned)(all >> (16 * (mine & 3))) & 0xffffu;
     }
     return b;
@@ -220,62 +244,91 @@ template <typename V, int E, int GE, typename OFF, bool MASK>
 struct Walk {
   using X = Lanes<V, E, OFF>;
   using G = Lanes<V, GE, OFF>;
+  // a stretch on its way
+  struct Fetched {
+    typename X::Raw x[KEEP];
+    typename G::Raw g[KEEP];
+    uint8_t use, valid;
+  };
   X x;
   G g;
   MaskLanes um, vm;
-  int T;
-  typename X::Raw rx[KEEP];
-  typename G::Raw rg[KEEP];
-  uint8_t ru, rv;
+  int T, rows, mine;       // rows of the wave, this lane's among them
 
   __device__ __forceinline__ Walk(const umt_gated_shape& S, const Place<E, OFF>& at, const V* x_, int64_t x_t, int64_t x_row, const V* gate_,
                                   const Masks& mk)
       : x(x_, x_t, x_row, at.row0, at.row, at.f), g(gate_, S.gate_t, S.gate_row, at.row0, at.row, at.gi), T(S.t) {
     if (MASK) {
-      int span = (int)(at.row - at.row0);
-      const int mine = span;
+      int span = mine = (int)(at.row - at.row0);
       for (int o = 32; o > 0; o >>= 1) span = max(span, __shfl_xor(span, o));
-      span = __builtin_amdgcn_readfirstlane(span) + 1;
-      um = {mk.use, S.use_t, S.use_row, at.row0, S.rows, span, mine};
-      vm = {mk.valid, S.valid_t, S.valid_row, at.row0, S.rows, span, mine};
+      rows = __builtin_amdgcn_readfirstlane(span) + 1;
+      um = MaskLanes(mk.use, S.use_t, S.use_row, at.row0);
+      vm = MaskLanes(mk.valid, S.valid_t, S.valid_row, at.row0);
     }
   }
-  __device__ __forceinline__ void fetch(int t0) {
+  __device__ __forceinline__ void fetch(int t0, const Masks& mk, Fetched& r) const {
     if (MASK) {
-      if (um.p) ru = um.fetch(t0, T, 0);
-      if (vm.p) rv = vm.fetch(t0, T, 0);
+      if (mk.use) r.use = um.fetch(t0, T, 0, rows);
+      if (mk.valid) r.valid = vm.fetch(t0, T, 0, rows);
     }
-    g.load(t0, T, rg);
-    x.load(t0, T, rx);
+    g.load(t0, T, r.g);
+    x.load(t0, T, r.x);
   }
-  // The fetched stretch: inputs, m of each step, mask bits.  Steps past the end are skipped frames.  BACK: the inputs are
-  // gradients, which no valid mask covers.
-  template <bool BACK>
-  __device__ __forceinline__ void take(int t0, float (&xs)[KEEP][E], float (&ms)[KEEP][GE], unsigned& ub, unsigned& vb) {
+  // mask bits of a fetched stretch; steps past the end are skipped frames
+  __device__ __forceinline__ void bits(const Fetched& r, int t0, const Masks& mk, unsigned& ub, unsigned& vb, unsigned& past) const {
     ub = vb = 0xffffu;
     if (MASK) {
-      if (um.p) ub = um.bits(ru, t0, T);
-      if (vm.p) vb = vm.bits(rv, t0, T);
+      if (mk.use) ub = um.bits(r.use, t0, T, rows, mine);
+      if (mk.valid) vb = vm.bits(r.valid, t0, T, rows, mine);
     }
     const int left = T - t0;
-    const unsigned past = left >= KEEP ? 0u : left <= 0 ? 0xffffu : 0xffffu << left & 0xffffu;
+    past = left >= KEEP ? 0u : left <= 0 ? 0xffffu : 0xffffu << left & 0xffffu;
     ub |= past;
     vb &= ~past;
+  }
+  // the fetched stretch: inputs, m of each step, mask bits
+  __device__ __forceinline__ void take(const Fetched& r, int t0, const Masks& mk, float (&xs)[KEEP][E], float (&ms)[KEEP][GE], unsigned& ub,
+                                       unsigned& vb) const {
+    unsigned past;
+    bits(r, t0, mk, ub, vb, past);
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-      Values<V, E>::open(rx[j], xs[j]);
-      Values<V, GE>::open(rg[j], ms[j]);
+      Values<V, E>::open(r.x[j], xs[j]);
+      Values<V, GE>::open(r.g[j], ms[j]);
 #pragma unroll
       for (int i = 0; i < GE; ++i) ms[j][i] = gate_step(ms[j][i]);
     }
-    if (MASK || left < KEEP) {
+    if (MASK || past) {
 #pragma unroll
       for (int j = 0; j < KEEP; ++j) {
         const unsigned v = bit_mask(vb, j), u = bit_mask(ub, j);
 #pragma unroll
-        for (int i = 0; i < E; ++i) xs[j][i] = masked_value(xs[j][i], BACK ? ~bit_mask(past, j) : v);
+        for (int i = 0; i < E; ++i) xs[j][i] = masked_value(xs[j][i], v);
 #pragma unroll
         for (int i = 0; i < GE; ++i) ms[j][i] = masked_step(ms[j][i], u, v);
+      }
+    }
+  }
+  // the fetched stretch walked from state st on: states (a step's registers are free again behind it)
+  __device__ __forceinline__ void follow(const Fetched& r, int t0, const Masks& mk, float (&st)[E], float (&hs)[KEEP][E]) const {
+    unsigned ub, vb, past;
+    bits(r, t0, mk, ub, vb, past);
+    const bool some = MASK || past;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      const unsigned v = bit_mask(vb, j), u = bit_mask(ub, j);
+      float xv[E], m[GE];
+      Values<V, E>::open(r.x[j], xv);
+      Values<V, GE>::open(r.g[j], m);
+#pragma unroll
+      for (int i = 0; i < GE; ++i) {
+        m[i] = gate_step(m[i]);
+        if (some) m[i] = masked_step(m[i], u, v);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (some) xv[i] = masked_value(xv[i], v);
+        hs[j][i] = st[i] = advance(MASK ? masked_value(st[i], u) : st[i], xv[i], m[i % GE]);
       }
     }
   }
@@ -358,33 +411,53 @@ template <typename V, int E, int GE, typename OFF, bool MASK, bool BACK>
 __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_shape S, Split P, const V* __restrict__ v, int64_t v_t, int64_t v_row,
                                                                     const V* __restrict__ gate, Masks mk, float* __restrict__ ws) {
   __shared__ float lds[RUN_WAVES][3 * E][64];
+  using W = Walk<V, E, GE, OFF, MASK>;
   const int lane = threadIdx.x & 63;
   const Part<1, true> part(P, S.t);
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, E, GE, OFF, MASK> w(S, at, v, v_t, v_row, gate, mk);
+  const W w(S, at, v, v_t, v_row, gate, mk);
   Stretch own[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
   const int last = part.first + part.count - 1;
-  if (part.count > 0) w.fetch((BACK ? last : part.first) * KEEP);
-  for (int k = 0; k < part.count; ++k) {
-    const int t0 = (BACK ? last - k : part.first + k) * KEEP;
-    float xs[KEEP][E], ms[KEEP][GE];
-    unsigned ub, vb;
-    w.template take<BACK>(t0, xs, ms, ub, vb);
-    if (k + 1 < part.count) w.fetch(BACK ? t0 - KEEP : t0 + KEEP);
+  auto start = [&](int k) { return (BACK ? last - k : part.first + k) * KEEP; };
+  auto walk = [&](int k, const typename W::Fetched& now, typename W::Fetched& next) __attribute__((always_inline)) {
+    const int t0 = start(k);
+    if (k + 1 < part.count) w.fetch(start(k + 1), mk, next);
+    unsigned ub, vb, past;
+    w.bits(now, t0, mk, ub, vb, past);
+    const bool some = MASK || past;
 #pragma unroll
     for (int n = 0; n < KEEP; ++n) {
       const int j = BACK ? KEEP - 1 - n : n;
+      const unsigned u = bit_mask(ub, j), va = bit_mask(vb, j);
+      float x[E], g[GE];
+      Values<V, E>::open(now.x[j], x);
+      Values<V, GE>::open(now.g[j], g);
+      Weights wt[GE];
+#pragma unroll
+      for (int i = 0; i < GE; ++i) {
+        wt[i] = Weights::of_gate(g[i]);
+        if (some) wt[i] = wt[i].masked(u, va);
+      }
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        if (BACK)
-          own[i].template backward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
-        else
-          own[i].template forward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
+        if (BACK) {
+          if (past) x[i] = masked_value(x[i], ~bit_mask(past, j));           // gradients: no valid mask covers them
+          own[i].template backward<MASK>(x[i], wt[i % GE], u);
+        } else {
+          if (some) x[i] = masked_value(x[i], va);
+          own[i].template forward<MASK>(x[i], wt[i % GE], u);
+        }
       }
     }
+  };
+  typename W::Fetched a, b;                // two in turn: no copies between them
+  if (part.count > 0) w.fetch(start(0), mk, a);
+  for (int k = 0; k < part.count; k += 2) {
+    walk(k, a, b);
+    if (k + 1 < part.count) walk(k + 1, b, a);
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) {
@@ -447,48 +520,57 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
   if (W == 1 && !RUNS && part.wave >= P.waves) return;
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, E, GE, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  using Wk = Walk<V, E, GE, OFF, MASK>;
+  const Wk w(S, at, x, S.x_t, S.x_row, gate, mk);
   const Lanes<V, E, OFF> out(h, S.out_t, S.out_row, at.row0, at.row, at.f);
-  if (part.count > 0) w.fetch(part.first * KEEP);
+  typename Wk::Fetched fa, fb;             // two in turn: no copies between them
+  if (part.count > 0) w.fetch(part.first * KEEP, mk, fa);
   Partners<PW, E> partners{reinterpret_cast<float(*)[PW][3 * E][64]>(lds)};
   float cur[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) cur[i] = h0 ? h0[at.e + i] : 0.f;
   if constexpr (RUNS) enter_run<false>(ws, P, N, at.e, part.tw, lane, cur, partners);
-  for (int k = 0; k < part.count; ++k) {
+  auto keep = [&](int c, const float(&st)[E]) __attribute__((always_inline)) {
+    if (kept && at.on)
+#pragma unroll
+      for (int i = 0; i < E; ++i) kept[(int64_t)c * N + at.e + i] = st[i];
+  };
+  auto walk = [&](int k, const typename Wk::Fetched& now, typename Wk::Fetched& next) __attribute__((always_inline)) {
     const int c = part.first + k * part.by, t0 = c * KEEP;
-    float xs[KEEP][E], ms[KEEP][GE], st[E];
-    unsigned ub, vb;
-    w.template take<false>(t0, xs, ms, ub, vb);
-    if (k + 1 < part.count) w.fetch(t0 + part.by * KEEP);
-    if (W > 1) {
+    float hs[KEEP][E], st[E];
+    if (k + 1 < part.count) w.fetch(t0 + part.by * KEEP, mk, next);
+    if constexpr (W > 1) {
+      float ms[KEEP][GE];
+      unsigned ub, vb;
+      w.take(now, t0, mk, hs, ms, ub, vb);
       Stretch own[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < KEEP; ++j)
 #pragma unroll
-        for (int i = 0; i < E; ++i) own[i].template forward<MASK>(xs[j][i], ms[j][i % GE], ub, j);
+        for (int i = 0; i < E; ++i) own[i].template forward<MASK>(hs[j][i], Weights::of_step(ms[j][i % GE]), bit_mask(ub, j));
       partners.template enter<false>(own, part.tw, lane, cur, st);
-      if (t0 >= S.t) continue;
+      if (t0 >= S.t) return;
+      keep(c, st);
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j)
+#pragma unroll
+        for (int i = 0; i < E; ++i) hs[j][i] = st[i] = advance(memory_of<MASK>(st[i], ub, j), hs[j][i], ms[j][i % GE]);
     } else {
+      keep(c, cur);
+      w.follow(now, t0, mk, cur, hs);
 #pragma unroll
       for (int i = 0; i < E; ++i) st[i] = cur[i];
     }
-    if (kept && at.on)
-#pragma unroll
-      for (int i = 0; i < E; ++i) kept[(int64_t)c * N + at.e + i] = st[i];
-#pragma unroll
-    for (int j = 0; j < KEEP; ++j)
-#pragma unroll
-      for (int i = 0; i < E; ++i) xs[j][i] = st[i] = advance(memory_of<MASK>(st[i], ub, j), xs[j][i], ms[j][i % GE]);
-    out.store(t0, S.t, at.on, xs);
+    out.store(t0, S.t, at.on, hs);
     if (h_last && at.on && t0 + KEEP >= S.t)
 #pragma unroll
       for (int i = 0; i < E; ++i) h_last[at.e + i] = st[i];
-    if (W == 1)
-#pragma unroll
-      for (int i = 0; i < E; ++i) cur[i] = st[i];
+  };
+  for (int k = 0; k < part.count; k += 2) {
+    walk(k, fa, fb);
+    if (k + 1 < part.count) walk(k + 1, fb, fa);
   }
 }
 
@@ -496,49 +578,78 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
 // Sums over the features of a gate.  A wave's lanes hold consecutive features, so a gate's are a run of lanes (a lane's own
 // two are added first; `share` and `per` count lanes here).  The KEEP
 // steps' products go through the wave's own LDS rows; lane 16 k + j adds up step j: whole gates k, k + 4, ... where the
-// wave holds many, a quarter of each where it holds few.  A gate that reaches into other waves leaves its part in `part`, and
+// wave holds many, every fourth product of each where it holds few.  A gate that reaches into other waves leaves its part in `part`, and
 // a second launch adds the parts in order.
 constexpr int SUM_ROW = 65;                // floats of a step's row: the 16 steps of a read lie in different banks
 
-struct GateSums {
-  int64_t G, group0, row0; // gates of a step, the wave's first, its row
-  int gi0;                 // and its place in the row
-  int count, lead, per;    // gates that the wave holds, lanes of the first that lie before it, lanes
-  int share, slots, slot0; // slot0: waves that hold the first gate before this one
-};
+constexpr int SUM_ROWS = KEEP * SUM_ROW + 64;      // reads past a gate's end are thrown away, but made
 
 template <typename V>
-__device__ __forceinline__ void sum_gates(const umt_gated_shape& S, const GateSums& A, float* rows, const float (&v)[KEEP][1], bool on,
-                                          int t0, V* __restrict__ dgate, float* __restrict__ part) {
-  const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4, t = t0 + j;
+struct GateSums {
+  int gi0, groups;         // the wave's first gate in its row, gates of a row
+  int left;                // gates from the wave's first to the call's last
+  int count, lead, per;    // gates that the wave holds, lanes of the first that lie before it, lanes
+  int share, slots, slot0; // slot0: waves that hold the first gate before this one
+  int64_t row_step;        // of dgate
+  V* to;                   // the first gate's places at step (lane & 15) of the axis
+  float* part;
+  __device__ __forceinline__ GateSums(const umt_gated_shape& S, int64_t row0, int64_t e0, int E, int per_, int slots_, V* dgate, float* parts) {
+    const int j = threadIdx.x & 15;
+    const int64_t G = (int64_t)S.rows * S.groups, inner = e0 - row0 * (S.groups * S.share);
+    gi0 = (int)inner / S.share;
+    groups = S.groups;
+    const int64_t group0 = row0 * S.groups + gi0;
+    left = (int)(G - group0 < 1 << 20 ? G - group0 : 1 << 20);
+    share = S.share / E;
+    per = per_ / E;
+    lead = ((int)inner - gi0 * S.share) / E;
+    slots = slots_;
+    slot0 = (lead + per - 1) / per;
+    count = share ? (lead + per + share - 1) / share : 0;
+    row_step = S.dgate_row;
+    to = dgate + j * S.dgate_t + row0 * S.dgate_row + gi0;
+    part = parts + ((int64_t)j * G + group0) * slots;
+  }
+};
+
+// v: this lane's products of KEEP steps; rows: the wave's LDS; the steps from t0 on lie to_t0 and part_t0 elements on
+template <typename V>
+__device__ __forceinline__ void sum_gates(const GateSums<V>& A, float* rows, const float (&v)[KEEP][1], bool on, int steps, int64_t to_t0,
+                                          int64_t part_t0) {
+  const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4;
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) rows[i * SUM_ROW + lane] = on ? v[i][0] : 0.f;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   const float* row = rows + j * SUM_ROW;
   const bool many = A.count > 6;
+  const int by = many ? 1 : 4, mine = many ? 0 : k0;
   for (int k = many ? k0 : 0; k < A.count; k += many ? 4 : 1) {
     const int lo = max(0, k * A.share - A.lead), hi = min(A.per, (k + 1) * A.share - A.lead), n = hi - lo;
     float s = 0.f;
-    if (many) {
-      for (int i = lo; i < hi; ++i) s += row[i];
-    } else {
-      const int each = (n + 3) >> 2, i1 = min(hi, lo + (k0 + 1) * each);
-      for (int i = lo + k0 * each; i < i1; ++i) s += row[i];
+    for (int m = 0; m < A.share; m += 4 * by) {            // four reads in flight, added in a fixed order
+      float r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = row[lo + mine + m + i * by];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = mine + m + i * by < n ? r[i] : 0.f;
+      s += (r[0] + r[1]) + (r[2] + r[3]);
+      if (!many && m + 16 >= n) break;
+    }
+    if (!many) {
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
     }
-    const int64_t group = A.group0 + k;
-    if (t < S.t && group < A.G && (many || k0 == 0)) {
+    if (j < steps && k < A.left && (many || k0 == 0)) {
       if (n == A.share) {
-        unsigned gi = A.gi0 + k, row = 0;   // at most 64 gates on: one row further where rows have that many
-        if (gi >= (unsigned)S.groups) {
-          row = S.groups >= 64 ? 1 : gi / (unsigned)S.groups;
-          gi -= row * S.groups;
+        int gi = k, row_on = 0;              // at most 64 gates on: one row further where rows have that many
+        if (A.gi0 + k >= A.groups) {
+          row_on = A.groups >= 64 ? 1 : (int)((unsigned)(A.gi0 + k) / (unsigned)A.groups);
+          gi -= row_on * A.groups;
         }
-        store_value(dgate + t * S.dgate_t + (A.row0 + row) * S.dgate_row + gi, s);
+        store_value(A.to + to_t0 + (row_on * A.row_step + gi), s);
       } else {
-        part[((int64_t)t * A.G + group) * A.slots + (k == 0 ? A.slot0 : 0)] = s;
+        A.part[part_t0 + k * A.slots + (k == 0 ? A.slot0 : 0)] = s;
       }
     }
   }
@@ -563,78 +674,84 @@ __global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int p
 }
 
 template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
-__global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backward_kernel(
+__global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_backward_kernel(
     umt_gated_shape S, Split P, int slots, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
     const V* __restrict__ dh, const float* __restrict__ dh_last, const float* __restrict__ ws, V* __restrict__ dx, V* __restrict__ dgate,
     float* __restrict__ parts, float* __restrict__ dh0) {
   constexpr int PW = partner_waves<W, RUNS>(), GW = group_threads<W, RUNS>() / 64;
   __shared__ float lds[PW > 1 ? 2 : 1][PW][3 * E][64];
-  __shared__ float sums[GW][KEEP * SUM_ROW];
+  __shared__ float sums[GW][SUM_ROWS];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
   if (W == 1 && !RUNS && part.wave >= P.waves) return;
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
-  Walk<V, E, GE, OFF, MASK> w(S, at, x, S.x_t, S.x_row, gate, mk);
+  using Wk = Walk<V, E, GE, OFF, MASK>;
+  const Wk w(S, at, x, S.x_t, S.x_row, gate, mk);
   const Lanes<V, E, OFF> d(dh, S.dh_t, S.dh_row, at.row0, at.row, at.f), out(dx, S.out_t, S.out_row, at.row0, at.row, at.f);
-  GateSums A;
-  A.G = (int64_t)S.rows * S.groups;
-  A.share = S.share / E;
-  A.per = P.per / E;
-  A.row0 = at.row0;
-  A.gi0 = (int)(at.e0 - at.row0 * (S.groups * S.share)) / S.share;
-  A.group0 = at.row0 * S.groups + A.gi0;
-  A.lead = (int)(at.e0 - A.group0 * S.share) / E;
-  A.slots = slots;
-  A.slot0 = (A.lead + A.per - 1) / A.per;
-  A.count = A.share ? (A.lead + A.per + A.share - 1) / A.share : 0;
+  const Lanes<V, GE, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
+  const GateSums<V> A(S, at.row0, at.e0, E, P.per, slots, dgate, parts);
   Partners<PW, E> partners{reinterpret_cast<float(*)[PW][3 * E][64]>(lds)};
   float v[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] = dh_last ? dh_last[at.e + i] : 0.f;
   if constexpr (RUNS) enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
+  typename Wk::Fetched now;                // a stretch ahead; its gradients are asked for when it begins and needed last
   typename Lanes<V, E, OFF>::Raw rd[KEEP];
-  if (part.count > 0) {
-    const int t1 = (part.first + (part.count - 1) * part.by) * KEEP;
-    w.fetch(t1);
-    d.load(t1, S.t, rd);
-  }
+  float first[E];
+  auto fetch = [&](int k) __attribute__((always_inline)) {
+    const int c = part.first + k * part.by;
+    w.fetch(c * KEEP, mk, now);
+#pragma unroll
+    for (int i = 0; i < E; ++i) first[i] = c * KEEP < S.t ? kept[(int64_t)c * N + at.e + i] : 0.f;
+  };
+  if (part.count > 0) fetch(part.count - 1);
   for (int k = part.count - 1; k >= 0; --k) {
-    const int c = part.first + k * part.by, t0 = c * KEEP;
-    float q[KEEP][E], ms[KEEP][GE], ds[KEEP][E], cur[E];
-    unsigned ub, vb;
+    const int t0 = (part.first + k * part.by) * KEEP;
+    float q[KEEP][E], ms[KEEP][GE], cur[E];
+    unsigned ub, vb, past;
+    d.load(t0, S.t, rd);
+    w.bits(now, t0, mk, ub, vb, past);
+    const bool some = MASK || past;
 #pragma unroll
-    for (int i = 0; i < E; ++i) cur[i] = t0 < S.t ? kept[(int64_t)c * N + at.e + i] : 0.f;
-    w.template take<false>(t0, q, ms, ub, vb);
+    for (int i = 0; i < E; ++i) cur[i] = first[i];
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {        // the states again; q becomes c a (h[t-1] - x[t]), the slope over the gate
-      Values<V, E>::open(rd[j], ds[j]);
+    for (int j = 0; j < KEEP; ++j) {        // the states again; q is c a (h[t-1] - x[t]), the slope over the gate
+      const unsigned va = bit_mask(vb, j), u = bit_mask(ub, j);
+      Values<V, E>::open(now.x[j], q[j]);
+      Values<V, GE>::open(now.g[j], ms[j]);
+#pragma unroll
+      for (int i = 0; i < GE; ++i) {
+        ms[j][i] = gate_step(ms[j][i]);
+        if (some) ms[j][i] = masked_step(ms[j][i], u, va);
+      }
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float m = ms[j][i % GE], am = fabsf(m), xv = q[j][i];
-        cur[i] = memory_of<MASK>(cur[i], ub, j);
-        q[j][i] = fmaf(-am, am, am) * (cur[i] - xv);
-        cur[i] = advance(cur[i], xv, m);
+        const float m = ms[j][i % GE], am = fabsf(m), x = some ? masked_value(q[j][i], va) : q[j][i];
+        if (MASK) cur[i] = masked_value(cur[i], u);
+        q[j][i] = fmaf(-am, am, am) * (cur[i] - x);
+        cur[i] = advance(cur[i], x, m);
       }
     }
-    if (k > 0) {
-      w.fetch(t0 - part.by * KEEP);
-      d.load(t0 - part.by * KEEP, S.t, rd);
-    }
-    if (t0 + KEEP > S.t)
+    if (k > 0) fetch(k - 1);
+    auto gradient = [&](int j, float(&g)[E]) __attribute__((always_inline)) {
+      Values<V, E>::open(rd[j], g);
+      if (past)
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j)
-#pragma unroll
-        for (int i = 0; i < E; ++i) ds[j][i] = t0 + j < S.t ? ds[j][i] : 0.f;
+        for (int i = 0; i < E; ++i) g[i] = masked_value(g[i], ~bit_mask(past, j));
+    };
     float b[E];
-    if (W > 1) {
+    if constexpr (W > 1) {
       Stretch own[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = KEEP - 1; j >= 0; --j)
+      for (int j = KEEP - 1; j >= 0; --j) {
+        float g[E];
+        gradient(j, g);
 #pragma unroll
-        for (int i = 0; i < E; ++i) own[i].template backward<MASK>(ds[j][i], ms[j][i % GE], ub, j);
+        for (int i = 0; i < E; ++i) own[i].template backward<MASK>(g[i], Weights::of_step(ms[j][i % GE]), bit_mask(ub, j));
+      }
       partners.template enter<true>(own, part.tw, lane, v, b);
       if (t0 >= S.t) continue;
     } else {
@@ -642,32 +759,40 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_backwar
       for (int i = 0; i < E; ++i) b[i] = v[i];
     }
     float slope[KEEP][GE];
+    asm volatile("" : "+v"(ub), "+v"(vb));  // the mask words anew: 32 registers of them across the two loops cost more
+    auto down = [&](auto whole) __attribute__((always_inline)) {
+      constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int j = KEEP - 1; j >= 0; --j) {
+      for (int j = KEEP - 1; j >= 0; --j) {
+        if (!WHOLE && t0 + j >= S.t) continue;
+        float g[E], x[E];
+        Values<V, E>::open(rd[j], g);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float m = ms[j][i % GE], s = ds[j][i] + b[i], l = s * q[j][i];
-        if (i < GE)
-          slope[j][i] = l;
-        else
-          slope[j][0] += l;
-        ds[j][i] = times_c(m, s);
-        if (MASK) ds[j][i] = masked_value(ds[j][i], bit_mask(vb, j));
-        b[i] = memory_of<MASK>(times_a(m, s), ub, j);
+        for (int i = 0; i < E; ++i) {
+          const float m = ms[j][i % GE], s = g[i] + b[i], l = s * q[j][i];
+          if (i < GE)
+            slope[j][i] = l;
+          else
+            slope[j][0] += l;
+          x[i] = times_c(m, s);
+          if (MASK) x[i] = masked_value(x[i], bit_mask(vb, j));
+          b[i] = memory_of<MASK>(times_a(m, s), ub, j);
+        }
+        if (MASK)
+#pragma unroll
+          for (int i = 0; i < GE; ++i) slope[j][i] = masked_value(slope[j][i], bit_mask(ub & vb, j));
+        if (dx) out.store_one(t0 + j, x);
+        if (dgate && S.share == 1) single.store_one(t0 + j, slope[j]);
       }
-      if (MASK)
-#pragma unroll
-        for (int i = 0; i < GE; ++i) slope[j][i] = masked_value(slope[j][i], bit_mask(ub & vb, j));
+    };
+    if (at.on) {
+      if (t0 + KEEP <= S.t)
+        down(std::true_type());
+      else
+        down(std::false_type());
     }
-    if (dx) out.store(t0, S.t, at.on, ds);
-    if (dgate) {
-      if (S.share == 1) {
-        const Lanes<V, GE, OFF> single(dgate, S.dgate_t, S.dgate_row, at.row0, at.row, at.gi);
-        single.store(t0, S.t, at.on, slope);
-      } else if constexpr (GE == 1) {
-        sum_gates(S, A, sums[threadIdx.x >> 6], slope, at.on, t0, dgate, parts);
-      }
-    }
+    if constexpr (GE == 1)
+      if (dgate && S.share > 1) sum_gates(A, sums[threadIdx.x >> 6], slope, at.on, S.t - t0, (int64_t)t0 * S.dgate_t, (int64_t)t0 * S.rows * S.groups * slots);
     if (dh0 && at.on && t0 == 0)
 #pragma unroll
       for (int i = 0; i < E; ++i) dh0[at.e + i] = b[i];
@@ -853,14 +978,16 @@ static bool pairs(const umt_gated_shape& S, const void* x, const void* gate, con
          (S.share > 1 || (even(S.gate_t, S.gate_row, gate) && (!dgate || even(S.dgate_t, S.dgate_row, dgate))));
 }
 
-// whether 32 bits address a wave's lanes from its first row in every stream (128 features are at most 128 rows), and
-// count the features of the call
+// whether 32 bits hold a step's distance and a lane's from its wave's first row in every stream (128 features are at most
+// 128 rows), and count the features of the call
 static bool near_rows(const umt_gated_shape& S, int64_t size) {
   const int F = S.groups * S.share;
   const int64_t rows = F >= 128 ? 2 : 128 / F + 2;
-  const int64_t st[] = {S.x_row, S.gate_row, S.out_row, S.dh_row, S.dgate_row};
-  for (int64_t r : st)
+  const int64_t by_row[] = {S.x_row, S.gate_row, S.out_row, S.dh_row, S.dgate_row}, by_step[] = {S.x_t, S.gate_t, S.out_t, S.dh_t, S.dgate_t};
+  for (int64_t r : by_row)
     if (r > ((1LL << 31) / size - F) / rows) return false;
+  for (int64_t t : by_step)
+    if (t >= (1LL << 31) / size) return false;
   return (int64_t)S.rows * F < (1LL << 31) - 128;
 }
 

@@ -351,6 +351,34 @@ def test_masks_across_stretches_and_segments(T):
         assert np.isfinite(a).all() and (np.abs(a - b) <= tol + 2 * U * np.abs(b)).all(), name
 
 
+@pytest.mark.parametrize("T", [40, 3000])
+def test_what_is_not_finite_stays_in_its_feature_until_the_memory_is_dropped(T):
+    """A NaN or infinite input, gate or state that no mask excludes: its feature is not finite from there to the drop, in
+    every stretch and run on the way, and no other feature notices.  Infinite gates hold or replace."""
+    R, G, K = 3, 4, 2
+    x, gate, h0, _, _ = make(T, R, G, K, "fp32", T, masks=False)
+    clean, _ = _gf().gated_scan(x, gate, h0)
+    drop = 3 * T // 4
+    use = torch.ones(T, R, dtype=torch.bool, device="cuda")
+    use[drop] = False
+    dropped, _ = _gf().gated_scan(x, gate, h0, use)
+    x[T // 8, 0, 1, 0] = float("nan")
+    x[T // 8, 0, 2, 1] = float("inf")
+    gate[T // 4, 1, 3] = float("nan")
+    h0[2, 0, 0] = -float("inf")
+    h, last = _gf().gated_scan(x, gate, h0, use)
+    bad = torch.zeros(T, R, G, K, dtype=torch.bool, device="cuda")
+    bad[T // 8:drop, 0, 1, 0] = bad[T // 8:drop, 0, 2, 1] = bad[:drop, 2, 0, 0] = True
+    bad[T // 4:drop, 1, 3] = True
+    assert torch.equal(~torch.isfinite(h), bad) and bool(torch.isfinite(last).all())
+    assert torch.equal(h[~bad], dropped[~bad]) and torch.equal(dropped[:drop], clean[:drop])
+    gate = torch.full((T, R), float("inf"), device="cuda")
+    gate[T // 2] = -float("inf")
+    x = torch.rand(T, R, K, device="cuda")
+    h, _ = _gf().gated_scan(x, gate, h0[:, 0].nan_to_num(0, 0, 0))
+    assert torch.equal(h[T // 2:], x[T // 2].expand(T - T // 2, R, K))
+
+
 def test_other_stream_and_graph_replays():
     """Forward and backward captured into one graph, replayed with new contents between eager work and synchronisations."""
     gf = _gf()

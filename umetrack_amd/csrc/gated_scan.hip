@@ -130,13 +130,18 @@ struct Stretch {
     p = w.a * (d + p);
     if (MASK) p = masked_value(p, use);
   }
+  // a = 0 is kept for a memory that was dropped (`ub`: the use bits of all steps): one that has merely faded below every
+  // float still hands on what is not finite
+  __device__ __forceinline__ void close(unsigned ub) { a = (ub & 0xffffu) != 0xffffu ? 0.f : fmaxf(a, FADED); }
+  static constexpr float FADED = 1.4e-45f;
 };
 __device__ __forceinline__ float join(float h, const Stretch& s) {
   const float slow = h + fmaf(-s.q, h, s.p), fast = fmaf(s.a, h, s.p);
   return s.a == 0.f ? s.p : s.q <= 0.5f ? slow : fast;      // a = 0: the memory was dropped on the way, whatever h holds
 }
 __device__ __forceinline__ Stretch then(const Stretch& f, const Stretch& s) {
-  return Stretch{f.a * s.a, join(f.q, Stretch{s.a, s.q, s.q}), join(f.p, s)};
+  const float a = f.a == 0.f || s.a == 0.f ? 0.f : fmaxf(f.a * s.a, Stretch::FADED);
+  return Stretch{a, join(f.q, Stretch{s.a, s.q, s.q}), join(f.p, s)};
 }
 
 struct Masks {
@@ -420,6 +425,7 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
   Stretch own[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) own[i] = {1.f, 0.f, 0.f};
+  unsigned all_use = ~0u;
   const int last = part.first + part.count - 1;
   auto start = [&](int k) { return (BACK ? last - k : part.first + k) * KEEP; };
   auto walk = [&](int k, const typename W::Fetched& now, typename W::Fetched& next) __attribute__((always_inline)) {
@@ -427,6 +433,7 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
     if (k + 1 < part.count) w.fetch(start(k + 1), mk, next);
     unsigned ub, vb, past;
     w.bits(now, t0, mk, ub, vb, past);
+    all_use &= ub;
     const bool some = MASK || past;
 #pragma unroll
     for (int n = 0; n < KEEP; ++n) {
@@ -461,6 +468,7 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) {
+    own[i].close(all_use);
     lds[part.tw][3 * i][lane] = own[i].a;
     lds[part.tw][3 * i + 1][lane] = own[i].q;
     lds[part.tw][3 * i + 2][lane] = own[i].p;
@@ -550,6 +558,8 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
       for (int j = 0; j < KEEP; ++j)
 #pragma unroll
         for (int i = 0; i < E; ++i) own[i].template forward<MASK>(hs[j][i], Weights::of_step(ms[j][i % GE]), bit_mask(ub, j));
+#pragma unroll
+      for (int i = 0; i < E; ++i) own[i].close(ub);
       partners.template enter<false>(own, part.tw, lane, cur, st);
       if (t0 >= S.t) return;
       keep(c, st);
@@ -752,6 +762,8 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
 #pragma unroll
         for (int i = 0; i < E; ++i) own[i].template backward<MASK>(g[i], Weights::of_step(ms[j][i % GE]), bit_mask(ub, j));
       }
+#pragma unroll
+      for (int i = 0; i < E; ++i) own[i].close(ub);
       partners.template enter<true>(own, part.tw, lane, v, b);
       if (t0 >= S.t) continue;
     } else {
@@ -760,11 +772,11 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
     }
     float slope[KEEP][GE];
     asm volatile("" : "+v"(ub), "+v"(vb));  // the mask words anew: 32 registers of them across the two loops cost more
-    auto down = [&](auto whole) __attribute__((always_inline)) {
-      constexpr bool WHOLE = decltype(whole)::value;
+    auto down = [&](auto usual) __attribute__((always_inline)) {
+      constexpr bool USUAL = decltype(usual)::value;
 #pragma unroll
       for (int j = KEEP - 1; j >= 0; --j) {
-        if (!WHOLE && t0 + j >= S.t) continue;
+        if (!USUAL && t0 + j >= S.t) continue;
         float g[E], x[E];
         Values<V, E>::open(rd[j], g);
 #pragma unroll
@@ -781,16 +793,17 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
         if (MASK)
 #pragma unroll
           for (int i = 0; i < GE; ++i) slope[j][i] = masked_value(slope[j][i], bit_mask(ub & vb, j));
-        if (dx) out.store_one(t0 + j, x);
-        if (dgate && S.share == 1) single.store_one(t0 + j, slope[j]);
+        if (USUAL || dx) out.store_one(t0 + j, x);
+        if (GE == 2 && (USUAL || dgate)) single.store_one(t0 + j, slope[j]);
       }
     };
     if (at.on) {
-      if (t0 + KEEP <= S.t)
-        down(std::true_type());
+      if (t0 + KEEP <= S.t && dx && (GE == 1 || dgate))
+        down(std::true_type());             // without a question a step
       else
         down(std::false_type());
     }
+    if (E == 1 && dgate && S.share == 1) single.store(t0, S.t, at.on, slope);
     if constexpr (GE == 1)
       if (dgate && S.share > 1) sum_gates(A, sums[threadIdx.x >> 6], slope, at.on, S.t - t0, (int64_t)t0 * S.dgate_t, (int64_t)t0 * S.rows * S.groups * slots);
     if (dh0 && at.on && t0 == 0)

@@ -76,8 +76,12 @@ def _state(name: str, s, shape, dev) -> Optional[torch.Tensor]:
     return s.contiguous()
 
 
-def _like(x: torch.Tensor, feat) -> torch.Tensor:
-    """An uninitialised tensor of x's first two dimensions and `feat` in x's memory order (rows outermost or time outermost)."""
+def _like(x: torch.Tensor, feat=None) -> torch.Tensor:
+    """An uninitialised tensor of x's first two dimensions and `feat` (None: x's) in x's memory order (rows or time outermost)."""
+    if feat is None:
+        feat = x.shape[2:]
+        if x.is_contiguous():
+            return torch.empty_like(x)
     T, R = x.shape[:2]
     if x.stride(1) > x.stride(0) and T > 1 and R > 1:
         return torch.empty((R, T) + tuple(feat), dtype=x.dtype, device=x.device).transpose(0, 1)
@@ -104,12 +108,11 @@ def _workspace(nbytes: int, dev):
 def _scan(x, gate, h0, use, valid, groups: int, share: int, keep: bool):
     """-> (h, h_last, kept).  Arguments are checked by the caller."""
     dev = x.device
-    feat = x.shape[2:]
     T, R = x.shape[:2]
     n = groups * share
     xs, gs = _rows_of(x, n), _rows_of(gate, groups)
-    h = _like(x, feat)
-    last = torch.empty(x.shape[1:], dtype=torch.float32, device=dev)
+    h = _like(x)
+    last = torch.empty(x.shape[1:], dtype=torch.float32, device=dev) if h0 is None else torch.empty_like(h0)
     kept = torch.empty((-(-T // nat.GATED_KEEP), R * n), dtype=torch.float32, device=dev) if keep else None
     if R * n:
         shape = _shape(xs, gs, use, valid, groups, share, h)
@@ -126,8 +129,8 @@ def _backward(x, gate, kept, dh, dh_last, use, valid, groups: int, share: int, n
     dev = x.device
     R, n = x.shape[1], groups * share
     xs, gs, ds = _rows_of(x, n), _rows_of(gate, groups), _rows_of(dh, n)
-    dx = _like(x, x.shape[2:]) if need[0] else None
-    dgate = _like(x, gate.shape[2:]) if need[1] else None
+    dx = _like(x) if need[0] else None
+    dgate = None if not need[1] else torch.empty_like(gate) if gate.is_contiguous() and x.is_contiguous() else _like(x, gate.shape[2:])
     dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=dev) if need[2] else None
     if R * n and any(need):
         shape = _shape(xs, gs, use, valid, groups, share, xs if dx is None else dx)
@@ -240,15 +243,15 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
         raise ValueError(f"gated_step: {B} samples and {rows} rows without memory_idx")
     use, ok = _mask("use_memory", use_memory, (B,), dev), _mask("valid", valid, (B,), dev)
     use, ok = None if use is None else use.contiguous(), None if ok is None else ok.contiguous()
+    x, gate = x.contiguous(), gate.contiguous()
     if out is None:
-        out = torch.empty((B,) + feat, dtype=x.dtype, device=dev)
+        out = torch.empty_like(x)
     elif tuple(out.shape) != (B,) + feat or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"gated_step: out is a contiguous {x.dtype} tensor {(B,) + feat} on {dev}")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or status.device != dev):
         raise ValueError(f"gated_step: status is int32[1] on {dev}")
     if out.numel() == 0:
         return out
-    x, gate = x.contiguous(), gate.contiguous()
     L = nat.lib()
     with nat.on_device(dev):
         ws = _workspace(L.umt_gated_step_workspace_bytes(B, rows) if memory_idx is not None else 0, dev)

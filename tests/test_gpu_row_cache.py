@@ -41,7 +41,8 @@ def status():
 
 
 @pytest.mark.parametrize("kind,rows,n", [("tracker", 2, 2), ("tracker", 64, 13), ("odd", 33, 33), ("odd", 1, 1), ("long", 9, 7),
-                                         ("tracker", 3000, 2500), ("odd", 20000, 19999), ("tracker", 40, 200)])
+                                         ("tracker", 3000, 2500), ("odd", 20000, 19999), ("tracker", 40, 200),
+                                         ("odd", 200000, 3000), ("odd", 300000, 900), ("long", 60, 50)])
 @pytest.mark.parametrize("how", ["any", "permutation", "apart"])
 def test_copy_reads_before_it_writes(kind, rows, n, how):
     bufs = buffers(kind, rows)
@@ -132,7 +133,7 @@ def test_rows_outside_the_cache_are_neither_freed_nor_forked():
 
 @pytest.mark.parametrize("kind,rows,dead", [("tracker", 1, 0), ("tracker", 1, 1), ("tracker", 2, 1), ("tracker", 64, 20), ("odd", 1024, 512),
                                             ("odd", 1025, 1000), ("tracker", 4100, 1300), ("long", 11, 5), ("odd", 9000, 0), ("odd", 9000, 9000),
-                                            ("odd", 70001, 23456)])
+                                            ("odd", 70001, 23456), ("odd", 131072, 40000), ("odd", 140001, 70000), ("odd", 131073, 131073)])
 def test_compact(kind, rows, dead):
     bufs = buffers(kind, rows)
     want = host(bufs)

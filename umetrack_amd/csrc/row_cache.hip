@@ -8,6 +8,7 @@
 // Ranks come from per-block counts that every block adds up for itself, in one workgroup where the cache is small.
 #include "umt_internal.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace umt {
@@ -210,6 +211,73 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
   }
 }
 
+// More: two launches.  Every workgroup of the first marks all targets in a bit map of the cache in its LDS (64 KB of row
+// numbers from L2 for 8191 copies, where three launches over tables in HBM took 8 us), decides on copies of its own and brings
+// those sources to safety that the call overwrites.  plan[i]: what the second launch does.
+enum { COPY_NOT = 0, COPY_ROW = 1, COPY_STAGED = 2 };
+constexpr int MAP_ROWS = 1 << 18;          // 32 KB of bits
+constexpr int MAP_COPIES = 1 << 14, MAP_GROUPS = 128, MAP_EACH = MAP_COPIES / MAP_GROUPS;
+__global__ __launch_bounds__(ONE) void copy_plan_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                        int rows, uint8_t* __restrict__ plan, char* __restrict__ stage,
+                                                        int32_t* __restrict__ status) {
+  extern __shared__ uint32_t map[];
+  __shared__ int twice, n_todo;             // some row is written by more than one copy; sources to bring to safety
+  __shared__ uint16_t todo[MAP_EACH];
+  __shared__ uint8_t late[MAP_EACH];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), pieces = B.piece0[B.n_long];
+  for (int i = tid; i < (rows + 31) / 32; i += ONE) map[i] = 0;
+  if (tid == 0) twice = n_todo = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += ONE) {
+    const int64_t d = dst[i];              // of a copy that will not be made too: a source too many brought to safety, no more
+    if (!in_cache(d, rows)) continue;
+    const uint32_t bit = 1u << (d & 31);
+    if (atomicOr(map + (d >> 5), bit) & bit) twice = 1;
+  }
+  __syncthreads();
+  const int each = (n + gridDim.x - 1) / gridDim.x, i0 = min(n, (int)blockIdx.x * each), i1 = min(n, i0 + each);
+  if (twice) {                              // of several writes to one row the highest i counts
+    for (int i = i0 + wv; i < i1; i += ONE / 64) {
+      const int64_t d = uniform(dst[i]);
+      bool last = true;
+      for (int o = i + 1 + lane; o < n; o += 64) last &= dst[o] != d || !in_cache(src[o], rows);
+      const bool counts = __all(last);
+      if (lane == 0) late[i - i0] = !counts;
+    }
+    __syncthreads();
+  }
+  for (int i = i0 + tid; i < i1; i += ONE) {
+    const int64_t s = src[i], d = dst[i];
+    int what = COPY_NOT;
+    if (!in_cache(s, rows) || !in_cache(d, rows)) {
+      if (status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
+    } else if (s != d && !(twice && late[i - i0])) {
+      what = map[s >> 5] >> (s & 31) & 1 ? COPY_STAGED : COPY_ROW;
+    }
+    plan[i] = (uint8_t)what;
+    if (what == COPY_STAGED) todo[atomicAdd(&n_todo, 1)] = (uint16_t)i;      // any order: each has its own place
+  }
+  __syncthreads();
+  for (int it = wv; it < n_todo * pieces; it += ONE / 64) {
+    const int k = it / pieces, i = todo[k];
+    move_piece(B, it - k * pieces, Staged<Global>{(Global)(stage + i * B.staged_bytes)}, Cached{uniform(src[i])}, lane);
+  }
+}
+__global__ __launch_bounds__(RT) void copy_planned_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
+                                                          const uint8_t* __restrict__ plan, char* stage) {
+  const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long];
+  const unsigned item = blockIdx.x * (RT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = (int)(item / (unsigned)pieces), p = (int)(item - (unsigned)i * (unsigned)pieces);
+  if (i >= n) return;
+  const int what = plan[i];
+  const int64_t s = src[i], d = dst[i];
+  if (what == COPY_STAGED)
+    move_piece(B, p, Cached{uniform(d)}, Staged<Global>{(Global)(stage + i * B.staged_bytes)}, lane);
+  else if (what == COPY_ROW)
+    move_piece(B, p, Cached{uniform(d)}, Cached{uniform(s)}, lane);
+}
+
+// Any number: five launches, with a table of a word a row.
 // last[r] = highest i that writes row r, -1 where none does; only rows that the call names are touched
 __global__ __launch_bounds__(RT) void copy_clear_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
                                                         int rows, int32_t* __restrict__ last, int32_t* __restrict__ todo,
@@ -237,33 +305,6 @@ __global__ __launch_bounds__(RT) void copy_list_kernel(const int64_t* __restrict
                                                        const int32_t* __restrict__ last, int32_t* __restrict__ todo) {
   const int i = blockIdx.x * RT + threadIdx.x;
   if (i < n && copies(last, src[i], dst[i], i, rows) && last[src[i]] >= 0) todo[4 + atomicAdd(todo, 1)] = i;
-}
-// the three of them in one workgroup, for a copy a thread (a CU takes 50 us over the scattered words of 8191)
-constexpr int INDEX_ONE = ONE;
-__global__ __launch_bounds__(ONE) void copy_index_kernel(const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n, int rows,
-                                                         int32_t* __restrict__ last, int32_t* __restrict__ todo, int32_t* __restrict__ status) {
-  const int tid = threadIdx.x;
-  if (tid == 0) todo[0] = 0;
-  for (int i = tid; i < n; i += ONE) {
-    if (in_cache(src[i], rows) && in_cache(dst[i], rows)) {
-      last[src[i]] = -1;
-      last[dst[i]] = -1;
-    } else if (status) {
-      atomicOr(status, (int)UMT_STATUS_BAD_ROW);
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < n; i += ONE)
-    if (in_cache(src[i], rows) && in_cache(dst[i], rows)) atomicMax(last + dst[i], i);
-  __threadfence();
-  __syncthreads();
-  for (int i = tid; i < n; i += ONE) {
-    const int64_t s = src[i], d = dst[i];
-    if (!in_cache(s, rows) || !in_cache(d, rows) || s == d) continue;
-    const int ls = __hip_atomic_load(last + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int ld = __hip_atomic_load(last + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (ld == i && ls >= 0) todo[4 + atomicAdd(todo, 1)] = i;
-  }
 }
 __global__ __launch_bounds__(RT) void copy_stage_kernel(RowBuffers B, const int64_t* __restrict__ src, const int32_t* __restrict__ todo,
                                                         char* __restrict__ stage) {
@@ -397,7 +438,8 @@ __global__ __launch_bounds__(RT) void free_rows_kernel(uint8_t* __restrict__ liv
 
 // ---------------------------------------------------------------- compact
 // lists: [0] = live rows c, [1] = moves, from [4] on the holes below c and behind them the live rows from c on, in order.
-// counts may be null in a grid of one block.  live is read only: the launch that moves writes it.
+// counts may be null in a grid of one block.  (Workgroups that count all 65536 flags for themselves take 17 us, these two
+// launches 10.)  live is read only: the launch that moves writes it.
 __global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __restrict__ live, int rows, const int32_t* __restrict__ counts,
                                                            int64_t* __restrict__ now, int32_t* __restrict__ lists) {
   __shared__ int lds[ONE / 64];
@@ -513,12 +555,15 @@ static int need_workspace(const char* what, const void* ws, int64_t have, int64_
 using namespace umt;
 
 static bool few_rows(const RowBuffers& B, int n) { return n <= FEW && n * B.staged_bytes <= SMALL_BYTES - 16 * FEW; }
+static bool planned(int rows, int n) { return rows <= MAP_ROWS && n <= MAP_COPIES; }
 static int blocks_of(int64_t n) { return (int)((n + BLOCK - 1) / BLOCK); }
 
 extern "C" int64_t umt_rows_copy_workspace_bytes(const umt_row_buffer* buffers, int n_buffers, int rows, int n) {
   RowBuffers B;
   if (n < 0 || row_buffers("rows copy", buffers, n_buffers, rows, &B) != 0) return -1;
-  return n == 0 || rows == 0 || few_rows(B, n) ? 0 : round_up64((int64_t)rows * 4, 16) + round_up64(16 + (int64_t)n * 4, 16) + n * B.staged_bytes;
+  if (n == 0 || rows == 0 || few_rows(B, n)) return 0;
+  const int64_t index = planned(rows, n) ? round_up64(n, 16) : round_up64((int64_t)rows * 4, 16) + round_up64(16 + (int64_t)n * 4, 16);
+  return index + n * B.staged_bytes;
 }
 
 extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int rows, const int64_t* src, const int64_t* dst, int n,
@@ -536,17 +581,22 @@ extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int r
   UMT_TRY(need_workspace("rows copy", workspace, workspace_bytes, umt_rows_copy_workspace_bytes(buffers, n_buffers, rows, n)));
   unsigned grid = 0;
   UMT_TRY(move_grid("rows copy", B, n, &grid));
+  if (planned(rows, n)) {
+    uint8_t* plan = (uint8_t*)workspace;
+    char* stage = (char*)workspace + round_up64(n, 16);
+    const int groups = std::min((n + ONE / 64 - 1) / (ONE / 64), MAP_GROUPS);       // at most MAP_EACH copies each
+    hipLaunchKernelGGL(copy_plan_kernel, dim3(groups), dim3(ONE), (size_t)((rows + 31) / 32) * 4, s, B, src, dst, n, rows, plan, stage, status);
+    hipLaunchKernelGGL(copy_planned_kernel, dim3(grid), dim3(RT), 0, s, B, src, dst, n, plan, stage);
+    UMT_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
   int32_t* last = (int32_t*)workspace;
   int32_t* todo = (int32_t*)((char*)workspace + round_up64((int64_t)rows * 4, 16));
   char* stage = (char*)todo + round_up64(16 + (int64_t)n * 4, 16);
   const dim3 per_pair((n + RT - 1) / RT);
-  if (n <= INDEX_ONE) {
-    hipLaunchKernelGGL(copy_index_kernel, dim3(1), dim3(ONE), 0, s, src, dst, n, rows, last, todo, status);
-  } else {
-    hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo, status);
-    hipLaunchKernelGGL(copy_claim_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last);
-    hipLaunchKernelGGL(copy_list_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo);
-  }
+  hipLaunchKernelGGL(copy_clear_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo, status);
+  hipLaunchKernelGGL(copy_claim_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last);
+  hipLaunchKernelGGL(copy_list_kernel, per_pair, dim3(RT), 0, s, src, dst, n, rows, last, todo);
   hipLaunchKernelGGL(copy_stage_kernel, dim3(grid < 2048 ? grid : 2048), dim3(RT), 0, s, B, src, todo, stage);
   hipLaunchKernelGGL(copy_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, dst, n, rows, last, stage);
   UMT_CHECK_HIP(hipGetLastError());
@@ -612,8 +662,9 @@ extern "C" int umt_rows_compact(const umt_row_buffer* buffers, int n_buffers, in
   UMT_TRY(move_grid("rows compact", B, rows / 2 + 1, &grid));              // at most half of the rows move
   int32_t *lists = (int32_t*)workspace, *counts = lists + 4 + 2 * (int64_t)rows;
   const int blocks = blocks_of(rows);
-  if (blocks > 1) hipLaunchKernelGGL(count_rows_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counts);
-  hipLaunchKernelGGL(compact_list_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, blocks > 1 ? counts : (int32_t*)nullptr, now, lists);
+  const bool counted = blocks > 1;
+  if (counted) hipLaunchKernelGGL(count_rows_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counts);
+  hipLaunchKernelGGL(compact_list_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counted ? counts : (int32_t*)nullptr, now, lists);
   hipLaunchKernelGGL(compact_move_kernel, dim3(grid < 4096 ? grid : 4096), dim3(RT), 0, s, B, lists, rows, live, now, count);
   UMT_CHECK_HIP(hipGetLastError());
   return 0;

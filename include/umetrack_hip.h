@@ -290,7 +290,7 @@ int umt_metric_partials_static(const float* gt, const float* pred, const uint8_t
  *
  * features = groups * share: `share` consecutive features use one gate (a landmark's 3 coordinates, a hand's 63, 1).
  * Element (t, row, feature) of x lies at t * x_t + row * x_row + feature, and so on: strides in elements, not negative,
- * 0 allowed for what is read.  h and dx share out_t / out_row.  What is written must not overlap itself.
+ * 0 allowed for what is read.  h and dx share out_t / out_row.  What is written overlaps neither itself nor what is read.
  * h0, h_last, dh0, dh_last: dev f32 (rows, features), contiguous.                                                  */
 enum { UMT_VALUES_F32 = 0, UMT_VALUES_BF16 = 1 };
 typedef struct {
@@ -319,7 +319,8 @@ int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const v
  * NULL: sample b is row b.  x (batch, features) and gate (batch, groups) are contiguous; use_memory and valid (batch) or
  * NULL.  Duplicates in memory_idx all read the same previous row and the highest batch index writes it, as
  * umt_temporal_step; an index outside the cache runs without memory, writes no row and raises
- * UMT_STATUS_BAD_MEMORY_IDX in *status (dev int32[1] or NULL).  Rows that no sample names are left as they are.     */
+ * UMT_STATUS_BAD_MEMORY_IDX in *status (dev int32[1] or NULL).  Rows that no sample names are left as they are.
+ * out may be x (and gate, where share is 1) itself; nothing else overlaps.                                          */
 int64_t umt_gated_step_workspace_bytes(int batch, int cache_rows);
 int umt_gated_step(int dtype, const void* x, const void* gate, const int64_t* memory_idx, const uint8_t* use_memory,
                    const uint8_t* valid, int batch, int groups, int share, float* state, int cache_rows, void* out,
@@ -328,7 +329,7 @@ int umt_gated_step(int dtype, const void* x, const void* gate, const int64_t* me
 /* ---- rows of state caches: the temporal memory of a model handle (umt_model_memory_buffers) and any caches of the
  * caller that hold one row per hand track (umt_gated_step's state, ...).  The buffers of one call have `rows` rows each
  * and move together.  buffers is a host array of n_buffers <= UMT_ROW_BUFFERS_MAX entries whose data is dev memory;
- * they must not overlap.  Row numbers are dev int64; status is dev int32[1] or NULL (UMT_STATUS_BAD_ROW,
+ * they must not overlap each other, the row numbers or live.  Row numbers are dev int64; status is dev int32[1] or NULL (UMT_STATUS_BAD_ROW,
  * UMT_STATUS_NO_FREE_ROW are OR-ed in).  live: dev uint8 (rows), non-zero = in use.                                */
 #define UMT_ROW_BUFFERS_MAX 8
 typedef struct {

@@ -473,3 +473,28 @@ def test_steps_follow_the_scan():
     h, last = _gf().gated_scan(x, gate, h0, use, valid)
     eh, _, _ = slack(x, gate, h0, valid, T)
     assert float((outs - h).abs().max()) <= 2 * eh and float((state - last).abs().max()) <= 2 * eh
+
+
+def test_gates_of_no_features_have_no_gradient():
+    x, g = torch.zeros(3, 2, 21, 0, device="cuda", requires_grad=True), torch.randn(3, 2, 21, device="cuda", requires_grad=True)
+    torch.full((3, 2, 21), float("nan"), device="cuda")          # what the allocator hands out next
+    h, last = _gf().gated_scan(x, g)
+    (h.sum() + last.sum()).backward()
+    assert h.shape == x.shape and x.grad.shape == x.shape and torch.equal(g.grad, torch.zeros_like(g))
+
+
+@pytest.mark.parametrize("share", [1, 3])
+def test_a_step_in_place(share):
+    gen = torch.Generator().manual_seed(5)
+    x, gate, state = torch.randn(40, 7 * share, generator=gen), torch.randn(40, 7, generator=gen), torch.randn(30, 7 * share, generator=gen)
+    idx = torch.randint(-2, 30, (40,), generator=gen)
+    x = x.view(40, 7, share).to("cuda")
+    a, b = state.view(30, 7, share).to("cuda"), state.view(30, 7, share).to("cuda").clone()
+    want = _gf().gated_step(x, gate.to("cuda"), a, memory_idx=idx.to("cuda"))
+    y = x.clone()
+    assert _gf().gated_step(y, gate.to("cuda"), b, memory_idx=idx.to("cuda"), out=y) is y
+    assert torch.equal(y, want) and torch.equal(a, b)
+    few = dict(gate=gate[:10].to("cuda"), memory_idx=idx[:10].to("cuda"))
+    for kw in (dict(x=x[:10], out=b[5:15]), dict(x=b[5:15], out=torch.empty_like(b[5:15])), dict(x=y[:10], out=y[1:11])):
+        with pytest.raises(nat.UmtError, match="overlap"):
+            _gf().gated_step(state=b, **few, **kw)

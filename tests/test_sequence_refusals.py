@@ -66,6 +66,39 @@ def test_step_arguments():
     assert step(batch=0, x=None, gate=None, out=None) == 0
 
 
+def test_strides_that_lead_out_of_memory():
+    L = nat.lib()
+    for bad in (dict(x_t=1 << 60), dict(gate_row=1 << 60), dict(out_t=1 << 50), dict(dh_t=(1 << 47) + 1), dict(rows=1 << 30, groups=1, share=3)):
+        s = shape(**{**dict(t=4), **bad})
+        assert L.umt_gated_scan_backward(s, P, P, None, None, P, P, None, P, P, None, P, 1 << 62, None) == 1, bad
+    # an axis of one step or row has no stride
+    assert L.umt_gated_scan(shape(t=1, x_t=1 << 60, gate_t=1 << 60, out_t=1 << 60), P, P, None, None, None, None, None, None, None, 0, None) == 1
+    assert b"null pointer" in L.umt_last_error()
+
+
+def test_step_places_and_sizes():
+    L = nat.lib()
+    x, gate, state, out = 1 << 20, 2 << 20, 3 << 20, 4 << 20          # 4 samples of 2 x 3 features, 5 rows
+
+    def step(x=x, gate=gate, state=state, out=out, batch=4, rows=5, share=3, dtype=0, ws=P, size=1 << 40):
+        return L.umt_gated_step(dtype, x, gate, P, None, None, batch, 2, share, state, rows, out, None, ws, size, None)
+    for kw in (dict(out=x + 4), dict(out=x + 4 * 24 - 4), dict(out=x - 4 * 24 + 4), dict(out=gate), dict(out=gate + 4 * 8 - 4), dict(state=x),
+               dict(state=x - 4 * 30 + 4), dict(state=out + 4 * 24 - 4), dict(state=gate), dict(out=gate + 4, share=1), dict(out=state + 4 * 29)):
+        assert step(**kw) == 1 and b"overlap" in L.umt_last_error(), kw
+    for batch, share in (((1 << 26), 1), ((1 << 31) - 1, 1), (1 << 20, 1 << 13)):
+        assert step(batch=batch, share=share) == 1 and b"samples of" in L.umt_last_error()
+
+
+def test_row_calls_too_large():
+    L = nat.lib()
+    thin, n = rows_buf((1 << 40, 4))
+    big = (1 << 31) - 1
+    assert L.umt_rows_copy(thin, n, 8, P, P, big, None, P, 1 << 60, None) == 1 and L.umt_rows_fork(thin, n, 8, P, P, big, P, None, P, 1 << 60, None) == 1
+    long, n = rows_buf((1 << 40, 1 << 30))
+    assert L.umt_rows_copy(long, n, 8, P, P, 1 << 9, None, P, 1 << 60, None) == 1 and b"pieces" in L.umt_last_error()
+    assert L.umt_rows_copy_workspace_bytes(long, n, big, 1) == -1                     # more than any memory holds
+
+
 def rows_buf(*entries):
     return (nat.RowBuffer * max(1, len(entries)))(*[nat.RowBuffer(p, n) for p, n in entries]), len(entries)
 
@@ -115,6 +148,16 @@ def test_groups_of_gates():
             split(feat, gate)
     with pytest.raises(ValueError, match="differ"):
         gf._split("t", torch.empty(2, 3, 4), torch.empty(2, 4), 2)
+
+
+def test_sizes_past_31_bits():
+    one = torch.empty(1, 1, 1)
+    for x, gate in ((one.expand(1 << 31, 1, 1), one.expand(1 << 31, 1, 1)), (one.expand(1, 1 << 32, 1), one[:, :, 0].expand(1, 1 << 32)),
+                    (one.expand(1, 1, 1 << 31), one[:, :, 0]), (one.expand(1, 1, 1 << 33), one.expand(1, 1, 1 << 33))):
+        with pytest.raises(ValueError):
+            gf._split("t", x, gate, 2)
+    with pytest.raises(ValueError):
+        rc._ids("t", torch.zeros(1, dtype=torch.int64).expand(1 << 31), torch.device("cpu"))
 
 
 def test_types_and_devices():

@@ -850,7 +850,7 @@ struct StepArgs {
 
 // STEP_SEG features of sample b, from f0 on; prev: the row's values.  -> the new state
 template <typename V>
-__device__ __forceinline__ void step_values(const StepArgs& A, const V* __restrict__ x, const V* __restrict__ gate, V* out, int b, int f0,
+__device__ __forceinline__ void step_values(const StepArgs& A, const V* x, const V* gate, V* out, int b, int f0,
                                             bool has_row, const float (&prev)[STEP_SEG / 64], float (&h)[STEP_SEG / 64]) {
   const int lane = threadIdx.x & 63, F = A.groups * A.share;
   const unsigned use = has_row && (!A.use || A.use[b]) ? ~0u : 0u, valid = !A.valid || A.valid[b] ? ~0u : 0u;
@@ -872,7 +872,7 @@ __device__ __forceinline__ void step_values(const StepArgs& A, const V* __restri
 // it reads the row once, computes the other samples' outputs from that, and writes the row last.  Who that is a small batch
 // finds by looking through memory_idx (64 a load, from L2), a large one in the owner table of two launches before.
 template <typename V>
-__global__ __launch_bounds__(GT) void gated_step_kernel(StepArgs A, const V* __restrict__ x, const V* __restrict__ gate, V* out) {
+__global__ __launch_bounds__(GT) void gated_step_kernel(StepArgs A, const V* x, const V* gate, V* out) {
   constexpr int K = STEP_SEG / 64;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * (GT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -918,13 +918,17 @@ static int check_shape(const umt_gated_shape* S, bool backward) {
   UMT_REQUIRE(S->t >= 0 && S->rows >= 0 && S->groups > 0 && S->share > 0, UMT_ERR_INVALID,
               "gated scan: t=%d rows=%d groups=%d share=%d", S->t, S->rows, S->groups, S->share);
   UMT_REQUIRE((int64_t)S->groups * S->share <= (1 << 24), UMT_ERR_INVALID, "gated scan: %d x %d features in a row", S->groups, S->share);
-  UMT_REQUIRE((int64_t)S->rows * S->groups * S->share <= (1LL << 36), UMT_ERR_INVALID, "gated scan: %d rows of %d x %d features",
+  // a launch counts its threads in 32 bits, and no lane owns less than a feature
+  UMT_REQUIRE((int64_t)S->rows * S->groups * S->share <= (1LL << 31), UMT_ERR_INVALID, "gated scan: %d rows of %d x %d features",
               S->rows, S->groups, S->share);
   UMT_REQUIRE(S->t <= (1 << 30) && (int64_t)S->rows * S->groups <= (1LL << 38) / (S->t > 0 ? S->t : 1), UMT_ERR_INVALID,
               "gated scan: %d steps of %d x %d gates", S->t, S->rows, S->groups);
   const int64_t st[] = {S->x_t, S->x_row, S->gate_t, S->gate_row, S->out_t, S->out_row, S->use_t, S->use_row, S->valid_t,
                         S->valid_row, S->dh_t, S->dh_row, S->dgate_t, S->dgate_row};
-  for (int i = 0; i < (backward ? 14 : 10); ++i) UMT_REQUIRE(st[i] >= 0, UMT_ERR_INVALID, "gated scan: negative stride %lld", (long long)st[i]);
+  for (int i = 0; i < (backward ? 14 : 10); ++i) {          // t strides and row strides in turn; no array reaches over 2^48 values
+    const int n = i % 2 ? S->rows : S->t;
+    UMT_REQUIRE(st[i] >= 0 && (n <= 1 || st[i] <= (1LL << 48) / n), UMT_ERR_INVALID, "gated scan: stride %lld over %d", (long long)st[i], n);
+  }
   return 0;
 }
 
@@ -981,7 +985,7 @@ static int gate_slots(const umt_gated_shape& S, int per) { return per % S.share 
 static int64_t part_floats(const umt_gated_shape& S, int per) { return (int64_t)S.t * S.rows * S.groups * gate_slots(S, per); }
 
 // Whether lanes can hold two values: they, and the gates where every feature has its own, lie in pairs at even places.
-// 4-byte loads in the place of 2-byte ones: scan_features (512 x 512 x 648) 267 -> %PAIR% us.
+// 4-byte loads in the place of 2-byte ones: 512 steps of 512 rows of 648 features 267 -> 251 us.
 static bool pairable(const umt_gated_shape& S) {
   return S.dtype == UMT_VALUES_BF16 && S.groups * S.share % 2 == 0 && (S.share == 1 || S.share % 2 == 0);
 }
@@ -1072,6 +1076,10 @@ static int by_variant(const umt_gated_shape& S, bool two, bool masks, Call call)
   if (S.dtype == UMT_VALUES_F32) return typed(0.f, Count<1>(), Count<1>());
   if (!two) return typed((__bf16)0.f, Count<1>(), Count<1>());
   return S.share == 1 ? typed((__bf16)0.f, Count<2>(), Count<2>()) : typed((__bf16)0.f, Count<2>(), Count<1>());
+}
+
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  return na > 0 && nb > 0 && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
 }
 
 template <typename V>
@@ -1170,7 +1178,14 @@ extern "C" int umt_gated_step(int dtype, const void* x, const void* gate, const 
   UMT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), UMT_ERR_WORKSPACE, "gated step: workspace %lld < %lld bytes",
               (long long)workspace_bytes, (long long)need);
   const int F = groups * share, segs = (F + STEP_SEG - 1) / STEP_SEG;
-  UMT_REQUIRE((int64_t)batch * segs <= (1LL << 32), UMT_ERR_INVALID, "gated step: %d samples of %d features", batch, F);
+  UMT_REQUIRE((int64_t)batch * segs < (1LL << 26) - GT, UMT_ERR_INVALID, "gated step: %d samples of %d features", batch, F);      // waves
+  // a row may be written while another sample's values are read; an output only by the wave that has read its place
+  const int64_t size = dtype == UMT_VALUES_BF16 ? 2 : 4, values = (int64_t)batch * F * size, gates = (int64_t)batch * groups * size;
+  const int64_t rows = (int64_t)cache_rows * F * (int64_t)sizeof(float);
+  UMT_REQUIRE(!overlap(state, rows, x, values) && !overlap(state, rows, gate, gates) && !overlap(state, rows, out, values), UMT_ERR_INVALID,
+              "gated step: state overlaps x, gate or out");
+  UMT_REQUIRE((out == x || !overlap(out, values, x, values)) && ((out == gate && share == 1) || !overlap(out, values, gate, gates)),
+              UMT_ERR_INVALID, "gated step: out overlaps a part of x or gate");
   hipStream_t s = (hipStream_t)stream;
   int32_t *owner = need ? (int32_t*)workspace : nullptr, *named = need ? owner + cache_rows : nullptr;
   if (need) {

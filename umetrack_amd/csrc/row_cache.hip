@@ -427,7 +427,7 @@ __global__ __launch_bounds__(RT) void fork_move_kernel(RowBuffers B, const int64
 // ---------------------------------------------------------------- free
 __global__ __launch_bounds__(RT) void free_rows_kernel(uint8_t* __restrict__ live, int rows, const int64_t* __restrict__ row_ids,
                                                        int n, int32_t* __restrict__ status) {
-  const int i = blockIdx.x * RT + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * RT + threadIdx.x;
   if (i >= n) return;
   const int64_t r = row_ids[i];
   if (in_cache(r, rows))
@@ -502,8 +502,8 @@ static int row_buffers(const char* what, const umt_row_buffer* buffers, int n, i
   B->n = n;
   for (int k = 0; k < n; ++k) {
     const umt_row_buffer& b = buffers[k];
-    UMT_REQUIRE((b.data || rows == 0) && b.row_bytes > 0 && b.row_bytes <= (1LL << 40), UMT_ERR_INVALID,
-                "%s: buffer %d is null or its rows have %lld bytes", what, k, (long long)b.row_bytes);
+    UMT_REQUIRE((b.data || rows == 0) && b.row_bytes > 0 && b.row_bytes <= (1LL << 40) / (rows > 0 ? rows : 1), UMT_ERR_INVALID,
+                "%s: buffer %d is null or has %d rows of %lld bytes", what, k, rows, (long long)b.row_bytes);
     const uint64_t lo = (uint64_t)b.data;
     for (int j = 0; j < k && rows > 0; ++j) {
       const uint64_t o = (uint64_t)buffers[j].data;
@@ -537,11 +537,13 @@ static int row_buffers(const char* what, const umt_row_buffer* buffers, int n, i
   return 0;
 }
 
-// workgroups of a move of n rows, a wave per piece
-static int move_grid(const char* what, const RowBuffers& B, int64_t n, unsigned* grid) {
-  const int64_t wg = (n * B.piece0[B.n_long] + RT / 64 - 1) / (RT / 64);
-  UMT_REQUIRE(n * B.piece0[B.n_long] < (1LL << 31), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n, B.piece0[B.n_long]);
-  *grid = (unsigned)wg;
+// Workgroups of a move of n rows, a wave per piece.  A launch counts its threads in 32 bits; where a launch of `most`
+// workgroups goes through the pieces in rounds, the pieces are counted in 31.
+static int move_grid(const char* what, const RowBuffers& B, int64_t n, int most, unsigned* grid) {
+  const int64_t pieces = n * B.piece0[B.n_long], wg = (pieces + RT / 64 - 1) / (RT / 64);
+  UMT_REQUIRE(pieces < (most ? 1LL << 31 : (1LL << 26) - RT), UMT_ERR_INVALID, "%s: %lld rows of %d pieces", what, (long long)n,
+              B.piece0[B.n_long]);
+  *grid = (unsigned)(most && wg > most ? most : wg);
   return 0;
 }
 
@@ -580,7 +582,7 @@ extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int r
   }
   UMT_TRY(need_workspace("rows copy", workspace, workspace_bytes, umt_rows_copy_workspace_bytes(buffers, n_buffers, rows, n)));
   unsigned grid = 0;
-  UMT_TRY(move_grid("rows copy", B, n, &grid));
+  UMT_TRY(move_grid("rows copy", B, n, 0, &grid));
   if (planned(rows, n)) {
     uint8_t* plan = (uint8_t*)workspace;
     char* stage = (char*)workspace + round_up64(n, 16);
@@ -618,7 +620,7 @@ extern "C" int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int r
   if (n == 0) return 0;
   UMT_TRY(need_workspace("rows fork", workspace, workspace_bytes, umt_rows_fork_workspace_bytes(rows, n)));
   unsigned grid = 0;
-  UMT_TRY(move_grid("rows fork", B, n, &grid));
+  UMT_TRY(move_grid("rows fork", B, n, 0, &grid));
   hipStream_t s = (hipStream_t)stream;
   int32_t *order = (int32_t*)workspace, *counts = order + n;
   if (one_group(rows, n)) {
@@ -639,7 +641,7 @@ extern "C" int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int r
 extern "C" int umt_rows_free(uint8_t* live, int rows, const int64_t* row_ids, int n, int32_t* status, void* stream) {
   UMT_REQUIRE(n >= 0 && rows >= 0 && (n == 0 || row_ids) && (live || rows == 0), UMT_ERR_INVALID, "rows free: n=%d rows=%d or null pointer", n, rows);
   if (n == 0) return 0;
-  hipLaunchKernelGGL(free_rows_kernel, dim3((n + RT - 1) / RT), dim3(RT), 0, (hipStream_t)stream, live, rows, row_ids, n, status);
+  hipLaunchKernelGGL(free_rows_kernel, dim3((unsigned)(((int64_t)n + RT - 1) / RT)), dim3(RT), 0, (hipStream_t)stream, live, rows, row_ids, n, status);
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }
@@ -659,13 +661,13 @@ extern "C" int umt_rows_compact(const umt_row_buffer* buffers, int n_buffers, in
   }
   UMT_TRY(need_workspace("rows compact", workspace, workspace_bytes, umt_rows_compact_workspace_bytes(rows)));
   unsigned grid = 0;
-  UMT_TRY(move_grid("rows compact", B, rows / 2 + 1, &grid));              // at most half of the rows move
+  UMT_TRY(move_grid("rows compact", B, rows / 2 + 1, 4096, &grid));              // at most half of the rows move
   int32_t *lists = (int32_t*)workspace, *counts = lists + 4 + 2 * (int64_t)rows;
   const int blocks = blocks_of(rows);
   const bool counted = blocks > 1;
   if (counted) hipLaunchKernelGGL(count_rows_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counts);
   hipLaunchKernelGGL(compact_list_kernel, dim3(blocks), dim3(ONE), 0, s, live, rows, counted ? counts : (int32_t*)nullptr, now, lists);
-  hipLaunchKernelGGL(compact_move_kernel, dim3(grid < 4096 ? grid : 4096), dim3(RT), 0, s, B, lists, rows, live, now, count);
+  hipLaunchKernelGGL(compact_move_kernel, dim3(grid), dim3(RT), 0, s, B, lists, rows, live, now, count);
   UMT_CHECK_HIP(hipGetLastError());
   return 0;
 }

@@ -30,7 +30,10 @@ def _split(name: str, x: torch.Tensor, gate: torch.Tensor, lead: int) -> Tuple[i
         g = g[:-1]
     if g != feat[:len(g)]:
         raise ValueError(f"{name}: gates {tuple(gate.shape[lead:])} are no leading dimensions of the features {feat}")
-    return math.prod(g), math.prod(feat[len(g):])
+    groups, share = math.prod(g), math.prod(feat[len(g):])
+    if max(xs[:lead]) >= 1 << 31 or max(groups, share) >= 1 << 31:             # the library takes them as ints
+        raise ValueError(f"{name}: x is {xs}")
+    return groups, share
 
 
 def _check_values(name: str, x, gate) -> torch.device:
@@ -131,6 +134,8 @@ def _backward(x, gate, kept, dh, dh_last, use, valid, groups: int, share: int, n
     xs, gs, ds = _rows_of(x, n), _rows_of(gate, groups), _rows_of(dh, n)
     dx = _like(x) if need[0] else None
     dgate = None if not need[1] else torch.empty_like(gate) if gate.is_contiguous() and x.is_contiguous() else _like(x, gate.shape[2:])
+    if dgate is not None and not n:
+        dgate.zero_()                                      # gates of no features
     dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=dev) if need[2] else None
     if R * n and any(need):
         shape = _shape(xs, gs, use, valid, groups, share, xs if dx is None else dx)
@@ -235,6 +240,8 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
         raise nat.UmtError("gated_step is not differentiable: use gated_scan, or call it under torch.no_grad()")
     rows = state.shape[0]
+    if rows >= 1 << 31:
+        raise ValueError(f"gated_step: state is {tuple(state.shape)}")
     if memory_idx is not None:
         if not isinstance(memory_idx, torch.Tensor) or memory_idx.dtype != torch.int64 or tuple(memory_idx.shape) != (B,) or memory_idx.device != dev:
             raise ValueError(f"gated_step: memory_idx is an int64 tensor ({B},) on {dev}")

@@ -53,6 +53,8 @@ def _collect(buffers, rows: Optional[int]):
         if have < rows:
             raise ValueError(f"{name}: the model has {have} memory rows reserved and not {rows}")
         entries[at:at + 2] = [(arr[0].data, arr[0].row_bytes), (arr[1].data, arr[1].row_bytes)]
+    if rows >= 1 << 31:                                                        # the library takes them as ints
+        raise ValueError(f"{name}: {rows} rows")
     arr = (nat.RowBuffer * len(entries))(*[nat.RowBuffer(p, n) for p, n in entries])
     return arr, len(entries), rows, dev
 
@@ -60,6 +62,8 @@ def _collect(buffers, rows: Optional[int]):
 def _ids(name: str, t, dev) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.dim() != 1 or t.device != dev:
         raise ValueError(f"{name}: expected a one-dimensional int64 tensor on {dev}")
+    if t.shape[0] >= 1 << 31:
+        raise ValueError(f"{name}: {t.shape[0]} row numbers")
     return t.contiguous()
 
 
@@ -122,6 +126,8 @@ def free_rows(live: torch.Tensor, rows: torch.Tensor, status: Optional[torch.Ten
     """live[rows] = False.  The content stays until a fork or a step overwrites it: start a new track with
     use_memory=False."""
     live = _live(live)
+    if live.shape[0] >= 1 << 31:
+        raise ValueError(f"live: {live.shape[0]} rows")
     dev = nat.require_gpu(live.device)
     rows = _ids("rows", rows, dev)
     st = _status(status, dev)

@@ -84,6 +84,22 @@ def test_weights_at_their_ends_and_refusals():
         LandmarkFilter(0.5).cuda()(x, sigmas=torch.ones(5, 2, 3, device="cuda"))
 
 
+def test_what_untracked_frames_hold_reaches_no_gradient():
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
+    g = torch.Generator().manual_seed(4)
+    x, sig, valid = torch.randn(40, 3, 21, 3, generator=g).cuda(), (torch.rand(40, 3, 21, generator=g) + 0.5).cuda(), (torch.rand(40, 3, generator=g) > 0.3).cuda()
+    grads = []
+    for poison in (1.0, 0.0, float("nan")):
+        filt = LandmarkFilter(0.6).cuda()
+        torch.nn.init.constant_(filt.slope, 0.25)
+        s = torch.where(valid[..., None], sig, torch.full((), poison, device="cuda"))
+        h, _ = filt(torch.where(valid[..., None, None], x, torch.full((), poison, device="cuda")), valid, s)
+        h.square().sum().backward()
+        grads.append((filt.bias.grad, filt.slope.grad))
+    for got in grads[1:]:
+        assert torch.equal(got[0], grads[0][0]) and torch.equal(got[1], grads[0][1])
+
+
 def test_fit_runs_and_its_gradients_are_the_formulas():
     from umetrack_amd.lib.common.landmark_filter import LandmarkFilter, filter_loss, fit_landmark_filter
     T, R = 60, 2

@@ -46,7 +46,8 @@ class LandmarkFilter(torch.nn.Module):
     def forward(self, landmarks: torch.Tensor, valid: Optional[torch.Tensor] = None, sigmas: Optional[torch.Tensor] = None,
                 h0: Optional[torch.Tensor] = None, use_memory: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """landmarks [T, R, 21, 3] float32 (any order of the first two dimensions, e.g. a result file's [2, T, 21, 3]
-        transposed), valid [T, R] bool: untracked frames keep the last filtered landmarks.  use_memory defaults to the
+        transposed), valid [T, R] bool: untracked frames keep the last filtered landmarks, and what landmarks and sigmas
+        hold there does not matter.  sigmas [T, R, 21] > 0.  use_memory defaults to the
         tracker's rule for `valid`, with h0 (state before the first frame) counting in frame 0.  Returns (filtered
         landmarks, state after the last frame [R, 21, 3])."""
         lead = tuple(landmarks.shape[:2])
@@ -55,6 +56,8 @@ class LandmarkFilter(torch.nn.Module):
             use_memory = memory_after_gaps(rule)
             if h0 is not None and lead[0]:
                 use_memory[0] = True
+        if valid is not None and sigmas is not None:       # a gate's gradient is 0 there, and 0 times the log of anything need not be
+            sigmas = torch.where(valid[..., None], sigmas, torch.ones((), device=sigmas.device))
         return gf.gated_scan(landmarks, self.gate(lead, sigmas), h0=h0, use_memory=use_memory, valid=valid)
 
     @torch.no_grad()

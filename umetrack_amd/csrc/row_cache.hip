@@ -212,8 +212,9 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
 }
 
 // More: two launches.  Every workgroup of the first marks all targets in a bit map of the cache in its LDS (64 KB of row
-// numbers from L2 for 8191 copies, where three launches over tables in HBM took 8 us), decides on copies of its own and brings
-// those sources to safety that the call overwrites.  plan[i]: what the second launch does.
+// numbers from L2 for 8191 copies), decides on copies of its own and brings those sources to safety that the call overwrites.
+// plan[i]: what the second launch does.  8191 of 32768 rows of 2592 + 64 + 252 bytes, sources and
+// targets drawn apart from each other: 6.3 + 10.4 us, where the five launches below take 25.
 enum { COPY_NOT = 0, COPY_ROW = 1, COPY_STAGED = 2 };
 constexpr int MAP_ROWS = 1 << 18;          // 32 KB of bits
 constexpr int MAP_COPIES = 1 << 14, MAP_GROUPS = 128, MAP_EACH = MAP_COPIES / MAP_GROUPS;
@@ -366,7 +367,7 @@ __device__ __forceinline__ int hand_out_rows(uint8_t* live, int rows, int64_t r0
   return all;
 }
 
-// everything in one workgroup; `moves`: the copies too
+// everything in one workgroup; `moves`: the copies too (6.7 us for 2 of 64 rows)
 __global__ __launch_bounds__(ONE) void fork_one_kernel(RowBuffers B, uint8_t* live, int rows, const int64_t* __restrict__ src, int n,
                                                        int64_t* ids, int32_t* order, int32_t* status, int moves) {
   __shared__ int lds[ONE / 64];
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(RT) void free_rows_kernel(uint8_t* __restrict__ liv
 // ---------------------------------------------------------------- compact
 // lists: [0] = live rows c, [1] = moves, from [4] on the holes below c and behind them the live rows from c on, in order.
 // counts may be null in a grid of one block.  (Workgroups that count all 65536 flags for themselves take 17 us, these two
-// launches 10.)  live is read only: the launch that moves writes it.
+// launches 2.8 + 7.1.)  live is read only: the launch that moves writes it.
 __global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __restrict__ live, int rows, const int32_t* __restrict__ counts,
                                                            int64_t* __restrict__ now, int32_t* __restrict__ lists) {
   __shared__ int lds[ONE / 64];
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __rest
   }
 }
 
-// rows at or above the live count move to free rows below it: no row is both
+// rows at or above the live count move to free rows below it: no row is both.  14600 of 65536 rows of 2592 + 64 + 252 bytes: 18 us, 4.6 TB/s.
 __global__ __launch_bounds__(RT) void compact_move_kernel(RowBuffers B, const int32_t* __restrict__ lists, int rows, uint8_t* __restrict__ live,
                                                           int64_t* __restrict__ now, int64_t* __restrict__ count) {
   const int lane = threadIdx.x & 63, pieces = B.piece0[B.n_long], c = lists[0], moves = lists[1];

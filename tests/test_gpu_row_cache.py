@@ -133,8 +133,11 @@ def test_rows_outside_the_cache_are_neither_freed_nor_forked():
 
 @pytest.mark.parametrize("kind,rows,dead", [("tracker", 1, 0), ("tracker", 1, 1), ("tracker", 2, 1), ("tracker", 64, 20), ("odd", 1024, 512),
                                             ("odd", 1025, 1000), ("tracker", 4100, 1300), ("long", 11, 5), ("odd", 9000, 0), ("odd", 9000, 9000),
-                                            ("odd", 70001, 23456), ("odd", 131072, 40000), ("odd", 140001, 70000), ("odd", 131073, 131073)])
-def test_compact(kind, rows, dead):
+                                            ("odd", 70001, 23456), ("odd", 131072, 40000), ("odd", 140001, 70000), ("odd", 131073, 131073),
+                                            ("odd", 262144, 5), ("odd", 262145, 262140), ("odd", 300003, 123456), ("tracker", 17, 16)])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_compact(kind, rows, dead, offset):
+    """offset: of the flags from an aligned address."""
     bufs = buffers(kind, rows)
     want = host(bufs)
     g = torch.Generator().manual_seed(dead)
@@ -146,8 +149,11 @@ def test_compact(kind, rows, dead):
     now[movers] = holes
     for w in want:
         w[holes] = w[movers]
-    live = mirror.cuda()
+    flags = torch.ones(rows + 32, dtype=torch.bool, device="cuda")
+    live = flags[offset:offset + rows]
+    live.copy_(mirror)
     got, count = _rc().compact_rows(bufs, live)
+    assert bool(flags[:offset].all()) and bool(flags[offset + rows:].all())
     assert count.tolist() == [c] and torch.equal(got.cpu(), now) and same(bufs, want)
     assert torch.equal(live.cpu(), torch.arange(rows) < c)
 

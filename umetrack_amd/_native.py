@@ -181,8 +181,9 @@ _NOTHING = _Nothing()
 
 
 def on_device(device):
-    """torch.cuda.device(device), or nothing where it is the current device already (1.5 us of a small call)."""
-    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """torch.cuda.device(device), or nothing where it is the current device already (1.5 us of a small call).  For
+    a device that holds a tensor already, so the runtime is up."""
+    return _NOTHING if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def raw_stream(device) -> int:

@@ -153,6 +153,33 @@ __device__ __forceinline__ int rank_in_group(int v, int* total, int* lds) {
   return before + incl - v;
 }
 
+// the same with the sums of two more numbers, behind one wait
+struct RankAndSums {
+  int rank, all, a, b;
+};
+__device__ __forceinline__ RankAndSums rank_and_sums(int v, int a, int b, int4* lds) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int incl = v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int w = __shfl_up(incl, o);
+    incl += lane >= o ? w : 0;
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  __syncthreads();
+  if (lane == 63) lds[wv] = make_int4(incl, a, b, 0);
+  __syncthreads();
+  RankAndSums r{incl - v, 0, 0, 0};
+  for (int k = 0; k < ONE / 64; ++k) {
+    const int4 w = lds[k];
+    r.rank += k < wv ? w.x : 0;
+    r.all += w.x;
+    r.a += w.y;
+    r.b += w.z;
+  }
+  return r;
+}
+
 // bit i: live[r + i] is set, i < 4; rows at or past `end` are not
 __device__ __forceinline__ int live4(const uint8_t* live, int64_t r, int64_t end) {
   int b = 0;
@@ -214,10 +241,10 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
 // More: two launches.  Every workgroup of the first marks all targets in a bit map of the cache in its LDS (64 KB of row
 // numbers from L2 for 8191 copies), decides on copies of its own and brings those sources to safety that the call overwrites.
 // plan[i]: what the second launch does.  8191 of 32768 rows of 2592 + 64 + 252 bytes, sources and
-// targets drawn apart from each other: 6.3 + 10.4 us, where the five launches below take 25.
+// targets drawn apart from each other: 5.3 + 10.9 us, where the five launches below take 25.
 enum { COPY_NOT = 0, COPY_ROW = 1, COPY_STAGED = 2 };
 constexpr int MAP_ROWS = 1 << 18;          // 32 KB of bits
-constexpr int MAP_COPIES = 1 << 14, MAP_GROUPS = 128, MAP_EACH = MAP_COPIES / MAP_GROUPS;
+constexpr int MAP_COPIES = 1 << 14, MAP_GROUPS = 128, MAP_EACH = MAP_COPIES / MAP_GROUPS;      // MAP_EACH <= ONE: a copy a thread
 __global__ __launch_bounds__(ONE) void copy_plan_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
                                                         int rows, uint8_t* __restrict__ plan, char* __restrict__ stage,
                                                         int32_t* __restrict__ status) {
@@ -228,35 +255,45 @@ __global__ __launch_bounds__(ONE) void copy_plan_kernel(RowBuffers B, const int6
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), pieces = B.piece0[B.n_long];
   for (int i = tid; i < (rows + 31) / 32; i += ONE) map[i] = 0;
   if (tid == 0) twice = n_todo = 0;
-  __syncthreads();
-  for (int i = tid; i < n; i += ONE) {
-    const int64_t d = dst[i];              // of a copy that will not be made too: a source too many brought to safety, no more
-    if (!in_cache(d, rows)) continue;
-    const uint32_t bit = 1u << (d & 31);
-    if (atomicOr(map + (d >> 5), bit) & bit) twice = 1;
+  const int each = (n + gridDim.x - 1) / gridDim.x, i0 = min(n, (int)blockIdx.x * each), i1 = min(n, i0 + each), mine = i0 + tid;
+  int64_t s = -1, d = -1;                   // a thread's own copy
+  if (mine < i1) {
+    s = src[mine];
+    d = dst[mine];
   }
   __syncthreads();
-  const int each = (n + gridDim.x - 1) / gridDim.x, i0 = min(n, (int)blockIdx.x * each), i1 = min(n, i0 + each);
+  constexpr int AHEAD = 8;
+  for (int k0 = tid; k0 < n; k0 += AHEAD * ONE) {
+    int64_t r[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) r[k] = k0 + k * ONE < n ? dst[k0 + k * ONE] : -1;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {      // of a copy that will not be made too: a source too many brought to safety, no more
+      if (!in_cache(r[k], rows)) continue;
+      const uint32_t bit = 1u << (r[k] & 31);
+      if (atomicOr(map + (r[k] >> 5), bit) & bit) twice = 1;
+    }
+  }
+  __syncthreads();
   if (twice) {                              // of several writes to one row the highest i counts
     for (int i = i0 + wv; i < i1; i += ONE / 64) {
-      const int64_t d = uniform(dst[i]);
+      const int64_t to = uniform(dst[i]);
       bool last = true;
-      for (int o = i + 1 + lane; o < n; o += 64) last &= dst[o] != d || !in_cache(src[o], rows);
+      for (int o = i + 1 + lane; o < n; o += 64) last &= dst[o] != to || !in_cache(src[o], rows);
       const bool counts = __all(last);
       if (lane == 0) late[i - i0] = !counts;
     }
     __syncthreads();
   }
-  for (int i = i0 + tid; i < i1; i += ONE) {
-    const int64_t s = src[i], d = dst[i];
+  if (mine < i1) {
     int what = COPY_NOT;
     if (!in_cache(s, rows) || !in_cache(d, rows)) {
       if (status) atomicOr(status, (int)UMT_STATUS_BAD_ROW);
-    } else if (s != d && !(twice && late[i - i0])) {
+    } else if (s != d && !(twice && late[tid])) {
       what = map[s >> 5] >> (s & 31) & 1 ? COPY_STAGED : COPY_ROW;
     }
-    plan[i] = (uint8_t)what;
-    if (what == COPY_STAGED) todo[atomicAdd(&n_todo, 1)] = (uint16_t)i;      // any order: each has its own place
+    plan[mine] = (uint8_t)what;
+    if (what == COPY_STAGED) todo[atomicAdd(&n_todo, 1)] = (uint16_t)mine;   // any order: each has its own place
   }
   __syncthreads();
   for (int it = wv; it < n_todo * pieces; it += ONE / 64) {
@@ -439,26 +476,29 @@ __global__ __launch_bounds__(RT) void free_rows_kernel(uint8_t* __restrict__ liv
 
 // ---------------------------------------------------------------- compact
 // lists: [0] = live rows c, [1] = moves, from [4] on the holes below c and behind them the live rows from c on, in order.
-// counts may be null in a grid of one block.  (Workgroups that count all 65536 flags for themselves take 17 us, these two
-// launches 2.8 + 7.1.)  live is read only: the launch that moves writes it.
+// counts may be null in a grid of one block.  (Workgroups that count all 65536 flags for themselves take 9.5 us, these two
+// launches 2.9 + 6.6, and a call is no shorter for it.)  live is read only: the launch that moves writes it.
 __global__ __launch_bounds__(ONE) void compact_list_kernel(const uint8_t* __restrict__ live, int rows, const int32_t* __restrict__ counts,
                                                            int64_t* __restrict__ now, int32_t* __restrict__ lists) {
-  __shared__ int lds[ONE / 64];
+  __shared__ int4 lds[ONE / 64];
   const int64_t r = (int64_t)blockIdx.x * BLOCK + threadIdx.x * 4;
   const int mine = live4(live, r, rows);
-  int here, k = rank_in_group(__popc(mine), &here, lds);
-  int c = here, below = 0;                  // live rows in all, before this block
-  if (counts) {
-    c = sum_counts(counts, gridDim.x, lds);
-    below = sum_counts(counts, blockIdx.x, lds);
-  }
+  int in_all = 0, before = 0;
+  if (counts)
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += ONE) {
+      const int n = counts[i];
+      in_all += n;
+      before += i < (int)blockIdx.x ? n : 0;
+    }
+  const RankAndSums first = rank_and_sums(__popc(mine), in_all, before, lds);
+  const int c = counts ? first.a : first.all;
   // live rows below row c: whole blocks, and the part of the block that row c lies in
   const int cut = counts ? c / BLOCK : 0;
-  int under;
-  rank_in_group(__popc(live4(live, (int64_t)cut * BLOCK + threadIdx.x * 4, c)), &under, lds);
-  if (counts) under += sum_counts(counts, cut, lds);
+  int part = __popc(live4(live, (int64_t)cut * BLOCK + threadIdx.x * 4, c));
+  for (int i = threadIdx.x; i < cut; i += ONE) part += counts[i];
+  const int under = rank_and_sums(0, part, 0, lds).a;
   int32_t *holes = lists + 4, *movers = holes + rows;
-  k += below;                               // live rows before row r
+  int k = first.rank + first.b;             // live rows before row r
   for (int i = 0; i < 4; ++i) {
     if (r + i >= rows) break;
     const bool lv = mine >> i & 1;

@@ -7,6 +7,7 @@ as the frames gave them.  ``gated_scan`` filters whole recordings in one call (c
 so a filter's constants can be learned from labelled recordings; ``gated_step`` does the same one frame at a time over a
 cache of rows, the way ``UmeTrackModel.temporal_step`` advances the temporal memory.  There is no CPU implementation.
 """
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -20,16 +21,21 @@ _DTYPES = {torch.float32: nat.VALUES_F32, torch.bfloat16: nat.VALUES_BF16}
 def _split(name: str, x: torch.Tensor, gate: torch.Tensor, lead: int) -> Tuple[int, int]:
     """(groups, share) of features x.shape[lead:] under gates gate.shape[lead:]: the gate's dimensions are the first of the
     feature's, up to dimensions of size 1 behind them; the features behind share a gate."""
-    xs, gs = tuple(x.shape), tuple(gate.shape)
+    return _split_shapes(name, x.shape, gate.shape, lead)
+
+
+@functools.lru_cache(maxsize=256)                          # a tracker asks for the same two shapes every frame
+def _split_shapes(name: str, x_shape, gate_shape, lead: int) -> Tuple[int, int]:
+    xs, gs = tuple(x_shape), tuple(gate_shape)
     feat, g = xs[lead:], gs[lead:]
     if xs[:lead] != gs[:lead]:
-        raise ValueError(f"{name}: x is {tuple(x.shape)} and gate {tuple(gate.shape)}: the first {lead} dimensions differ")
+        raise ValueError(f"{name}: x is {xs} and gate {gs}: the first {lead} dimensions differ")
     while g and (len(g) > len(feat) or g[-1] == 1 != feat[len(g) - 1]):
         if g[-1] != 1:
             break
         g = g[:-1]
     if g != feat[:len(g)]:
-        raise ValueError(f"{name}: gates {tuple(gate.shape[lead:])} are no leading dimensions of the features {feat}")
+        raise ValueError(f"{name}: gates {gs[lead:]} are no leading dimensions of the features {feat}")
     groups, share = math.prod(g), math.prod(feat[len(g):])
     if max(xs[:lead]) >= 1 << 31 or max(groups, share) >= 1 << 31:             # the library takes them as ints
         raise ValueError(f"{name}: x is {xs}")
@@ -42,9 +48,9 @@ def _check_values(name: str, x, gate) -> torch.device:
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         raise TypeError(f"{name}: x and gate are both float32 or both bfloat16, got {x.dtype} and {gate.dtype}")
     dev = x.device
-    if dev.type != "cuda":
+    if not x.is_cuda:
         nat.require_gpu()
-    if dev.type != "cuda" or gate.device != dev:
+    if not x.is_cuda or gate.device != dev:
         raise ValueError(f"{name}: x is on {x.device} and gate on {gate.device}: both have to be on one GPU")
     return dev
 
@@ -234,8 +240,8 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     if x.dim() < 1 or not isinstance(state, torch.Tensor):
         raise ValueError("gated_step: x is [B, ...features] and state a tensor")
     groups, share = _split("gated_step", x, gate, 1)
-    B, feat = x.shape[0], tuple(x.shape[1:])
-    if state.dtype != torch.float32 or state.dim() < 1 or tuple(state.shape[1:]) != feat or state.device != dev or not state.is_contiguous():
+    B, feat = x.shape[0], x.shape[1:]
+    if state.dtype != torch.float32 or state.dim() < 1 or state.shape[1:] != feat or state.device != dev or not state.is_contiguous():
         raise ValueError(f"gated_step: state is a contiguous float32 tensor [rows, {', '.join(map(str, feat))}] on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
         raise nat.UmtError("gated_step is not differentiable: use gated_scan, or call it under torch.no_grad()")
@@ -243,7 +249,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     if rows >= 1 << 31:
         raise ValueError(f"gated_step: state is {tuple(state.shape)}")
     if memory_idx is not None:
-        if not isinstance(memory_idx, torch.Tensor) or memory_idx.dtype != torch.int64 or tuple(memory_idx.shape) != (B,) or memory_idx.device != dev:
+        if not isinstance(memory_idx, torch.Tensor) or memory_idx.dtype != torch.int64 or memory_idx.shape != (B,) or memory_idx.device != dev:
             raise ValueError(f"gated_step: memory_idx is an int64 tensor ({B},) on {dev}")
         memory_idx = memory_idx.contiguous()
     elif B > rows:
@@ -253,8 +259,8 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     x, gate = x.contiguous(), gate.contiguous()
     if out is None:
         out = torch.empty_like(x)
-    elif tuple(out.shape) != (B,) + feat or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"gated_step: out is a contiguous {x.dtype} tensor {(B,) + feat} on {dev}")
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"gated_step: out is a contiguous {x.dtype} tensor {tuple(x.shape)} on {dev}")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or status.device != dev):
         raise ValueError(f"gated_step: status is int32[1] on {dev}")
     if out.numel() == 0:

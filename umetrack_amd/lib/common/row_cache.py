@@ -24,15 +24,16 @@ def _collect(buffers, rows: Optional[int]):
     entries, dev, models, name = [], None, [], "row cache"
     for b in buffers:
         if isinstance(b, torch.Tensor):
-            if b.dim() < 1 or not b.is_cuda or not b.is_contiguous() or b.numel() == 0 and b.shape[0] > 0:
+            have, size = b.shape[0] if b.dim() else 0, b.nbytes
+            if b.dim() < 1 or not b.is_cuda or not b.is_contiguous() or have and not size:
                 raise ValueError(f"{name}: a buffer is a contiguous GPU tensor [rows, ...], got {tuple(b.shape)} on {b.device}")
             if b.requires_grad and torch.is_grad_enabled():
                 raise nat.UmtError(f"{name}: a buffer that requires gradients cannot be moved in place")
-            rows = b.shape[0] if rows is None else rows
-            if b.shape[0] != rows:
-                raise ValueError(f"{name}: a buffer has {b.shape[0]} rows and not {rows}")
+            rows = have if rows is None else rows
+            if have != rows:
+                raise ValueError(f"{name}: a buffer has {have} rows and not {rows}")
             d = b.device
-            entries.append((b.data_ptr(), b.numel() // rows * b.element_size() if rows else 1))
+            entries.append((b.data_ptr(), size // rows if rows else 1))
         elif hasattr(b, "memory_buffers"):
             d = b.device
             if d is None:
@@ -55,7 +56,7 @@ def _collect(buffers, rows: Optional[int]):
         entries[at:at + 2] = [(arr[0].data, arr[0].row_bytes), (arr[1].data, arr[1].row_bytes)]
     if rows >= 1 << 31:                                                        # the library takes them as ints
         raise ValueError(f"{name}: {rows} rows")
-    arr = (nat.RowBuffer * len(entries))(*[nat.RowBuffer(p, n) for p, n in entries])
+    arr = (nat.RowBuffer * len(entries))(*entries)
     return arr, len(entries), rows, dev
 
 

@@ -170,29 +170,37 @@ struct Lanes {
     step = (OFF)(t_stride * (int64_t)sizeof(V));
     mine = (OFF)(((row - row0) * row_stride + inner) * (int64_t)sizeof(V));
   }
+  // `mine`, hidden from the compiler, which would add it to `at` ahead of the loops and then address every step by 64-bit
+  // vector additions instead of a scalar base and a 32-bit offset
+  __device__ __forceinline__ OFF here() const {
+    OFF m = mine;
+    asm volatile("" : "+v"(m));
+    return m;
+  }
   // steps t0 .. t0 + KEEP - 1; those past the end read the last one
   __device__ __forceinline__ void load(int t0, int T, Raw (&r)[KEEP]) const {
     Global p = at + (int64_t)(t0 < T ? t0 : T - 1) * (int64_t)step;
     const int more = T - 1 - t0;            // steps that follow the first
+    const OFF m = here();
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-      r[j] = *(At)(p + mine);
+      r[j] = *(At)(p + m);
       p += j < more ? step : (OFF)0;
     }
   }
-  __device__ __forceinline__ void store_one(int t, const float (&v)[E]) const {
-    *(At)(at + (int64_t)t * (int64_t)step + mine) = Values<V, E>::close(v);
-  }
+  __device__ __forceinline__ Global step_at(int t) const { return at + (int64_t)t * (int64_t)step; }
+  __device__ __forceinline__ void store_at(Global p, OFF m, const float (&v)[E]) const { *(At)(p + m) = Values<V, E>::close(v); }
   __device__ __forceinline__ void store(int t0, int T, bool on, const float (&v)[KEEP][E]) const {
     Global p = at + (int64_t)t0 * (int64_t)step;
     if (!on) return;
+    const OFF m = here();
     if (t0 + KEEP <= T) {
 #pragma unroll
-      for (int j = 0; j < KEEP; ++j, p += step) *(At)(p + mine) = Values<V, E>::close(v[j]);
+      for (int j = 0; j < KEEP; ++j, p += step) *(At)(p + m) = Values<V, E>::close(v[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < KEEP; ++j, p += step)
-        if (t0 + j < T) *(At)(p + mine) = Values<V, E>::close(v[j]);
+        if (t0 + j < T) *(At)(p + m) = Values<V, E>::close(v[j]);
     }
   }
 };
@@ -591,12 +599,23 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
 
 // ---------------------------------------------------------------- backward
 // Sums over the features of a gate.  A wave's lanes hold consecutive features, so a gate's are a run of lanes (a lane's own
-// two are added first; `share` and `per` count lanes here).  The KEEP steps' products go through the wave's own LDS rows;
-// lane 16 k + j adds up step j: whole gates k, k + 4, ... where the wave holds many, every fourth product of each where it
-// holds few.  A gate that reaches into other waves leaves its part in `part`, and a second launch adds the parts in order
-// (255 steps of 384 x 18 gates: 7.5 us).
-constexpr int SUM_ROW = 65;                // floats of a step's row: the 16 steps of a read lie in different banks
+// two are added first; `share` and `per` count lanes here).  The KEEP steps' products go through the wave's own LDS rows.
+// Gates of 16 lanes and more: lane 16 k + j reads the 16 products of step j that lanes 16 k .. 16 k + 15 left, at most two
+// gates' of which the second begins at `bound`, and the four such parts of a step are added across the wave.  Smaller gates:
+// with n gates in the wave, lane n i + k adds up gate k of the steps i, i + 64 / n, ...  A gate that reaches into other waves leaves its part in `part`,
+// and a second launch adds the parts in order (255 steps of 384 x 18 gates: 7.5 us).
+constexpr int SUM_ROW = 68;                // floats of a step's row: 16-byte reads of 16 steps lie in different banks
 constexpr int SUM_ROWS = KEEP * SUM_ROW + 64;      // reads past a gate's end are thrown away, but made
+constexpr int WIDE_GATE = 16;
+constexpr int WIDE_GATES = 5;              // that a wave can hold parts of
+
+// v of the lanes 16 and 32 away added: the same sum in all four
+__device__ __forceinline__ float add_quarters(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
 
 template <typename V>
 struct GateSums {
@@ -604,11 +623,16 @@ struct GateSums {
   int left;                // gates from the wave's first to the call's last
   int count, lead, per;    // gates that the wave holds, lanes of the first that lie before it, lanes
   int share, slots, slot0; // slot0: waves that hold the first gate before this one
+  int step;                // this lane's first step: lane & 15, or of gates of fewer than WIDE_GATE lanes lane / count
+  int wide0, bound;        // wide gates: that of lane (lane & ~15), and how many lanes on the next begins
+  int lo, n;               // smaller ones: the first product of gate lane % count, and how many the wave has
+  bool whole;              // all of them, so this is the sum
+  int64_t off;             // and where it goes
   int64_t row_step;        // of dgate
-  V* to;                   // the first gate's places at step (lane & 15) of the axis
+  V* to;                   // the first gate's places at this lane's first step
   float* part;
   __device__ __forceinline__ GateSums(const umt_gated_shape& S, int64_t row0, int64_t e0, int E, int per_, int slots_, V* dgate, float* parts) {
-    const int j = threadIdx.x & 15;
+    const int lane = threadIdx.x & 63;
     const int64_t G = (int64_t)S.rows * S.groups, inner = e0 - row0 * (S.groups * S.share);
     gi0 = (int)inner / S.share;
     groups = S.groups;
@@ -621,50 +645,96 @@ struct GateSums {
     slot0 = (lead + per - 1) / per;
     count = share ? (lead + per + share - 1) / share : 0;
     row_step = S.dgate_row;
-    to = dgate + j * S.dgate_t + row0 * S.dgate_row + gi0;
-    part = parts + ((int64_t)j * G + group0) * slots;
+    step = lane & 15;
+    if (share >= WIDE_GATE) {
+      const int from = lead + (lane & 48);
+      wide0 = from / share;
+      bound = (wide0 + 1) * share - from;
+    } else if (share > 0) {
+      step = lane / count;
+      const int k = lane - step * count, at = k * share - lead;
+      lo = max(0, at);
+      n = min(per, at + share) - lo;
+      whole = n == share;
+      off = whole ? place(k) : part_place(k);
+      if (step >= 64 / count || k >= left) step = KEEP;    // nothing to do
+    }
+    to = dgate + step * S.dgate_t + row0 * S.dgate_row + gi0;
+    part = parts + ((int64_t)step * G + group0) * slots;
   }
+  // gate k of the wave from its first: one row further where rows have as many as the 64 that a wave may hold
+  __device__ __forceinline__ int64_t place(int k) const {
+    const int row_on = gi0 + k < groups ? 0 : groups >= 64 ? 1 : (int)((unsigned)(gi0 + k) / (unsigned)groups);
+    return row_on * row_step + (k - row_on * groups);
+  }
+  __device__ __forceinline__ int64_t part_place(int k) const { return (int64_t)k * slots + (k == 0 ? slot0 : 0); }
 };
 
-// v: this lane's products of KEEP steps; rows: the wave's LDS; the steps from t0 on lie to_t0 and part_t0 elements on
+// v: this lane's products of KEEP steps; rows: the wave's LDS; the steps from t0 on lie to_t0 and part_t0 elements on, to_t and
+// part_t from one to the next
 template <typename V>
 __device__ __forceinline__ void sum_gates(const GateSums<V>& A, float* rows, const float (&v)[KEEP][1], bool on, int steps, int64_t to_t0,
-                                          int64_t part_t0) {
-  const int lane = threadIdx.x & 63, j = lane & 15, k0 = lane >> 4;
+                                          int64_t to_t, int64_t part_t0, int64_t part_t) {
+  const int lane = threadIdx.x & 63, k0 = lane >> 4;
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) rows[i * SUM_ROW + lane] = on ? v[i][0] : 0.f;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const float* row = rows + j * SUM_ROW;
-  const bool many = A.count > 6;
-  const int by = many ? 1 : 4, mine = many ? 0 : k0;
-  for (int k = many ? k0 : 0; k < A.count; k += many ? 4 : 1) {
-    const int lo = max(0, k * A.share - A.lead), hi = min(A.per, (k + 1) * A.share - A.lead), n = hi - lo;
-    float s = 0.f;
-    for (int m = 0; m < A.share; m += 4 * by) {            // four reads in flight, added in a fixed order
-      float r[4];
+  if (A.share >= WIDE_GATE) {
+    const float* row = rows + A.step * SUM_ROW;
+    float4 r[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = row[lo + mine + m + i * by];
+    for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const float4*>(row + 16 * k0 + 4 * i);
+    float lo[4], hi[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = mine + m + i * by < n ? r[i] : 0.f;
-      s += (r[0] + r[1]) + (r[2] + r[3]);
-      if (!many && m + 16 >= n) break;
-    }
-    if (!many) {
-      s += __shfl_xor(s, 16);
-      s += __shfl_xor(s, 32);
-    }
-    if (j < steps && k < A.left && (many || k0 == 0)) {
-      if (n == A.share) {
-        int gi = k, row_on = 0;              // at most 64 gates on: one row further where rows have that many
-        if (A.gi0 + k >= A.groups) {
-          row_on = A.groups >= 64 ? 1 : (int)((unsigned)(A.gi0 + k) / (unsigned)A.groups);
-          gi -= row_on * A.groups;
-        }
-        store_value(A.to + to_t0 + (row_on * A.row_step + gi), s);
-      } else {
-        A.part[part_t0 + k * A.slots + (k == 0 ? A.slot0 : 0)] = s;
+    for (int i = 0; i < 4; ++i) {
+      const float p[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const bool next = 4 * i + m >= A.bound;
+        lo[m] = (i ? lo[m] : 0.f) + (next ? 0.f : p[m]);
+        hi[m] = (i ? hi[m] : 0.f) + (next ? p[m] : 0.f);
       }
+    }
+    const float first = (lo[0] + lo[1]) + (lo[2] + lo[3]), second = (hi[0] + hi[1]) + (hi[2] + hi[3]);
+    float mine = 0.f, fifth = 0.f;           // gate k0; gate 4 where there is one
+#pragma unroll
+    for (int k = 0; k < WIDE_GATES; ++k) {
+      if (k >= A.count) break;
+      const float sum = add_quarters(A.wide0 == k ? first : A.wide0 + 1 == k ? second : 0.f);
+      if (k < 4)
+        mine = k0 == k ? sum : mine;
+      else
+        fifth = sum;
+    }
+    auto put = [&](int k, float sum) __attribute__((always_inline)) {
+      if (A.step >= steps || k >= A.left || k >= A.count) return;
+      if (min(A.per, (k + 1) * A.share - A.lead) - max(0, k * A.share - A.lead) == A.share)
+        store_value(A.to + to_t0 + A.place(k), sum);
+      else
+        A.part[part_t0 + A.part_place(k)] = sum;
+    };
+    put(k0, mine);
+    if (A.count > 4 && k0 == 0) put(4, fifth);
+  } else {
+    const int by = 64 / A.count;             // steps at once: neighbouring lanes write neighbouring gates
+    V* to = A.to + (to_t0 + A.off);
+    float* part = A.part + (part_t0 + A.off);
+    for (int i = A.step; i < min(steps, KEEP); i += by, to += by * to_t, part += by * part_t) {
+      const float* row = rows + i * SUM_ROW + A.lo;
+      float sum = 0.f;
+      for (int m = 0; m < A.share; m += 4) {               // four reads in flight, added in a fixed order
+        float r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[q] = row[m + q];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[q] = m + q < A.n ? r[q] : 0.f;
+        sum += (r[0] + r[1]) + (r[2] + r[3]);
+      }
+      if (A.whole)
+        store_value(to, sum);
+      else
+        *part = sum;
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -699,7 +769,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
     float* __restrict__ parts, float* __restrict__ dh0) {
   constexpr int PW = partner_waves<W, RUNS>(), GW = group_threads<W, RUNS>() / 64;
   __shared__ float lds[PW > 1 ? 2 : 1][PW][3 * E][64];
-  __shared__ float sums[GW][SUM_ROWS];
+  __shared__ alignas(16) float sums[GW][SUM_ROWS];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
   if (W == 1 && !RUNS && part.wave >= P.waves) return;
@@ -783,8 +853,13 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
     asm volatile("" : "+v"(ub), "+v"(vb));  // the mask words anew: 32 registers of them across the two loops cost more
     auto down = [&](auto usual) __attribute__((always_inline)) {
       constexpr bool USUAL = decltype(usual)::value;
+      Global xp = out.step_at(t0 + KEEP - 1), gp = single.step_at(t0 + KEEP - 1);
+      const OFF xm = out.here(), gm = single.here();
 #pragma unroll
       for (int j = KEEP - 1; j >= 0; --j) {
+        const Global xa = xp, ga = gp;
+        xp -= out.step;
+        gp -= single.step;
         if (!USUAL && t0 + j >= S.t) continue;
         float g[E], x[E];
         Values<V, E>::open(rd[j], g);
@@ -802,8 +877,8 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
         if (MASK)
 #pragma unroll
           for (int i = 0; i < GE; ++i) slope[j][i] = masked_value(slope[j][i], bit_mask(ub & vb, j));
-        if (USUAL || dx) out.store_one(t0 + j, x);
-        if (GE == 2 && (USUAL || dgate)) single.store_one(t0 + j, slope[j]);
+        if (USUAL || dx) out.store_at(xa, xm, x);
+        if (GE == 2 && (USUAL || dgate)) single.store_at(ga, gm, slope[j]);
       }
     };
     if (at.on) {
@@ -814,7 +889,9 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
     }
     if (E == 1 && dgate && S.share == 1) single.store(t0, S.t, at.on, slope);
     if constexpr (GE == 1)
-      if (dgate && S.share > 1) sum_gates(A, sums[threadIdx.x >> 6], slope, at.on, S.t - t0, (int64_t)t0 * S.dgate_t, (int64_t)t0 * S.rows * S.groups * slots);
+      if (dgate && S.share > 1)
+        sum_gates(A, sums[threadIdx.x >> 6], slope, at.on, S.t - t0, (int64_t)t0 * S.dgate_t, S.dgate_t, (int64_t)t0 * S.rows * S.groups * slots,
+                  (int64_t)S.rows * S.groups * slots);
     if (dh0 && at.on && t0 == 0)
 #pragma unroll
       for (int i = 0; i < E; ++i) dh0[at.e + i] = b[i];

@@ -121,6 +121,14 @@ def test_scan_and_gradients(shape, dtype, masks, rows_first):
         assert torch.equal(h.detach()[-1], last.detach())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("share", [2, 4, 6, 14, 15, 16, 17, 20, 21, 22, 28, 30, 31, 32, 33, 34, 36, 42, 47, 48, 62, 63, 64, 66, 126, 127, 128, 129, 250])
+def test_gate_sums_of_every_width(share, dtype):
+    """Gates that begin and end anywhere among a wave's lanes, in rows of few gates and of many."""
+    for shape in ((19, 5, 7, share), (16, 3, 1, share), (3, 2, 67, share)):
+        test_scan_and_gradients(shape, dtype, True, False)
+
+
 def test_every_mask_combination_and_what_lies_under_it():
     """Rows that are never valid, never keep memory, or neither; NaN, infinities and the type's extremes under the masks."""
     T, R = 40, 8

@@ -760,8 +760,9 @@ __global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int p
 // From the last stretch to the first: the states of a stretch again from the kept one before it, then the gradients down.
 //   s = dh + v,  dx = c s,  dgate = sum a c s (h' - x),  v' = a s
 // 512 steps of 512 rows of 648 bf16 values with a gate each: 380 us for 1.74 GB (4.6 TB/s).  255 steps of 384 rows of 18 x 36
-// values: 130 us for 0.40 GB (3.1 TB/s): two waves a SIMD, about 55 vector operations for the two values of a lane and step,
-// and the sums.  A stretch of inputs ahead is what fits: gradients ahead too spill (x1.4 to x3.7).
+// values: 112 us for 0.40 GB (3.5 TB/s): two waves a SIMD, of which the vector operations alone take 70 us (about 65 for the
+// two values of a lane and step) and the sums about 10.  A stretch of inputs ahead is what fits: gradients ahead too spill
+// (x1.4 to x3.7).  Both weights a step in the place of m: 3 % less there, 3 % more with a gate a value.
 template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
 __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_backward_kernel(
     umt_gated_shape S, Split P, int slots, const V* __restrict__ x, const V* __restrict__ gate, Masks mk, const float* __restrict__ kept,
@@ -1043,7 +1044,7 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
 // How the axis is shared out, for waves of `per` values.  A wave that walks alone needs about four others on its CU to keep
 // HBM busy; below that the waves of a workgroup take turns.  Fewer than 128 workgroups leave half of the CUs without one: an
 // axis of more than two such tiles is cut into runs then, 2048 waves in all, at the price of reading the inputs twice
-// (4000 x 64 x 63 fp32: backward 270 us in tiles, 106 in runs; 2000 x 200 x 63: 165 in tiles, 225 in runs).
+// (4000 x 64 x 63 fp32: backward 270 us in tiles, 97 in runs; 2000 x 200 x 63: 136 in tiles, 225 in runs).
 static Split split_axis(const umt_gated_shape& S, int per) {
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   const int all = S.t > 0 ? (S.t + KEEP - 1) / KEEP : 1;

@@ -389,21 +389,33 @@ struct Split {
   int64_t waves;           // of `per` values
 };
 
+// Workgroups go to the 8 XCDs in turn, and each XCD has an L2 of its own: neighbours among `all` pieces of work share the
+// 128-byte lines that lie across their border, so each XCD gets an unbroken eighth of them.
+constexpr unsigned XCDS = 8;
+static unsigned xcd_grid(int64_t all) { return (unsigned)((all + XCDS - 1) / XCDS * XCDS); }
+__device__ __forceinline__ unsigned xcd_piece() { return (blockIdx.x % XCDS) * (gridDim.x / XCDS) + blockIdx.x / XCDS; }
+
 // Where a wave works: its lanes' wave, its first stretch, how many stretches, the distance between them
 template <int W, bool RUNS>
 struct Part {
   int64_t wave;
+  int group;               // of runs
   int tw, first, count, by;
+  bool none;               // nowhere: the same for a whole workgroup where it shares work
   __device__ __forceinline__ Part(const Split& P, int T) {
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), all = (T + KEEP - 1) / KEEP;
+    const unsigned piece = xcd_piece();
     if (RUNS) {
-      wave = blockIdx.x;
+      group = (int)(piece / (unsigned)P.waves);            // fewer than 128 waves
+      wave = piece - (unsigned)group * (unsigned)P.waves;
+      none = group >= P.groups;
       tw = wv;
-      first = (blockIdx.y * RUN_WAVES + wv) * P.len;
+      first = (group * RUN_WAVES + wv) * P.len;
       count = max(0, min(P.len, all - first));
       by = 1;
     } else {
-      wave = W == 1 ? (int64_t)blockIdx.x * (GT / 64) + wv : blockIdx.x;
+      wave = W == 1 ? (int64_t)piece * (GT / 64) + wv : piece;
+      none = wave >= P.waves;
       tw = first = W == 1 ? 0 : wv;
       count = (all + W - 1) / W;            // the same for all waves of a workgroup, which meet at a barrier a tile
       by = W;
@@ -429,6 +441,7 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
   using W = Walk<V, E, GE, OFF, MASK>;
   const int lane = threadIdx.x & 63;
   const Part<1, true> part(P, S.t);
+  if (part.none) return;
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   const W w(S, at, v, v_t, v_row, gate, mk);
@@ -482,7 +495,7 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
     lds[part.tw][3 * i][lane] = own[i].a;
     lds[part.tw][3 * i + 1][lane] = own[i].q;
     lds[part.tw][3 * i + 2][lane] = own[i].p;
-    if (at.on) store_stretch(run_at(ws, N, blockIdx.y * RUN_WAVES + part.tw), N, at.e + i, own[i]);
+    if (at.on) store_stretch(run_at(ws, N, part.group * RUN_WAVES + part.tw), N, at.e + i, own[i]);
   }
   __syncthreads();
   if (part.tw != 0 || !at.on) return;
@@ -493,16 +506,16 @@ __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_sh
       const int k = BACK ? RUN_WAVES - 1 - n : n;
       all = then(all, Stretch{lds[k][3 * i][lane], lds[k][3 * i + 1][lane], lds[k][3 * i + 2][lane]});
     }
-    store_stretch(run_at(ws, N, P.groups * RUN_WAVES + blockIdx.y), N, at.e + i, all);
+    store_stretch(run_at(ws, N, P.groups * RUN_WAVES + part.group), N, at.e + i, all);
   }
 }
 
 // State with which this wave's run begins: the workgroups before it (BACK: behind it) are joined by the waves, an equal
 // share each, then the runs before it in its own
 template <bool BACK, int E>
-__device__ __forceinline__ void enter_run(const float* ws, const Split& P, int64_t N, int64_t e, int tw, int lane, float (&h)[E],
+__device__ __forceinline__ void enter_run(const float* ws, const Split& P, int group, int64_t N, int64_t e, int tw, int lane, float (&h)[E],
                                           Partners<RUN_WAVES, E>& partners) {
-  const int group = blockIdx.y, count = BACK ? P.groups - 1 - group : group, each = (count + RUN_WAVES - 1) / RUN_WAVES;
+  const int count = BACK ? P.groups - 1 - group : group, each = (count + RUN_WAVES - 1) / RUN_WAVES;
   const int i0 = min(count, tw * each), i1 = min(count, i0 + each);
   const float* joined = ws + (int64_t)P.groups * RUN_WAVES * 3 * N;
   Stretch run[E], own[E];
@@ -538,7 +551,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
   __shared__ float lds[PW > 1 ? 2 : 1][PW][3 * E][64];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
-  if (W == 1 && !RUNS && part.wave >= P.waves) return;
+  if (part.none) return;
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   using Wk = Walk<V, E, GE, OFF, MASK>;
@@ -550,7 +563,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
   float cur[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) cur[i] = h0 ? h0[at.e + i] : 0.f;
-  if constexpr (RUNS) enter_run<false>(ws, P, N, at.e, part.tw, lane, cur, partners);
+  if constexpr (RUNS) enter_run<false>(ws, P, part.group, N, at.e, part.tw, lane, cur, partners);
   auto keep = [&](int c, const float(&st)[E]) __attribute__((always_inline)) {
     if (kept && at.on)
 #pragma unroll
@@ -773,7 +786,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
   __shared__ alignas(16) float sums[GW][SUM_ROWS];
   const int lane = threadIdx.x & 63;
   const Part<W, RUNS> part(P, S.t);
-  if (W == 1 && !RUNS && part.wave >= P.waves) return;
+  if (part.none) return;
   const Place<E, OFF> at(S, part.wave, P.per);
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   using Wk = Walk<V, E, GE, OFF, MASK>;
@@ -785,7 +798,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
   float v[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] = dh_last ? dh_last[at.e + i] : 0.f;
-  if constexpr (RUNS) enter_run<true>(ws, P, N, at.e, part.tw, lane, v, partners);
+  if constexpr (RUNS) enter_run<true>(ws, P, part.group, N, at.e, part.tw, lane, v, partners);
   typename Wk::Fetched now;                // a stretch ahead; its gradients are asked for when it begins and needed last
   typename Lanes<V, E, OFF>::Raw rd[KEEP];
   float first[E];
@@ -1101,20 +1114,20 @@ template <typename V, int E, int GE, typename OFF, bool MASK>
 static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* h0, V* h, float* h_last, float* kept,
                        float* ws, hipStream_t s) {
   const Split p = split_axis(S, 64 * E);
-  const unsigned n = (unsigned)p.waves;
+  const dim3 runs(xcd_grid(p.waves * p.groups)), tiles(xcd_grid(p.waves)), alone(xcd_grid((p.waves + 3) / 4));
 #define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                              \
   hipLaunchKernelGGL((gated_scan_kernel<V, E, GE, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, x, gate, mk, h0, ws, h, h_last, \
                      kept)
   if (p.len) {
-    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, false>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, x, S.x_t, S.x_row,
+    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, false>), runs, dim3(64 * RUN_WAVES), 0, s, S, p, x, S.x_t, S.x_row,
                        gate, mk, ws);
-    UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
+    UMT_SCAN(1, true, runs, 64 * RUN_WAVES);
   } else if (p.w == 1) {
-    UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
+    UMT_SCAN(1, false, alone, GT);
   } else if (p.w == 4) {
-    UMT_SCAN(4, false, dim3(n), 256);
+    UMT_SCAN(4, false, tiles, 256);
   } else {
-    UMT_SCAN(8, false, dim3(n), 512);
+    UMT_SCAN(8, false, tiles, 512);
   }
 #undef UMT_SCAN
   UMT_CHECK_HIP(hipGetLastError());
@@ -1126,21 +1139,21 @@ static int launch_backward(const umt_gated_shape& S, const V* x, const V* gate, 
                            const float* dh_last, V* dx, V* dgate, float* dh0, float* ws, hipStream_t s) {
   const int per = backward_values(S, E), slots = gate_slots(S, per);
   const Split p = split_axis(S, per);
-  const unsigned n = (unsigned)p.waves;
+  const dim3 runs(xcd_grid(p.waves * p.groups)), tiles(xcd_grid(p.waves)), alone(xcd_grid((p.waves + 3) / 4));
   float* parts = ws + run_floats(S, per);
 #define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                               \
   hipLaunchKernelGGL((gated_scan_backward_kernel<V, E, GE, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, slots, x, gate, mk, kept, \
                      dh, dh_last, ws, dx, dgate, parts, dh0)
   if (p.len) {
-    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, true>), dim3(n, p.groups), dim3(64 * RUN_WAVES), 0, s, S, p, dh, S.dh_t,
+    hipLaunchKernelGGL((gated_runs_kernel<V, E, GE, OFF, MASK, true>), runs, dim3(64 * RUN_WAVES), 0, s, S, p, dh, S.dh_t,
                        S.dh_row, gate, mk, ws);
-    UMT_SCAN(1, true, dim3(n, p.groups), 64 * RUN_WAVES);
+    UMT_SCAN(1, true, runs, 64 * RUN_WAVES);
   } else if (p.w == 1) {
-    UMT_SCAN(1, false, dim3((unsigned)((p.waves + 3) / 4)), GT);
+    UMT_SCAN(1, false, alone, GT);
   } else if (p.w == 4) {
-    UMT_SCAN(4, false, dim3(n), 256);
+    UMT_SCAN(4, false, tiles, 256);
   } else {
-    UMT_SCAN(8, false, dim3(n), 512);
+    UMT_SCAN(8, false, tiles, 512);
   }
 #undef UMT_SCAN
   if (dgate && slots) {

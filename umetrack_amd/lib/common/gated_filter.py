@@ -213,7 +213,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: Optional[torch.Tensor] =
     included).  Both False: h = 0.
 
     Returns (h [T, R, ...] in x's dtype and memory order, h_last [R, ...] float32, the state after the last step), and the
-    states a backward pass starts from as a third value with ``keep``.  Differentiable with respect to x, gate and h0."""
+    states a backward pass starts from as a third value with ``keep``, for ``gated_scan_backward``; autograd records nothing
+    then.  Without ``keep`` differentiable with respect to x, gate and h0."""
     dev = _check_values("gated_scan", x, gate)
     if x.dim() < 2:
         raise ValueError(f"gated_scan: x is [T, R, ...features], got {tuple(x.shape)}")

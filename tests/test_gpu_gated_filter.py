@@ -88,7 +88,8 @@ def slack(x, gate, h0, valid, T):
 SHAPES = [(1, 1, 1, 1), (1, 3, 21, 3), (2, 2, 22, 1), (15, 2, 21, 3), (16, 1, 1, 63), (17, 5, 7, 9), (31, 2, 1, 64), (33, 3, 5, 13),
           (64, 128, 21, 3), (65, 2, 2, 65), (100, 1, 18, 36), (257, 3, 1, 130), (640, 2, 21, 3), (1500, 1, 1, 2), (1025, 2, 3, 5),
           (48, 700, 63, 2), (5000, 2, 21, 3), (33, 100, 1, 1), (2000, 40, 1, 1), (70, 90, 5, 1), (9000, 1, 1, 70), (300, 300, 21, 3),
-          (40, 30, 6, 400), (700, 3, 22, 1), (90, 700, 300, 1), (4000, 2, 40, 1), (50, 64, 18, 36)]
+          (40, 30, 6, 400), (700, 3, 22, 1), (90, 700, 300, 1), (4000, 2, 40, 1), (50, 64, 18, 36), (400, 100, 21, 3),
+          (300, 165, 21, 3), (290, 20, 72, 5)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])

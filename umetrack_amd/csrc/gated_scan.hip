@@ -406,7 +406,7 @@ struct Part {
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), all = (T + KEEP - 1) / KEEP;
     const unsigned piece = xcd_piece();
     if (RUNS) {
-      group = (int)(piece / (unsigned)P.waves);            // fewer than 128 waves
+      group = (int)(piece / (unsigned)P.waves);
       wave = piece - (unsigned)group * (unsigned)P.waves;
       none = group >= P.groups;
       tw = wv;
@@ -1055,20 +1055,28 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
 }
 
 // How the axis is shared out, for waves of `per` values.  A wave that walks alone needs about four others on its CU to keep
-// HBM busy; below that the waves of a workgroup take turns.  Fewer than 128 workgroups leave half of the CUs without one: an
-// axis of more than two such tiles is cut into runs then, 2048 waves in all, at the price of reading the inputs twice
-// (4000 x 64 x 63 fp32: backward 270 us in tiles, 97 in runs; 2000 x 200 x 63: 136 in tiles, 225 in runs).
+// HBM busy; below that the waves of a workgroup take turns.  With a tile on fewer than two thirds of the CUs, an axis of more
+// than two tiles is cut into runs, at the price of reading the inputs twice (fp32, forward / backward: 3000 steps of 148
+// waves 92 / 169 us in tiles, 82 / 144 in runs; 2000 steps of 197 waves 64 / 122 and 78 / 135).  Eight runs are a workgroup,
+// and as many of them as fill the CUs evenly run at once: of one to four per CU what has the shortest way, with a stretch
+// more for the start of each (3000 steps of 99 waves: 57 / 89 us in 495 workgroups, 79 / 129 in 297).
+constexpr int CUS = 256;
 static Split split_axis(const umt_gated_shape& S, int per) {
   const int64_t N = (int64_t)S.rows * S.groups * S.share;
   const int all = S.t > 0 ? (S.t + KEEP - 1) / KEEP : 1;
   Split p{per, 1, 0, 1, (N + per - 1) / per};
-  if (p.waves >= 1024 || all == 1) return p;
-  if (p.waves >= 128 || all <= 16) {
+  if (p.waves >= 1024 || all == 1 || p.waves == 0) return p;
+  if (p.waves >= 2 * CUS / 3 || all <= 16) {
     p.w = p.waves >= 256 || all <= 4 ? 4 : 8;
     return p;
   }
-  const int64_t runs = p.waves > 0 ? (2048 + p.waves - 1) / p.waves : 1;
-  p.len = (int)((all + runs - 1) / runs);
+  int64_t best = 0;
+  for (int each = 1; each <= 4; ++each) {   // workgroups per CU
+    const int64_t runs = each * CUS / p.waves * RUN_WAVES, len = (all + runs - 1) / runs;
+    if (best && each * (len + 1) >= best) continue;
+    best = each * (len + 1);
+    p.len = (int)len;
+  }
   p.groups = (all + p.len * RUN_WAVES - 1) / (p.len * RUN_WAVES);
   return p;
 }

@@ -432,8 +432,8 @@ __device__ __forceinline__ void store_stretch(float* s, int64_t N, int64_t e, co
   s[2 * N + e] = v.p;
 }
 
-// The step that each run is (BACK: of the gradient that comes from behind).  108001 steps of 2 x 21 landmarks, fp32: 21 us
-// for 72 MB, of which about 6 are the launch and the first loads.
+// The step that each run is (BACK: of the gradient that comes from behind).  108001 steps of 2 x 21 landmarks, fp32: 18.4 us
+// for 72 MB, of which about 5 are the launch and the first loads.
 template <typename V, int E, int GE, typename OFF, bool MASK, bool BACK>
 __global__ __launch_bounds__(64 * RUN_WAVES) void gated_runs_kernel(umt_gated_shape S, Split P, const V* __restrict__ v, int64_t v_t, int64_t v_row,
                                                                     const V* __restrict__ gate, Masks mk, float* __restrict__ ws) {
@@ -539,7 +539,7 @@ template <int W, bool RUNS>
 constexpr int group_threads() { return RUNS ? 64 * RUN_WAVES : W == 1 ? GT : 64 * W; }
 
 // A wave alone (512 steps of 512 rows of 648 bf16 values, a gate each): 235 us for 1.02 GB, 4.3 TB/s where a copy reaches 5.06.
-// Tiles (64 steps of 128 x 21 landmarks, fp32): 6 us.  Runs (108001 steps of 2 x 21 landmarks): 34 us for 127 MB, about 7 of
+// Tiles (64 steps of 128 x 21 landmarks, fp32): 6 us.  Runs (108001 steps of 2 x 21 landmarks): 27 us for 127 MB, about 6 of
 // them the launch, the first loads and the joining; the inputs have been read once before.
 template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
 __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(umt_gated_shape S, Split P, const V* __restrict__ x,
@@ -1084,6 +1084,13 @@ static int64_t run_floats(const umt_gated_shape& S, int per) {
   const Split p = split_axis(S, per);
   return p.len ? (int64_t)p.groups * (RUN_WAVES + 1) * 3 * S.rows * S.groups * S.share : 0;
 }
+// Values of a forward wave whose lanes hold E: 64 E, or as many whole rows as fit where rows lie further apart than steps and
+// that leaves at most 4 lanes idle (300 steps of 2000 rows of 63 fp32 values, rows first: 91 -> 81 us; with steps further
+// apart 78 -> 82).
+static int forward_values(const umt_gated_shape& S, int E) {
+  const int F = S.groups * S.share / E, whole = S.x_row > S.x_t && F > 0 && F <= 64 ? 64 / F * F : 0;
+  return (whole >= 60 ? whole : 64) * E;
+}
 // Values of a backward wave whose lanes hold E: 64 E, or as many whole gates as fit (21 landmarks of 3 coordinates: 63
 // lanes) where that leaves at most 4 lanes idle, so that their sums need no second launch.
 static int backward_values(const umt_gated_shape& S, int E) {
@@ -1121,7 +1128,7 @@ static bool near_rows(const umt_gated_shape& S, int64_t size) {
 template <typename V, int E, int GE, typename OFF, bool MASK>
 static int launch_scan(const umt_gated_shape& S, const V* x, const V* gate, Masks mk, const float* h0, V* h, float* h_last, float* kept,
                        float* ws, hipStream_t s) {
-  const Split p = split_axis(S, 64 * E);
+  const Split p = split_axis(S, forward_values(S, E));
   const dim3 runs(xcd_grid(p.waves * p.groups)), tiles(xcd_grid(p.waves)), alone(xcd_grid((p.waves + 3) / 4));
 #define UMT_SCAN(W, RUNS, GRID, THREADS)                                                                                              \
   hipLaunchKernelGGL((gated_scan_kernel<V, E, GE, OFF, W, MASK, RUNS>), GRID, dim3(THREADS), 0, s, S, p, x, gate, mk, h0, ws, h, h_last, \
@@ -1208,8 +1215,8 @@ using namespace umt;
 
 extern "C" int64_t umt_gated_scan_workspace_bytes(const umt_gated_shape* shape) {
   if (check_shape(shape, false) != 0) return -1;
-  int64_t n = run_floats(*shape, 64);                       // whichever way the tensors' places allow
-  if (pairable(*shape)) n = std::max(n, run_floats(*shape, 128));
+  int64_t n = 0;                                            // whichever way the tensors' places allow
+  for (int E = 1; E <= (pairable(*shape) ? 2 : 1); ++E) n = std::max(n, run_floats(*shape, forward_values(*shape, E)));
   return n * (int64_t)sizeof(float);
 }
 

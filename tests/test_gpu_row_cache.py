@@ -172,6 +172,16 @@ def test_empty_calls_and_an_empty_cache():
     assert now.shape == (0,) and count.tolist() == [0]
 
 
+@pytest.mark.parametrize("n", [1, 256, 257, 3000, 1 << 14, (1 << 14) + 1, 40000])
+def test_copies_into_an_empty_cache(n):
+    """No row number is good: nothing happens but the status bit, in all three forms of the copy."""
+    g = torch.Generator().manual_seed(n)
+    src, dst = torch.randint(-3, 9, (n,), generator=g).cuda(), torch.randint(-3, 9, (n,), generator=g).cuda()
+    st = status()
+    _rc().copy_rows([torch.empty(0, 3, device="cuda"), torch.empty(0, 2, 5, dtype=torch.uint8, device="cuda")], src, dst, st)
+    assert int(st) == nat.STATUS_BAD_ROW
+
+
 def test_rows_past_32_bits():
     """A row of 640 MB: the fourth starts past 2^31 bytes."""
     rows, n = 5, 160_000_000

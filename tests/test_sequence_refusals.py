@@ -125,6 +125,20 @@ def test_row_arguments():
     assert L.umt_rows_copy(good, n, 8, P, P, 0, None, None, 0, None) == 0 and L.umt_rows_fork(good, n, 8, P, P, 0, P, None, None, 0, None) == 0
 
 
+@pytest.mark.parametrize("row_bytes", [1, 252, 2656])
+def test_copies_into_an_empty_cache_have_their_workspace(row_bytes):
+    """What the launches write whatever the row numbers are: a byte a copy where the copies are planned in LDS, a count
+    and a word a copy where they are not."""
+    L = nat.lib()
+    for n, index in ((257, 257), (1 << 14, 1 << 14), ((1 << 14) + 1, 16 + 4 * ((1 << 14) + 1))):
+        for data in (None, P):
+            arr, k = rows_buf((data, row_bytes))
+            need = L.umt_rows_copy_workspace_bytes(arr, k, 0, n)
+            assert need >= index, (n, need)
+            assert L.umt_rows_copy(arr, k, 0, P, P, n, None, P, need - 1, None) == 5
+            assert L.umt_rows_copy(arr, k, 0, P, P, n, None, None, need, None) == 5
+
+
 def test_model_without_rows_and_null_handles():
     L = nat.lib()
     arr, rows = (nat.RowBuffer * 2)(), ctypes.c_int(7)

@@ -604,9 +604,10 @@ static int blocks_of(int64_t n) { return (int)((n + BLOCK - 1) / BLOCK); }
 extern "C" int64_t umt_rows_copy_workspace_bytes(const umt_row_buffer* buffers, int n_buffers, int rows, int n) {
   RowBuffers B;
   if (n < 0 || row_buffers("rows copy", buffers, n_buffers, rows, &B) != 0) return -1;
-  if (n == 0 || rows == 0 || few_rows(B, n)) return 0;
+  if (n == 0 || few_rows(B, n)) return 0;
+  // the index part holds a place for every copy asked for, also where no row number can be good
   const int64_t index = planned(rows, n) ? round_up64(n, 16) : round_up64((int64_t)rows * 4, 16) + round_up64(16 + (int64_t)n * 4, 16);
-  return index + n * B.staged_bytes;
+  return index + (rows ? n * B.staged_bytes : 0);
 }
 
 extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int rows, const int64_t* src, const int64_t* dst, int n,

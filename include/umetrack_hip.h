@@ -285,8 +285,10 @@ int umt_metric_partials_static(const float* gt, const float* pred, const uint8_t
  * use_memory[t,row] == 0 drops the memory (h[t] = x[t], whatever h[t-1] holds), valid[t,row] == 0 skips the frame
  * (h[t] = h[t-1]; x and gate of that frame may hold anything, NaN included); both 0 leave h[t] = 0.  Either mask may
  * be NULL (all ones).  Long axes are worked on in stretches, so equal states of different stretches may differ in the
- * last bits of a float32.  A non-finite x, gate or state that no mask excludes makes its feature non-finite until the memory is
- * dropped (gate = +-inf is a weight of 1 or 0).  The state is float32 whatever the dtype; h is rounded once, to nearest even.
+ * last bits of a float32.  Finite x and h0 of up to 3e38, of either sign, mix to finite states.  A non-finite x, gate or state
+ * that no mask excludes makes its feature non-finite until the memory is dropped (gate = +-inf is a weight of 1 or 0): an infinity
+ * stays one while frames are skipped and where it is mixed with finite values, and makes the gates' gradients behind it non-finite.
+ * The state is float32 whatever the dtype; h is rounded once, to nearest even.
  *
  * features = groups * share: `share` consecutive features use one gate (a landmark's 3 coordinates, a hand's 63, 1).
  * Element (t, row, feature) of x lies at t * x_t + row * x_row + feature, and so on: strides in elements, not negative,

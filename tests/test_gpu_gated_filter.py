@@ -177,6 +177,80 @@ def test_gates_at_their_ends_and_a_poisoned_memory():
     assert torch.equal(st, x[0])
 
 
+RANGE_SHAPES = [(1, 2, 3, 2), (40, 3, 5, 3), (300, 20, 21, 3), (3000, 2, 7, 4), (40, 1100, 63, 1)]     # alone, tiles, runs
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", RANGE_SHAPES, ids=str)
+@pytest.mark.parametrize("masks", [True, False])
+def test_values_at_the_ends_of_the_range(shape, dtype, masks):
+    """Inputs and states of either sign up to 3e38: their differences are beyond the largest float, the mix is not.  The
+    tolerances are the module's with M = 3e38; gradients small enough that no slope (a quarter of the difference times s) leaves
+    the range."""
+    T, R, G, K = shape
+    _, gate, _, use, valid = make(T, R, G, K, dtype, 3 * sum(shape), masks)
+    g = torch.Generator().manual_seed(1)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g) * 2.0 - 1
+    x = (sign(T, R, G, K) * (2e38 + 1e38 * torch.rand(T, R, G, K, generator=g))).to(DT[dtype]).cuda()
+    h0 = (sign(R, G, K) * 3e38).cuda()
+    dh = (1e-4 * torch.randn(T, R, G, K, generator=g)).to(DT[dtype]).cuda()
+    dl = (1e-4 * torch.randn(R, G, K, generator=g)).cuda()
+    before, gate_of = h0[:, :, :].clone(), gate.detach()
+    for t in (x, gate, h0):
+        t.requires_grad_(True)
+    h, last = _gf().gated_scan(x, gate, h0, use, valid)
+    grads = torch.autograd.grad((h, last), (x, gate, h0), (dh, dl))
+    want = oracle(*map(np64, (x, gate, h0, use, valid, dh, dl)))
+    eh, M, kk = slack(x, gate, h0, valid, T)
+    S = np.abs(want[5]).max()
+    es = 6 * U * S * kk
+    rnd = 2.0 ** -8 if dtype == "bf16" else 2 * U
+    slope = K * 0.25 * (S * (eh + 4 * U * M) + 2 * M * es + 12 * U * S * 2 * M)
+    assert np.abs(want[3]).max() < 3e38
+    for name, got, ref, tol in (("h", h, want[0], eh), ("last", last, want[1], eh), ("dx", grads[0], want[2], es + 4 * U * S),
+                                ("dgate", grads[1], want[3], slope), ("dh0", grads[2], want[4], es)):
+        got = np64(got)
+        assert np.isfinite(got).all(), name
+        assert (np.abs(got - ref) <= tol + (rnd if name in ("h", "dx", "dgate") else 2 * U) * np.abs(ref)).all(), name
+    with torch.no_grad():
+        one, _ = _gf().gated_scan(x[:1], gate_of[:1], before, None if use is None else use[:1], None if valid is None else valid[:1])
+        out = _gf().gated_step(x[0].detach(), gate_of[0], before, use_memory=None if use is None else use[0], valid=None if valid is None else valid[0])
+    assert torch.equal(out, one[0]) and bool(torch.isfinite(before).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 2, 1, 2), (40, 2, 1, 2), (300, 20, 21, 3), (3000, 2, 1, 2), (40, 1100, 63, 1)], ids=str)
+def test_an_infinite_state_is_kept_while_frames_are_skipped_and_mixed_as_the_formula_says(shape, dtype):
+    """In the first feature: an infinite h0, all frames skipped in row 0; frames that count in row 1, where an infinity of the
+    other sign then meets it (NaN) and the memory is dropped after that.  In the last one: an infinite input, whichever
+    weight is the larger."""
+    T, R, G, K = shape
+    x, gate, h0, _, _ = make(T, R, G, K, "fp32", T, masks=False)
+    use, valid = (torch.ones(T, R, dtype=torch.bool, device="cuda") for _ in range(2))
+    valid[:, 0] = False
+    x[:, 0], gate[:, 0] = float("nan"), float("nan")
+    h0[0, 0, 0], h0[1, 0, 0] = float("inf"), -float("inf")
+    if T > 20:
+        x[T // 2, 1, 0, 0] = float("inf")
+        use[T - T // 4, 1] = False
+        x[T // 3, 1, 0, K - 1] = -float("inf") if K > 1 else x[T // 3, 1, 0, 0]
+    x, gate = x.to(DT[dtype]), gate.to(DT[dtype])
+    state = h0.clone()
+    h, last = _gf().gated_scan(x, gate, h0, use, valid)
+    want, wl = oracle(*map(np64, (x, gate, h0, use, valid)))
+    assert np.isposinf(want[:, 0, 0, 0]).all() and np.isneginf(want[0, 1, 0, 0])
+    kind = lambda v: np.where(np.isnan(v), 3, np.where(np.isposinf(v), 2, np.where(np.isneginf(v), 1, 0)))
+    assert np.array_equal(kind(np64(h)), kind(want)) and np.array_equal(kind(np64(last)), kind(wl))
+    ok = np.isfinite(want)
+    h0f = torch.nan_to_num(h0, 0, 0, 0)
+    xf = torch.nan_to_num(x.float(), 0, 0, 0)
+    eh, _, _ = slack(xf, gate, h0f, valid, T)
+    assert (np.abs(np64(h)[ok] - want[ok]) <= eh + (2.0 ** -8 if dtype == "bf16" else 2 * U) * np.abs(want[ok])).all()
+    for t in range(min(T, 3)):
+        out = _gf().gated_step(x[t], gate[t], state, use_memory=use[t], valid=valid[t])
+        assert np.array_equal(kind(np64(out)), kind(want[t]))
+
+
 def test_slow_memory_and_old_outliers_keep_their_precision():
     """c = 8e-7 over 20000 frames: the response to a constant is 1 - a^T up to the rounding of the state, T u of it (1.2e-3);
     rounding a itself would change c by up to u / c = 7 % of it.  An outlier of 1e6 ahead of values

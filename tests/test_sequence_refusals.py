@@ -196,6 +196,44 @@ def test_types_and_devices():
         rc.free_rows(torch.ones(4, dtype=torch.bool), torch.zeros(1, dtype=torch.int64))
 
 
+def test_forward_mode_tangents():
+    """The kernels read values alone: a dual tensor's tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+    x, g, h0, one = torch.zeros(4, 2, 3), torch.zeros(4, 2), torch.zeros(2, 3), torch.zeros(1, dtype=torch.int64)
+    kept, dh = torch.zeros(1, 6), torch.zeros(4, 2, 3)
+    calls = ((lambda d: gf.gated_scan(d, g), x), (lambda d: gf.gated_scan(x, d), g), (lambda d: gf.gated_scan(x, g, h0=d), h0),
+             (lambda d: gf.gated_scan(d, g, keep=True), x), (lambda d: gf.gated_step(d, g[0], h0), x[0]), (lambda d: gf.gated_step(x[0], d, h0), g[0]),
+             (lambda d: gf.gated_step(x[0], g[0], d), h0), (lambda d: gf.gated_scan_backward(d, g, kept, dh), x),
+             (lambda d: gf.gated_scan_backward(x, g, kept, d), dh), (lambda d: gf.gated_scan_backward(x, g, kept, dh, d), h0))
+    with forward_ad.dual_level():
+        for call, t in calls:
+            for grad in (torch.enable_grad(), torch.no_grad()):
+                with grad, pytest.raises(nat.UmtError, match="forward-mode"):
+                    call(forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(Exception) as plain:            # a tensor without a tangent gets as far as it does outside
+            gf.gated_scan(x, g)
+        assert "forward-mode" not in str(plain.value)
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_on_the_gpu():
+    from torch.autograd import forward_ad
+    d = "cuda"
+    x, g, st, one = torch.rand(4, 2, 3, device=d), torch.zeros(4, 2, device=d), torch.zeros(2, 3, device=d), torch.zeros(1, dtype=torch.int64, device=d)
+    want = gf.gated_scan(x, g)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: gf.gated_scan(dual, g), lambda: gf.gated_step(dual[0], g[0], st),
+                     lambda: rc.copy_rows([forward_ad.make_dual(st, torch.ones_like(st))], one, one)):
+            with pytest.raises(nat.UmtError, match="forward-mode"):
+                call()
+        assert all(torch.equal(a, b) for a, b in zip(gf.gated_scan(x, g), want))
+        xr = x.clone().requires_grad_(True)
+        h, _ = gf.gated_scan(xr, g)
+        with pytest.raises(nat.UmtError, match="forward-mode"):
+            torch.autograd.grad(h, xr, forward_ad.make_dual(torch.ones_like(h), torch.ones_like(h)))
+
+
 @pytest.mark.gpu
 def test_tensors_that_do_not_fit():
     d = "cuda"

@@ -8,6 +8,7 @@ import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # (UMT_LIB_PATH: diagnostics only - A/B runs of an experiment build of the same ABI, e.g. tools/bin/*.so)
@@ -189,6 +190,16 @@ def on_device(device):
 def raw_stream(device) -> int:
     """The current stream's handle, without the Stream object that `stream_ptr` goes through (2 us of a small call)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def no_tangents(name: str, *tensors) -> None:
+    """Refuses tensors that carry a forward-mode tangent (torch.autograd.forward_ad): the kernels read values alone, and the
+    outputs would silently have none.  Only looked for inside a dual level (0.6 us a tensor otherwise)."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise UmtError(f"{name} has no forward-mode derivative")
 
 
 def dev_tensor(t, dtype, device) -> torch.Tensor:

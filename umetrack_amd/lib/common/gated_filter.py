@@ -42,9 +42,11 @@ def _split_shapes(name: str, x_shape, gate_shape, lead: int) -> Tuple[int, int]:
     return groups, share
 
 
-def _check_values(name: str, x, gate) -> torch.device:
+def _check_values(name: str, x, gate, *others) -> torch.device:
+    """The device of x and gate; `others`: what else may carry derivatives."""
     if not (isinstance(x, torch.Tensor) and isinstance(gate, torch.Tensor)):
         raise TypeError(f"{name}: x and gate are tensors")
+    nat.no_tangents(name, x, gate, *others)
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         raise TypeError(f"{name}: x and gate are both float32 or both bfloat16, got {x.dtype} and {gate.dtype}")
     dev = x.device
@@ -163,7 +165,7 @@ def gated_scan_backward(x: torch.Tensor, gate: torch.Tensor, kept: torch.Tensor,
     """(dx, dgate, dh0) of ``gated_scan(..., keep=True)`` for the gradients dh (of h, x's dtype) and dh_last (of h_last,
     float32): what autograd calls, and what a program calls that captures its backward pass into a HIP graph, where
     autograd's own bookkeeping of leaves does not belong.  ``need`` leaves out gradients that nobody asked for (None)."""
-    dev = _check_values("gated_scan_backward", x, gate)
+    dev = _check_values("gated_scan_backward", x, gate, kept, dh, dh_last)
     if x.dim() < 2:
         raise ValueError(f"gated_scan_backward: x is [T, R, ...], got {tuple(x.shape)}")
     groups, share = _split("gated_scan_backward", x, gate, 2)
@@ -193,6 +195,7 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dh_last):
         if dh is None and dh_last is None:
             return None, None, None, None, None, None, None
+        nat.no_tangents("gated_scan's backward pass", dh, dh_last)
         x, gate, kept, use, valid = ctx.saved_tensors
         if dh is None:
             dh = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
@@ -214,8 +217,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: Optional[torch.Tensor] =
 
     Returns (h [T, R, ...] in x's dtype and memory order, h_last [R, ...] float32, the state after the last step), and the
     states a backward pass starts from as a third value with ``keep``, for ``gated_scan_backward``; autograd records nothing
-    then.  Without ``keep`` differentiable with respect to x, gate and h0."""
-    dev = _check_values("gated_scan", x, gate)
+    then.  Without ``keep`` differentiable with respect to x, gate and h0, once and in reverse mode; tensors with forward-mode
+    tangents are refused."""
+    dev = _check_values("gated_scan", x, gate, h0)
     if x.dim() < 2:
         raise ValueError(f"gated_scan: x is [T, R, ...features], got {tuple(x.shape)}")
     groups, share = _split("gated_scan", x, gate, 2)
@@ -237,7 +241,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     [rows, ...features] float32 in place; returns its new value in x's dtype.  Masks [B] as ``gated_scan``'s.  Duplicates in
     memory_idx all read the previous row and the highest b writes it; an index outside the cache runs without memory, writes
     none and ORs UMT_STATUS_BAD_MEMORY_IDX into ``status`` (int32[1] on the device).  Not differentiable."""
-    dev = _check_values("gated_step", x, gate)
+    dev = _check_values("gated_step", x, gate, state, out)
     if x.dim() < 1 or not isinstance(state, torch.Tensor):
         raise ValueError("gated_step: x is [B, ...features] and state a tensor")
     groups, share = _split("gated_step", x, gate, 1)

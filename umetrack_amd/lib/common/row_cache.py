@@ -29,6 +29,7 @@ def _collect(buffers, rows: Optional[int]):
                 raise ValueError(f"{name}: a buffer is a contiguous GPU tensor [rows, ...], got {tuple(b.shape)} on {b.device}")
             if b.requires_grad and torch.is_grad_enabled():
                 raise nat.UmtError(f"{name}: a buffer that requires gradients cannot be moved in place")
+            nat.no_tangents(name, b)
             rows = have if rows is None else rows
             if have != rows:
                 raise ValueError(f"{name}: a buffer has {have} rows and not {rows}")

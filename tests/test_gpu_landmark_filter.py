@@ -70,6 +70,41 @@ def test_filter_over_recordings_and_frame_by_frame():
     assert worst <= 12 * U * np.abs(lm).max() / (1 - amax)
 
 
+@pytest.mark.parametrize("cut", range(1, 12))
+def test_a_recording_in_pieces_is_the_recording(cut):
+    """Cut inside gaps of one and of several frames, before and behind them, without use_memory."""
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
+    flags = ("110001111111", "110111011111", "000011111000", "111111111111", "000000000000")
+    valid = torch.tensor([[c == "1" for c in f] for f in flags]).t().contiguous()
+    T, R = valid.shape
+    lm = torch.randn(T, R, 21, 3, generator=torch.Generator().manual_seed(2)) * 30 + 300
+    filt = LandmarkFilter(0.7).cuda()
+    x, v = lm.cuda(), valid.cuda()
+    with torch.no_grad():
+        h, last = filt(x, v)
+        a, mid = filt(x[:cut], v[:cut])
+        b, end = filt(x[cut:], v[cut:], h0=mid, valid_before=v[cut - 1])
+        # every hand tracked throughout: nothing to say about the frame before
+        c, cm = filt(x[:cut])
+        d, _ = filt(x[cut:], h0=cm)
+        whole, _ = filt(x)
+    tol = 2 * 8 * U * float(lm.abs().max()) / 0.3
+    assert float((torch.cat([a, b]) - h).abs().max()) <= tol and float((end - last).abs().max()) <= tol
+    assert float((torch.cat([c, d]) - whole).abs().max()) <= tol
+    want = plain_filter(lm.double().numpy(), valid.numpy(), 0.7)
+    assert np.abs(torch.cat([a, b]).cpu().numpy() - want).max() <= tol
+
+
+def test_a_state_without_word_of_the_frame_before_is_refused():
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
+    x, v, h0 = torch.zeros(4, 2, 21, 3, device="cuda"), torch.ones(4, 2, dtype=torch.bool, device="cuda"), torch.zeros(2, 21, 3, device="cuda")
+    filt = LandmarkFilter(0.5).cuda()
+    for kw in (dict(valid=v, h0=h0), dict(valid=v, valid_before=v[0]), dict(valid=v, h0=h0, valid_before=v[0], use_memory=v),
+               dict(valid=v, h0=h0, valid_before=v), dict(valid=v, h0=h0, valid_before=v[0].float())):
+        with pytest.raises(ValueError, match="valid_before"):
+            filt(x, **kw)
+
+
 def test_weights_at_their_ends_and_refusals():
     from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
     x = torch.randn(5, 2, 21, 3, device="cuda")

@@ -15,11 +15,13 @@ from . import gated_filter as gf
 from .hand import NUM_LANDMARKS_PER_HAND
 
 
-def memory_after_gaps(valid: torch.Tensor) -> torch.Tensor:
+def memory_after_gaps(valid: torch.Tensor, before: Optional[torch.Tensor] = None) -> torch.Tensor:
     """use_memory [T, R] of the tracker's rule for valid [T, R]: a hand's memory counts in a frame when the hand was tracked
-    in the one before (tracker.py:233-236, 278-285)."""
+    in the one before (tracker.py:233-236, 278-285); `before` [R] says so for the frame ahead of the first (None: no hand was)."""
     use = torch.zeros_like(valid)
     use[1:] = valid[:-1]
+    if before is not None:
+        use[:1] = before
     return use
 
 
@@ -44,18 +46,28 @@ class LandmarkFilter(torch.nn.Module):
         return torch.addcmul(self.bias, self.slope, torch.log(sigmas))
 
     def forward(self, landmarks: torch.Tensor, valid: Optional[torch.Tensor] = None, sigmas: Optional[torch.Tensor] = None,
-                h0: Optional[torch.Tensor] = None, use_memory: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                h0: Optional[torch.Tensor] = None, use_memory: Optional[torch.Tensor] = None,
+                valid_before: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """landmarks [T, R, 21, 3] float32 (any order of the first two dimensions, e.g. a result file's [2, T, 21, 3]
         transposed), valid [T, R] bool: untracked frames keep the last filtered landmarks, and what landmarks and sigmas
-        hold there does not matter.  sigmas [T, R, 21] > 0.  use_memory defaults to the
-        tracker's rule for `valid`, with h0 (state before the first frame) counting in frame 0.  Returns (filtered
-        landmarks, state after the last frame [R, 21, 3])."""
+        hold there does not matter.  sigmas [T, R, 21] > 0.  use_memory defaults to the tracker's rule for `valid`.  Returns
+        (filtered landmarks, state after the last frame [R, 21, 3]).
+
+        A recording filtered in pieces: h0 is the state that the piece before returned, valid_before [R] its last frame's
+        `valid`, so that a hand that was not tracked there starts afresh.  Both can be left out where every hand was tracked in
+        every frame (valid None); with `valid`, h0 needs valid_before, or use_memory [T, R] in the place of the rule."""
         lead = tuple(landmarks.shape[:2])
+        if valid_before is not None:
+            if h0 is None or use_memory is not None:
+                raise ValueError("valid_before goes with h0 and without use_memory")
+            if tuple(valid_before.shape) != lead[1:] or valid_before.dtype != torch.bool:
+                raise ValueError(f"valid_before: expected a bool tensor {lead[1:]}")
+        elif h0 is not None and valid is not None and use_memory is None:
+            raise ValueError("h0 with valid: valid_before [R] has to say which hands were tracked in the frame before (or use_memory, "
+                             "in which frames memory counts)")
         if use_memory is None:
             rule = valid if valid is not None else torch.ones(lead, dtype=torch.bool, device=landmarks.device)
-            use_memory = memory_after_gaps(rule)
-            if h0 is not None and lead[0]:
-                use_memory[0] = True
+            use_memory = memory_after_gaps(rule, torch.ones_like(rule[:1]) if h0 is not None and valid_before is None else valid_before)
         if valid is not None and sigmas is not None:       # a gate's gradient is 0 there, and 0 times the log of anything need not be
             sigmas = torch.where(valid[..., None], sigmas, torch.ones((), device=sigmas.device))
         return gf.gated_scan(landmarks, self.gate(lead, sigmas), h0=h0, use_memory=use_memory, valid=valid)

@@ -70,6 +70,28 @@ def test_filter_over_recordings_and_frame_by_frame():
     assert worst <= 12 * U * np.abs(lm).max() / (1 - amax)
 
 
+def test_what_untracked_frames_show():
+    """The last landmarks once and then 0 by the tracker's rule; the last ones for the whole gap where the memory is kept in
+    untracked frames.  Tracked frames and gaps of one frame are the same in both."""
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter, memory_after_gaps
+    valid = torch.tensor([[c == "1" for c in f] for f in ("0110001011", "1000000000", "1101111100")]).t().cuda()
+    lm = (torch.rand(10, 3, 21, 3, generator=torch.Generator().manual_seed(1)) + 1).cuda()
+    filt = LandmarkFilter(0.6).cuda()
+    with torch.no_grad():
+        h, last = filt(lm, valid)
+        held, hl = filt(lm, valid, use_memory=memory_after_gaps(valid) | ~valid)
+    v = valid.tolist()
+    for r in range(3):
+        for t in range(10):
+            if v[t][r]:
+                assert torch.equal(h[t, r], held[t, r])
+            else:
+                seen = any(v[k][r] for k in range(t))
+                assert torch.equal(held[t, r], held[t - 1, r]) if seen else bool((held[t, r] == 0).all())
+                assert torch.equal(h[t, r], h[t - 1, r]) if t and v[t - 1][r] else bool((h[t, r] == 0).all())
+        assert torch.equal(last[r], h[9, r]) and torch.equal(hl[r], held[9, r])
+
+
 @pytest.mark.parametrize("cut", range(1, 12))
 def test_a_recording_in_pieces_is_the_recording(cut):
     """Cut inside gaps of one and of several frames, before and behind them, without use_memory."""

@@ -97,7 +97,8 @@ class BulkSequenceRunner:
     def smooth_landmarks(self, landmarks: torch.Tensor, filt: LandmarkFilter, out: Optional[RegressorOutput] = None,
                          valid: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Landmarks [S,21,3] of ``run``'s poses (skin_landmarks) smoothed along every (recording, hand) row in one call; same
-        order and shape.  ``out``: run's outputs, whose sigmas the filter may weigh by; ``valid`` as ``run``'s."""
+        order and shape.  ``out``: run's outputs, whose sigmas the filter may weigh by; ``valid`` as ``run``'s: untracked
+        hand-frames hold the last landmarks once and are 0 from a gap's second frame on (LandmarkFilter.forward)."""
         T, R = self.T, self.n_rec * 2
         sig = None if out is None else out.landmark_uncertainty_sigmas.view(R, T, 21).transpose(0, 1)
         h, _ = filt(landmarks.view(R, T, 21, 3).transpose(0, 1), None if valid is None else valid.t(), sig)

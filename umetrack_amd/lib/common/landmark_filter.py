@@ -49,9 +49,13 @@ class LandmarkFilter(torch.nn.Module):
                 h0: Optional[torch.Tensor] = None, use_memory: Optional[torch.Tensor] = None,
                 valid_before: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """landmarks [T, R, 21, 3] float32 (any order of the first two dimensions, e.g. a result file's [2, T, 21, 3]
-        transposed), valid [T, R] bool: untracked frames keep the last filtered landmarks, and what landmarks and sigmas
-        hold there does not matter.  sigmas [T, R, 21] > 0.  use_memory defaults to the tracker's rule for `valid`.  Returns
-        (filtered landmarks, state after the last frame [R, 21, 3]).
+        transposed), valid [T, R] bool: what landmarks and sigmas hold in untracked frames does not matter.  sigmas [T, R, 21]
+        > 0.  use_memory defaults to the tracker's rule for `valid`.  Returns (filtered landmarks, state after the last frame
+        [R, 21, 3]).
+
+        By that rule the first untracked frame of a gap still holds the last filtered landmarks; from the second one on the
+        memory is gone and the landmarks (and the state, where the recording ends there) are 0, as the result files have them.
+        use_memory = memory_after_gaps(valid) | ~valid holds the last ones through the whole gap; tracked frames are the same.
 
         A recording filtered in pieces: h0 is the state that the piece before returned, valid_before [R] its last frame's
         `valid`, so that a hand that was not tracked there starts afresh.  Both can be left out where every hand was tracked in

@@ -241,6 +241,27 @@ def test_tracker_smooths_the_landmarks_it_returns():
         assert all(np.isfinite(p.landmarks_mm).all() for p in res.hand_poses.values())
 
 
+def test_trackers_that_share_a_filter():
+    """One on the CPU stays there and works as one on the GPU does; one on the GPU is the tracker's own, also as it is fitted."""
+    from umetrack_amd import eval as ev
+    from umetrack_amd.lib.common.hand import load_generic_hand_model
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
+    from umetrack_amd.lib.models.model_loader import model_from_state_dict
+    from umetrack_amd.lib.tracker.tracker import HandTracker, HandTrackerOpts
+    hm = load_generic_hand_model()
+    rec = ev.SyntheticRecording(4, seed=3, hand_model=hm)
+    model = model_from_state_dict(arch.make_synthetic_state(4)).to("cuda")
+    opts = HandTrackerOpts(landmark_filter=LandmarkFilter(0.6))
+    a = _tracked(opts, rec, model, hm)
+    assert all(p.device.type == "cpu" for p in opts.landmark_filter.parameters())
+    b = _tracked(HandTrackerOpts(landmark_filter=LandmarkFilter(0.6).cuda()), rec, model, hm)
+    for p, q in zip(a, b):
+        assert set(p.hand_poses) == set(q.hand_poses)
+        assert all(np.array_equal(p.hand_poses[h].landmarks_mm, q.hand_poses[h].landmarks_mm) for h in p.hand_poses)
+    filt = LandmarkFilter(0.6).cuda()
+    assert HandTracker(model, HandTrackerOpts(landmark_filter=filt))._filter is filt
+
+
 def test_evaluation_with_smoothing(tmp_path):
     from oracle import metrics as omx
     from umetrack_amd import eval as ev

@@ -215,6 +215,17 @@ def test_forward_mode_tangents():
         assert "forward-mode" not in str(plain.value)
 
 
+def test_a_tracker_leaves_the_callers_filter_where_it_is():
+    from umetrack_amd.lib.common.landmark_filter import LandmarkFilter
+    from umetrack_amd.lib.tracker import tracker
+    filt, other = LandmarkFilter(0.3), torch.device("meta")
+    kept = list(filt.parameters())
+    moved = tracker._filter_on(filt, other)
+    assert moved is not filt and all(p.device == other for p in moved.parameters())
+    assert all(p is q and p.device.type == "cpu" for p, q in zip(filt.parameters(), kept))
+    assert tracker._filter_on(filt, torch.device("cpu")) is filt and tracker._filter_on(None, other) is None
+
+
 @pytest.mark.gpu
 def test_forward_mode_tangents_on_the_gpu():
     from torch.autograd import forward_ad

@@ -4,6 +4,7 @@ The image warp, the network and the forward kinematics run on the GPU; this clas
 only packs inputs and unpacks outputs.  ``HandTracker`` needs a model created by
 ``umetrack_amd.lib.models.model_loader`` and an MI355X.
 """
+import copy
 import logging
 from dataclasses import dataclass
 from typing import Dict, List, Optional
@@ -53,7 +54,8 @@ class HandTrackerOpts:
     min_required_vis_landmarks: int = 19
     warp_mode: int = gpu_warp.MODE_CV2     # OpenCV-compatible fixed-point sampling (see csrc/warp.hip)
     # smooths the landmarks that the returned poses carry (landmarks_mm), frame by frame on the GPU; the poses themselves
-    # stay as the model gave them.  None (the reference): landmarks as the frame gave them
+    # stay as the model gave them.  A filter on the tracker's GPU is used as it is (what is fitted later counts), one that
+    # lies elsewhere is copied when the tracker is made.  None (the reference): landmarks as the frame gave them
     landmark_filter: Optional[LandmarkFilter] = None
 
 
@@ -229,6 +231,14 @@ class _FrameIO:
         torch.cuda.current_stream(self.device).synchronize()
 
 
+def _filter_on(filt: Optional[LandmarkFilter], device: torch.device) -> Optional[LandmarkFilter]:
+    """The caller's filter where it lies on `device` already, else a copy there: Module.to would move the caller's own, and
+    with it that of every other tracker made from the same options."""
+    if filt is None or all(p.device == device for p in filt.parameters()):
+        return filt
+    return copy.deepcopy(filt).to(device)
+
+
 class HandTracker:
     def __init__(self, model, opts: HandTrackerOpts) -> None:
         self._device = "cuda"
@@ -246,9 +256,8 @@ class HandTracker:
         self._hm_dev: Optional[HandModel] = None
         self._skel: Optional[InputSkeletonData] = None
         self._src_rows = {}                          # id(camera) -> (camera, packed row): rig cameras are constant
-        self._filter = opts.landmark_filter
+        self._filter = _filter_on(opts.landmark_filter, self._io.device)
         if self._filter is not None:
-            self._filter = self._filter.to(self._io.device)
             self._filter_state = torch.zeros(NUM_HANDS, 21, 3, device=self._io.device)
         self._filter_history = np.zeros(NUM_HANDS, dtype=bool)       # hands whose filter row is the last frame's and finite
 

@@ -426,6 +426,7 @@ class HandTracker:
                                 wrist_translation_scale=M_TO_MM, status=status_dev[1:2],
                                 out=io.devt("lm").view(bs, 21, 3) if self._filter is None else None)
             if self._filter is not None:    # memory as the model's: it counts when the hand was tracked in the frame before
+                self._filter_history[:] = False         # the rows move on now: a frame that raises below leaves none that counts
                 self._filter.step(lm, self._filter_state, io.devt("fuse").view(bs).view(torch.bool), io.devt("midx").view(bs),
                                   sigmas=out.landmark_uncertainty_sigmas, out=io.devt("lm").view(bs, 21, 3))
         self._model.status_to(status_dev[0:1])

@@ -228,6 +228,41 @@ def test_graph_replays():
         assert all(torch.equal(a, b) for a, b in zip(bufs, fresh))
 
 
+def test_what_a_call_writes_in_place_autograd_sees():
+    """A tensor that a graph has saved and a call then overwrites: its backward pass raises, as after torch's own operations in
+    place, instead of using the new content."""
+    from umetrack_amd.lib.common import gated_filter as gf
+    rc, one = _rc(), torch.tensor([1], device="cuda")
+
+    def saved(t):
+        w = torch.ones(1, device="cuda", requires_grad=True)
+        return (t * w).sum()
+    x, gate, live = torch.rand(2, 3, device="cuda"), torch.zeros(2, device="cuda"), torch.tensor([True, True, False], device="cuda")
+    calls = {"out": lambda s: gf.gated_step(x, gate, torch.zeros(3, 3, device="cuda"), out=s[:2]), "state": lambda s: gf.gated_step(x, gate, s),
+             "copy": lambda s: rc.copy_rows([s], one, one - 1), "fork": lambda s: rc.fork_rows([s], live.clone(), one),
+             "compact": lambda s: rc.compact_rows([s], live.clone())}
+    for name, call in calls.items():
+        s = torch.rand(3, 3, device="cuda")
+        loss = saved(s)
+        call(s)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    for call in (lambda: rc.free_rows(live, one), lambda: rc.fork_rows([x.new_zeros(3, 1)], live, one), lambda: rc.compact_rows([x.new_zeros(3, 1)], live)):
+        before = live._version
+        call()
+        assert live._version > before
+    with pytest.raises(nat.UmtError, match="not differentiable"):
+        gf.gated_step(x, gate, torch.zeros(3, 3, device="cuda"), out=torch.zeros(2, 3, device="cuda", requires_grad=True))
+    read = x._version, gate._version
+    gf.gated_step(x, gate, torch.zeros(3, 3, device="cuda"))
+    gf.gated_scan(x[None], gate[None])
+    assert (x._version, gate._version) == read
+    with torch.inference_mode():
+        s = torch.zeros(3, 3, device="cuda")
+        gf.gated_step(x, gate, s)
+        rc.copy_rows([s], one, one - 1)
+
+
 def test_model_memory_moves_with_the_filter_state():
     """The model's temporal rows as one of the buffers: frames of two hands, the state of one hand forked, the other's row
     freed and the cache closed up; the fork then goes on exactly as the original does."""

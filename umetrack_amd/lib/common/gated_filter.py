@@ -12,6 +12,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ... import _native as nat
 
@@ -248,7 +249,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     B, feat = x.shape[0], x.shape[1:]
     if state.dtype != torch.float32 or state.dim() < 1 or state.shape[1:] != feat or state.device != dev or not state.is_contiguous():
         raise ValueError(f"gated_step: state is a contiguous float32 tensor [rows, {', '.join(map(str, feat))}] on {dev}")
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad or out is not None and out.requires_grad):
         raise nat.UmtError("gated_step is not differentiable: use gated_scan, or call it under torch.no_grad()")
     rows = state.shape[0]
     if rows >= 1 << 31:
@@ -262,6 +263,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
     use, ok = _mask("use_memory", use_memory, (B,), dev), _mask("valid", valid, (B,), dev)
     use, ok = None if use is None else use.contiguous(), None if ok is None else ok.contiguous()
     x, gate = x.contiguous(), gate.contiguous()
+    written = (state,) if out is None else (state, out)
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
@@ -276,4 +278,5 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, memory_
         nat.check(L.umt_gated_step(_DTYPES[x.dtype], x.data_ptr(), gate.data_ptr(), _raw(memory_idx), _raw(use), _raw(ok), B, groups, share,
                                    state.data_ptr(), rows, out.data_ptr(), _raw(status), _raw(ws), 0 if ws is None else ws.numel(),
                                    nat.raw_stream(dev)), "umt_gated_step")
+    increment_version(written)                             # a backward pass that has saved one of them raises
     return out

@@ -13,6 +13,7 @@ import ctypes
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ... import _native as nat
 
@@ -21,7 +22,7 @@ def _collect(buffers, rows: Optional[int]):
     """-> (umt_row_buffer array, its length, rows, device, tensors).  `rows` None: what the first tensor has, else the model."""
     if isinstance(buffers, torch.Tensor) or not isinstance(buffers, (list, tuple)):
         buffers = [buffers]
-    entries, dev, models, name = [], None, [], "row cache"
+    entries, dev, models, tensors, name = [], None, [], [], "row cache"
     for b in buffers:
         if isinstance(b, torch.Tensor):
             have, size = b.shape[0] if b.dim() else 0, b.nbytes
@@ -35,6 +36,7 @@ def _collect(buffers, rows: Optional[int]):
                 raise ValueError(f"{name}: a buffer has {have} rows and not {rows}")
             d = b.device
             entries.append((b.data_ptr(), size // rows if rows else 1))
+            tensors.append(b)
         elif hasattr(b, "memory_buffers"):
             d = b.device
             if d is None:
@@ -58,7 +60,7 @@ def _collect(buffers, rows: Optional[int]):
     if rows >= 1 << 31:                                                        # the library takes them as ints
         raise ValueError(f"{name}: {rows} rows")
     arr = (nat.RowBuffer * len(entries))(*entries)
-    return arr, len(entries), rows, dev
+    return arr, len(entries), rows, dev, tensors
 
 
 def _ids(name: str, t, dev) -> torch.Tensor:
@@ -92,7 +94,7 @@ def _work(nbytes: int, dev):
 def copy_rows(buffers: Sequence, src: torch.Tensor, dst: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
     """Row dst[i] becomes what row src[i] was before the call (so permutations and swaps are fine); of several writes to one
     row the highest i counts."""
-    arr, n_buf, rows, dev = _collect(buffers, None)
+    arr, n_buf, rows, dev, tensors = _collect(buffers, None)
     src, dst = _ids("src", src, dev), _ids("dst", dst, dev)
     if src.shape != dst.shape:
         raise ValueError(f"copy_rows: {src.shape[0]} sources and {dst.shape[0]} targets")
@@ -103,13 +105,14 @@ def copy_rows(buffers: Sequence, src: torch.Tensor, dst: torch.Tensor, status: O
     with nat.on_device(dev):
         ws, p, size = _work(L.umt_rows_copy_workspace_bytes(arr, n_buf, rows, n), dev)
         nat.check(L.umt_rows_copy(arr, n_buf, rows, src.data_ptr(), dst.data_ptr(), n, st, p, size, nat.raw_stream(dev)), "umt_rows_copy")
+    increment_version(tensors)                             # a backward pass that has saved one of them raises
 
 
 def fork_rows(buffers: Sequence, live: torch.Tensor, src: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """For each of ``src``, in order, the lowest free row becomes a live copy of it.  Returns the new row numbers (int64);
     -1 where src[i] is not a live row or no free row was left."""
     live = _live(live)
-    arr, n_buf, rows, dev = _collect(buffers, live.shape[0])
+    arr, n_buf, rows, dev, tensors = _collect(buffers, live.shape[0])
     _live(live, rows, dev)
     src = _ids("src", src, dev)
     n, st = src.shape[0], _status(status, dev)
@@ -121,6 +124,7 @@ def fork_rows(buffers: Sequence, live: torch.Tensor, src: torch.Tensor, status: 
         ws, p, size = _work(L.umt_rows_fork_workspace_bytes(rows, n), dev)
         nat.check(L.umt_rows_fork(arr, n_buf, rows, live.data_ptr(), src.data_ptr(), n, ids.data_ptr(), st, p, size,
                                   nat.raw_stream(dev)), "umt_rows_fork")
+    increment_version(tensors + [live])
     return ids
 
 
@@ -138,6 +142,7 @@ def free_rows(live: torch.Tensor, rows: torch.Tensor, status: Optional[torch.Ten
     with nat.on_device(dev):
         nat.check(nat.lib().umt_rows_free(live.data_ptr(), live.shape[0], rows.data_ptr(), rows.shape[0], st, nat.raw_stream(dev)),
                   "umt_rows_free")
+    increment_version(live)
 
 
 def compact_rows(buffers: Sequence, live: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -145,7 +150,7 @@ def compact_rows(buffers: Sequence, live: torch.Tensor) -> Tuple[torch.Tensor, t
     updated).  Only rows that have to move do; the others keep their numbers.  Returns (now, count): now[r] (int64 [rows]) is
     the row that holds what row r held, -1 for a free one; count is int64[1]."""
     live = _live(live)
-    arr, n_buf, rows, dev = _collect(buffers, live.shape[0])
+    arr, n_buf, rows, dev, tensors = _collect(buffers, live.shape[0])
     _live(live, rows, dev)
     now = torch.empty(rows, dtype=torch.int64, device=dev)
     count = torch.empty(1, dtype=torch.int64, device=dev)
@@ -154,4 +159,5 @@ def compact_rows(buffers: Sequence, live: torch.Tensor) -> Tuple[torch.Tensor, t
         ws, p, size = _work(L.umt_rows_compact_workspace_bytes(rows), dev)
         nat.check(L.umt_rows_compact(arr, n_buf, rows, live.data_ptr(), now.data_ptr(), count.data_ptr(), p, size,
                                      nat.raw_stream(dev)), "umt_rows_compact")
+    increment_version(tensors + [live])
     return now, count

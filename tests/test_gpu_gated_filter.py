@@ -123,6 +123,49 @@ def test_scan_and_gradients(shape, dtype, masks, rows_first):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows_first", [False, True])
+def test_types_shapes_and_order_of_the_outputs(dtype, rows_first):
+    for T, R, G, K in SHAPES:
+        if T * R * G * K > 2_000_000:
+            continue
+        x, gate, h0, use, valid = make(T, R, G, K, dtype, 1, True, rows_first)
+        h, last, kept = _gf().gated_scan(x, gate, h0, use, valid, keep=True)
+        assert h.dtype == x.dtype and h.shape == x.shape and last.dtype == torch.float32 and last.shape == h0.shape
+        assert kept.dtype == torch.float32 and kept.shape == (-(-T // nat.GATED_KEEP), R * G * K)
+        assert T == 1 or R == 1 or h.stride()[:2] == x.stride()[:2]
+        dx, dg, d0 = _gf().gated_scan_backward(x, gate, kept, torch.ones_like(h), last, use, valid)
+        assert dx.dtype == dg.dtype == x.dtype and d0.dtype == torch.float32
+        assert dx.shape == x.shape and dg.shape == gate.shape and d0.shape == h0.shape
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(3000, 2, 21, 3), (300, 20, 21, 3), (300, 200, 21, 3), (40, 1100, 63, 1), (2500, 3, 1, 63)], ids=str)
+def test_the_gradient_of_a_stretched_gate(shape, dtype):
+    """A filter's constants stretched over frames and rows, through every way the axis is shared out: T R slopes, each off by the
+    module's bound (with gates within 0.5 of 0, so K = 1 / sigmoid(-0.5) = 2.7) and rounded to the type, then summed by torch
+    (a rounding of the partial sums for each level of the sum) and rounded once more."""
+    T, R, G, K = shape
+    g = torch.Generator().manual_seed(sum(shape))
+    x, dh = (torch.randn(T, R, G, K, generator=g).to(DT[dtype]).cuda() for _ in range(2))
+    valid = (torch.rand(T, R, generator=g) > 0.1).cuda()
+    use = (torch.rand(T, R, generator=g) > 0.1).cuda()
+    bias = (torch.rand(G, generator=g) - 0.5).to(DT[dtype]).cuda().requires_grad_(True)
+    gate = bias.expand(T, R, G)
+    h, _ = _gf().gated_scan(x, gate, None, use, valid)
+    (got,) = torch.autograd.grad(h, bias, dh)
+    *_, slopes, _, s = oracle(*map(np64, (x, gate, None, use, valid, dh)))
+    eh, M, kk = slack(x, gate, None, valid, T)
+    S = np.abs(s).max()
+    es = 6 * U * S * kk
+    each = K * 0.25 * (S * (eh + 4 * U * M) + 2 * M * es + 12 * U * S * 2 * M)
+    half_step = 2.0 ** -8 if dtype == "bf16" else U
+    size = np.abs(slopes).sum((0, 1))
+    want = slopes.sum((0, 1))
+    tol = T * R * each + (half_step + 64 * U) * size + half_step * np.abs(want)
+    assert (np.abs(np64(got) - want) <= tol).all(), float((np.abs(np64(got) - want) / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("share", [2, 4, 6, 14, 15, 16, 17, 20, 21, 22, 28, 30, 31, 32, 33, 34, 36, 42, 47, 48, 62, 63, 64, 66, 126, 127, 128, 129, 250])
 def test_gate_sums_of_every_width(share, dtype):
     """Gates that begin and end anywhere among a wave's lanes, in rows of few gates and of many."""

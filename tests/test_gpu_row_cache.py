@@ -79,6 +79,35 @@ def test_copy_skips_rows_outside_the_cache():
     assert same(bufs, want) and int(st) == nat.STATUS_BAD_ROW
 
 
+@pytest.mark.parametrize("kind,rows,n", [("tracker", 10, 20), ("tracker", 900, 3000), ("odd", 200000, 3000), ("odd", 5000, (1 << 14) + 5),
+                                         ("odd", (1 << 18) + 9, 3000)])
+def test_every_form_of_the_copy_skips_rows_outside_the_cache(kind, rows, n):
+    """A few rows, copies planned in LDS, a table of the cache.  A third of the pairs has a bad source or target; targets are
+    named twice, and of some the highest copy is a bad one, which then does not count."""
+    bufs = buffers(kind, rows)
+    want = host(bufs)
+    old = [w.clone() for w in want]
+    g = torch.Generator().manual_seed(rows + n)
+    src, dst = torch.randint(0, rows, (n,), generator=g), torch.randint(0, min(rows, n // 3 + 1), (n,), generator=g)
+    bad = torch.tensor([-1, rows, rows + 7, 1 << 40, -(1 << 40)])
+    for t in (src, dst):
+        at = torch.rand(n, generator=g) < 0.18
+        t[at] = bad[torch.randint(0, 5, (int(at.sum()),), generator=g)]
+    half = torch.arange(n // 2, n)[:max(1, n // 20)]
+    dst[half + (n - n // 2) // 2] = dst[half]              # the second of these is the higher one, and its source is bad
+    src[half + (n - n // 2) // 2] = rows
+    for s, d in zip(src.tolist(), dst.tolist()):
+        if 0 <= s < rows and 0 <= d < rows:
+            for w, o in zip(want, old):
+                w[d] = o[s]
+    st = status()
+    _rc().copy_rows(bufs, src.cuda(), dst.cuda(), st)
+    assert same(bufs, want) and int(st) == nat.STATUS_BAD_ROW
+    bufs = buffers(kind, rows)
+    _rc().copy_rows(bufs, src.cuda(), dst.cuda())                            # without a status word
+    assert same(bufs, want)
+
+
 @pytest.mark.parametrize("kind,rows,n,dead", [("tracker", 4, 2, 2), ("tracker", 64, 5, 9), ("odd", 1000, 300, 300), ("odd", 1025, 100, 40),
                                               ("tracker", 5000, 1500, 2000), ("long", 9, 3, 4), ("odd", 70000, 30000, 33000), ("odd", 5, 3, 0)])
 def test_free_and_fork(kind, rows, n, dead):

@@ -17,7 +17,7 @@ constexpr int RT = 256;
 constexpr int64_t MOVE_BYTES = 4096;       // 64 lanes x 16 bytes x 4 loads in flight
 constexpr int ONE = 1024;                  // threads of a workgroup that ranks rows
 constexpr int BLOCK = 4 * ONE;             // rows it takes at once
-constexpr int SMALL_BYTES = 64 * 1024;     // moves that one workgroup makes itself rather than wait for another launch
+constexpr int LDS_BYTES = 64 * 1024;       // of a workgroup that stages rows
 
 struct RowBuffers {
   char* data[UMT_ROW_BUFFERS_MAX];
@@ -209,8 +209,9 @@ __device__ __forceinline__ int sum_counts(const int32_t* counts, int upto, int* 
 }
 
 // ---------------------------------------------------------------- copy
-// A few rows: one workgroup holds them all in LDS between reading and writing.
-constexpr int FEW = 256;
+// A few rows: one workgroup holds them all in LDS between reading and writing (calls replayed in a graph, this against the
+// two launches below: 20 rows of 2908 bytes 17.0 and 17.2 us, 64 rows of 252 bytes 16.2 and 16.1, 200 of them 29.9 and 16.2).
+constexpr int FEW = 64;
 __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n,
                                                        int rows, int32_t* __restrict__ status) {
   extern __shared__ uint4 stage[];
@@ -241,7 +242,9 @@ __global__ __launch_bounds__(ONE) void copy_few_kernel(RowBuffers B, const int64
 // More: two launches.  Every workgroup of the first marks all targets in a bit map of the cache in its LDS (64 KB of row
 // numbers from L2 for 8191 copies), decides on copies of its own and brings those sources to safety that the call overwrites.
 // plan[i]: what the second launch does.  8191 of 32768 rows of 2592 + 64 + 252 bytes, sources and
-// targets drawn apart from each other: 5.3 + 10.9 us, where the five launches below take 25.
+// targets drawn apart from each other: 5.3 + 10.9 us, where the five launches below take 25.  The limits are the bit map's LDS
+// and the launch's share of the numbers; both are ahead of the five up to there (calls replayed in a graph: 16384 copies in
+// 262144 rows 17.8 and 23.8 us, 300 in 262144 rows 16.5 and 17.7).
 enum { COPY_NOT = 0, COPY_ROW = 1, COPY_STAGED = 2 };
 constexpr int MAP_ROWS = 1 << 18;          // 32 KB of bits
 constexpr int MAP_COPIES = 1 << 14, MAP_GROUPS = 128, MAP_EACH = MAP_COPIES / MAP_GROUPS;      // MAP_EACH <= ONE: a copy a thread
@@ -404,7 +407,8 @@ __device__ __forceinline__ int hand_out_rows(uint8_t* live, int rows, int64_t r0
   return all;
 }
 
-// everything in one workgroup; `moves`: the copies too (6.7 us for 2 of 64 rows)
+// everything in one workgroup; `moves`: the copies too (6.7 us for 2 of 64 rows), where every wave has one at most (calls
+// replayed in a graph, against another launch for them: 8 rows of 2908 bytes 16.8 and 17.8 us, 64 rows of 252 19.3 and 16.8)
 __global__ __launch_bounds__(ONE) void fork_one_kernel(RowBuffers B, uint8_t* live, int rows, const int64_t* __restrict__ src, int n,
                                                        int64_t* ids, int32_t* order, int32_t* status, int moves) {
   __shared__ int lds[ONE / 64];
@@ -597,7 +601,7 @@ static int need_workspace(const char* what, const void* ws, int64_t have, int64_
 
 using namespace umt;
 
-static bool few_rows(const RowBuffers& B, int n) { return n <= FEW && n * B.staged_bytes <= SMALL_BYTES - 16 * FEW; }
+static bool few_rows(const RowBuffers& B, int n) { return n <= FEW && n * B.staged_bytes <= LDS_BYTES - 16 * FEW; }
 static bool planned(int rows, int n) { return rows <= MAP_ROWS && n <= MAP_COPIES; }
 static int blocks_of(int64_t n) { return (int)((n + BLOCK - 1) / BLOCK); }
 
@@ -647,7 +651,9 @@ extern "C" int umt_rows_copy(const umt_row_buffer* buffers, int n_buffers, int r
   return 0;
 }
 
-// one workgroup ranks this many rows or sources in the time of the other launches' start
+// One workgroup ranks this many rows or sources in the time of the other launches' start (calls replayed in a graph, one
+// workgroup against the four launches: 1000 of 4096 rows 18.0 and 22.9 us; of 16384 rows 2 17.4 and 20.6, 1000 23.8 and 22.5;
+// 1000 of 32768 rows 31.6 and 22.9)
 static bool one_group(int rows, int n) { return rows <= 4 * BLOCK && n <= BLOCK; }
 
 extern "C" int64_t umt_rows_fork_workspace_bytes(int rows, int n) {
@@ -666,7 +672,7 @@ extern "C" int umt_rows_fork(const umt_row_buffer* buffers, int n_buffers, int r
   hipStream_t s = (hipStream_t)stream;
   int32_t *order = (int32_t*)workspace, *counts = order + n;
   if (one_group(rows, n)) {
-    const int moves = n <= FEW && n * B.staged_bytes <= SMALL_BYTES;
+    const int moves = (int64_t)n * B.piece0[B.n_long] <= ONE / 64;
     hipLaunchKernelGGL(fork_one_kernel, dim3(1), dim3(ONE), 0, s, B, live, rows, src, n, ids, order, status, moves);
     if (!moves) hipLaunchKernelGGL(fork_move_kernel, dim3(grid), dim3(RT), 0, s, B, src, ids, n);
   } else {

@@ -1,6 +1,6 @@
 // What the matrix pipe of THIS chip sustains in loops with no memory traffic at all (experiments only, not part of the
 // library): the practical ceiling the convolution kernels are compared with in DESIGN.md beside the datasheet peak.
-//   hipcc -O3 --offload-arch=gfx950 tools/mfma_peak.hip -o tools/bin/mfma_peak && tools/bin/mfma_peak
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_peak.hip -o tools/bin/mfma_peak && tools/bin/mfma_peak
 // Every wave runs ITERS x 8 independent MFMAs on register operands (8 accumulator tiles, so issue is back to back), one or
 // two waves per SIMD, all 256 CUs.  The LDS variants re-read both operands with ds_read_b128 before every MFMA pair, which
 // is what a 2x2-tile GEMM inner loop does.
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(256) void k_bf16_32_lds12(float* out, float seed) {
 }
 
 // Does vector arithmetic of one wave overlap the MFMAs of another wave on the same SIMD?  512-thread workgroups: waves
-// 0-3 run MFMAs back to back (when mode & 1), waves 4-7 packed fp32 FMAs (when mode & 2).  g_mix[0..1] = ticks of wave 0,
+// 0-3 run MFMAs back to back (when mode & 1), waves 4-7 pairs of fp32 FMAs (when mode & 2; two instructions a pair, as the
+// build leaves the packed form out).  g_mix[0..1] = ticks of wave 0,
 // g_mix[2..3] = ticks of wave 4.
 __device__ unsigned long long g_mix[4];
 template <int mode>
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(512) void k_mix(float* out, int) {
     constexpr int nops = (mode >> 4) & 3;       // mode bits 4-5: s_nop cycles after every MFMA: 0, 8, 16 or 24
     f32x2 w[4] = {{1.f, 2.f}, {3.f, 4.f}, {5.f, 6.f}, {7.f, 8.f}};
     const f32x2 wm = {1.0001f, 0.9999f}, wc = {rnd(threadIdx.x), rnd(threadIdx.x + 99)};
-    constexpr int own = (mode >> 6) & 7;        // mode bits 6-8: packed FMAs of this same wave after every MFMA
+    constexpr int own = (mode >> 6) & 7;        // mode bits 6-8: FMA pairs of this same wave after every MFMA
     for (int it = 0; it < 2048; ++it) {
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
@@ -210,7 +211,7 @@ static void run_mix(float* out) {
     (void)hipDeviceSynchronize();
     unsigned long long t[4];
     (void)hipMemcpyFromSymbol(t, HIP_SYMBOL(g_mix), sizeof(t));
-    printf("mix, %-30s: ticks per MFMA %.1f (16384 per wave), ticks per v_pk_fma_f32 %.2f (65536 per wave)\n", names[k],
+    printf("mix, %-30s: ticks per MFMA %.1f (16384 per wave), ticks per pair of fp32 FMAs %.2f (65536 per wave)\n", names[k],
            (mode & 1) ? (double)(t[1] - t[0]) / 16384.0 : 0.0, (mode & 2) ? (double)(t[3] - t[2]) / 65536.0 : 0.0);
   }
 }

@@ -625,7 +625,7 @@ __global__ __launch_bounds__((group_threads<W, RUNS>())) void gated_scan_kernel(
 // two are added first; `share` and `per` count lanes here).  The KEEP steps' products go through the wave's own LDS rows.
 // Gates of 16 lanes and more: lane 16 k + j reads the 16 products of step j that lanes 16 k .. 16 k + 15 left, at most two
 // gates' of which the second begins at `bound`, and the four such parts of a step are added across the wave (255 steps of
-// 384 x 18 gates of 18 lanes: 14 us in the place of 30 with the gates one after the other).  Smaller gates: with n of them in
+// 384 x 18 gates of 18 lanes: 18 us of the kernel, 32 with the gates one after the other).  Smaller gates: with n of them in
 // the wave, lane n i + k adds up gate k of the steps i, i + 64 / n, ..., and neighbouring lanes write neighbouring gates.  A
 // gate that reaches into other waves leaves its part in `part`, and a second launch adds the parts in order (7.5 us there).
 constexpr int SUM_ROW = 68;                // floats of a step's row: 16-byte reads of 16 steps lie in different banks
@@ -785,7 +785,7 @@ __global__ __launch_bounds__(GT) void gate_parts_kernel(umt_gated_shape S, int p
 //   s = dh + v,  dx = c s,  dgate = sum a c s (h' - x),  v' = a s
 // 512 steps of 512 rows of 648 bf16 values with a gate each: 380 us for 1.74 GB (4.6 TB/s).  255 steps of 384 rows of 18 x 36
 // values: 112 us for 0.40 GB (3.5 TB/s): two waves a SIMD, of which the vector operations alone take 70 us (about 65 for the
-// two values of a lane and step) and the sums about 10.  A stretch of inputs ahead is what fits: gradients ahead too spill
+// two values of a lane and step); the gate sums are 18 of the 112.  A stretch of inputs ahead is what fits: gradients ahead too spill
 // (x1.4 to x3.7).  Both weights a step in the place of m: 3 % less there, 3 % more with a gate a value.
 template <typename V, int E, int GE, typename OFF, int W, bool MASK, bool RUNS>
 __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_backward_kernel(
@@ -932,7 +932,10 @@ __global__ __launch_bounds__((group_threads<W, RUNS>()), 2) void gated_scan_back
 
 // ---------------------------------------------------------------- one frame over a cache of rows
 constexpr int STEP_SEG = 256;              // features one wave advances
-constexpr int STEP_LOOK = 1024;            // samples among which a wave looks for its row's other names itself
+// Samples among which a wave looks for its row's other names itself, rather than wait for two launches that make a table (calls
+// replayed in a graph, looking against the table: rows of 648 values, 512 samples 16.2 and 16.3 us, 1024 15.9 and 16.1, 1500
+// 18.4 and 16.7, 4096 58 and 22; of 63 values, 1500 16.7 and 16.9, 4096 27.5 and 16.1).
+constexpr int STEP_LOOK = 1024;
 
 // owner[r] = highest sample that names row r, named[r] = how many do; only rows that are named are touched
 __global__ __launch_bounds__(GT) void step_clear_kernel(const int64_t* __restrict__ idx, int batch, int cache_rows,
@@ -1069,12 +1072,19 @@ static int copy_ends(float* to, const float* from, int64_t n, hipStream_t s) {
   return 0;
 }
 
-// How the axis is shared out, for waves of `per` values.  A wave that walks alone needs about four others on its CU to keep
-// HBM busy; below that the waves of a workgroup take turns.  With a tile on fewer than two thirds of the CUs, an axis of more
-// than two tiles is cut into runs, at the price of reading the inputs twice (fp32, forward / backward: 3000 steps of 148
-// waves 92 / 169 us in tiles, 82 / 144 in runs; 2000 steps of 197 waves 64 / 122 and 78 / 135).  Eight runs are a workgroup,
-// and as many of them as fill the CUs evenly run at once: of one to four per CU what has the shortest way, with a stretch
-// more for the start of each (3000 steps of 99 waves: 57 / 89 us in 495 workgroups, 79 / 129 in 297).
+// How the axis is shared out, for waves of `per` values (times: fp32, forward / backward in us, calls replayed in a graph).
+// * A wave that walks alone needs about four others on its CU to keep HBM busy; below 1024 the waves of a workgroup take
+//   turns.  Alone against four: 1000 steps of 900 waves 132 / 245 and 169 / 260, of 1024 152 / 260 and 176 / 274, of 1200
+//   233 / 366 and 208 / 366; 250 steps of 700 waves 33 / 56 and 31 / 49, of 1024 39 / 70 and 39 / 73.  (From 1024 on the lone
+//   waves come in rounds, and which is ahead goes with what is left for the last round.)
+// * Eight waves take turns where tiles leave CUs free, else four.  600 steps of 200 waves: 28 / 40 in eights, 32 / 49 in fours;
+//   of 300 waves 45 / 69 and 42 / 59.  Four where they cover the axis: 48 steps of 300 waves 15 in fours, 21 in eights, backward.
+// * With a tile on fewer than two thirds of the CUs, an axis of more than two tiles is cut into runs, at the price of reading
+//   the inputs twice.  Tiles against runs: 3000 steps of 148 waves 92 / 169 and 82 / 144; 2000 steps of 197 waves 64 / 122 and
+//   78 / 135; of 40 waves 300 steps 17 / 23 and 16 / 19, of 100 waves 300 steps 18 / 24 and 22 / 28, 600 steps 25 / 35 and
+//   27 / 35; up to 256 steps they are within 2 us of each other.
+// * Eight runs are a workgroup, and as many of them as fill the CUs evenly run at once: of one to four per CU what has the
+//   shortest way, with a stretch more for the start of each.  3000 steps of 99 waves: 57 / 89 in 495 workgroups, 79 / 129 in 297.
 constexpr int CUS = 256;
 static Split split_axis(const umt_gated_shape& S, int per) {
   const int64_t N = (int64_t)S.rows * S.groups * S.share;

@@ -69,8 +69,8 @@ __global__ __launch_bounds__(256) void stem_kernel(StemParams p, const float* __
 #pragma unroll
       for (int dx = 0; dx < 4; ++dx) patch[dy][dx] = row[dx];
     }
-    // two channels per instruction (v_pk_fma_f32: the packed form is what reaches the vector fp32 rate); each lane of a
-    // pair is the same fmaf chain as before, so the results are unchanged
+    // two channels at a time; each half of a pair is the same fmaf chain as one channel alone.  (The build leaves packed fp32
+    // arithmetic out, so a pair is two v_fma_f32.)
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     float res[8];
 #pragma unroll

@@ -311,7 +311,8 @@ int umt_gated_scan(const umt_gated_shape* shape, const void* x, const void* gate
                    int64_t workspace_bytes, void* stream);
 /* Gradients of umt_gated_scan for dh (t, rows, features) and dh_last (NULL: zero).  x, gate, the masks and kept as in the
  * forward call.  dx, dgate (t, rows, groups) and dh0 are written whole; any of them may be NULL.  Skipped frames get
- * dx = dgate = 0, a dropped memory dgate = 0 and no gradient to what lies before it.                              */
+ * dx = dgate = 0, a dropped memory dgate = 0 and no gradient to what lies before it.  A gradient that is not finite makes those
+ * of its feature ahead of it non-finite up to a dropped memory.                                                    */
 int64_t umt_gated_scan_backward_workspace_bytes(const umt_gated_shape* shape);
 int umt_gated_scan_backward(const umt_gated_shape* shape, const void* x, const void* gate, const uint8_t* use_memory,
                             const uint8_t* valid, const float* kept, const void* dh, const float* dh_last, void* dx,

@@ -192,11 +192,14 @@ def raw_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def dual_level() -> bool:
+    """Inside torch.autograd.forward_ad.dual_level(), the only place where tensors have tangents."""
+    return forward_ad._current_level >= 0
+
+
 def no_tangents(name: str, *tensors) -> None:
-    """Refuses tensors that carry a forward-mode tangent (torch.autograd.forward_ad): the kernels read values alone, and the
-    outputs would silently have none.  Only looked for inside a dual level (0.6 us a tensor otherwise)."""
-    if forward_ad._current_level < 0:
-        return
+    """Refuses tensors that carry a forward-mode tangent: the kernels read values alone, and the outputs would silently have
+    none.  0.6 us a tensor, so callers ask dual_level() first."""
     for t in tensors:
         if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
             raise UmtError(f"{name} has no forward-mode derivative")

@@ -47,7 +47,8 @@ def _check_values(name: str, x, gate, *others) -> torch.device:
     """The device of x and gate; `others`: what else may carry derivatives."""
     if not (isinstance(x, torch.Tensor) and isinstance(gate, torch.Tensor)):
         raise TypeError(f"{name}: x and gate are tensors")
-    nat.no_tangents(name, x, gate, *others)
+    if nat.dual_level():
+        nat.no_tangents(name, x, gate, *others)
     if x.dtype not in _DTYPES or gate.dtype != x.dtype:
         raise TypeError(f"{name}: x and gate are both float32 or both bfloat16, got {x.dtype} and {gate.dtype}")
     dev = x.device
@@ -196,7 +197,8 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dh_last):
         if dh is None and dh_last is None:
             return None, None, None, None, None, None, None
-        nat.no_tangents("gated_scan's backward pass", dh, dh_last)
+        if nat.dual_level():
+            nat.no_tangents("gated_scan's backward pass", dh, dh_last)
         x, gate, kept, use, valid = ctx.saved_tensors
         if dh is None:
             dh = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)

@@ -30,7 +30,8 @@ def _collect(buffers, rows: Optional[int]):
                 raise ValueError(f"{name}: a buffer is a contiguous GPU tensor [rows, ...], got {tuple(b.shape)} on {b.device}")
             if b.requires_grad and torch.is_grad_enabled():
                 raise nat.UmtError(f"{name}: a buffer that requires gradients cannot be moved in place")
-            nat.no_tangents(name, b)
+            if nat.dual_level():
+                nat.no_tangents(name, b)
             rows = have if rows is None else rows
             if have != rows:
                 raise ValueError(f"{name}: a buffer has {have} rows and not {rows}")
@@ -50,7 +51,8 @@ def _collect(buffers, rows: Optional[int]):
         dev = d
     if not entries or len(entries) > nat.ROW_BUFFERS_MAX:
         raise ValueError(f"{name}: 1 to {nat.ROW_BUFFERS_MAX} buffers (a model counts as two), got {len(entries)}")
-    nat.require_gpu(dev)
+    if not tensors:                                        # those are on a GPU
+        nat.require_gpu(dev)
     for m, at in models:
         arr, have = m.memory_buffers()
         rows = have if rows is None else rows
@@ -71,10 +73,9 @@ def _ids(name: str, t, dev) -> torch.Tensor:
     return t.contiguous()
 
 
-def _live(t, rows: Optional[int] = None, dev=None) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bool or t.dim() != 1 or not t.is_cuda or not t.is_contiguous() \
-            or (rows is not None and t.shape[0] != rows) or (dev is not None and t.device != dev):
-        raise ValueError(f"live: expected a contiguous bool tensor ({'rows' if rows is None else rows},) on {dev or 'a GPU'}")
+def _live(t) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bool or t.dim() != 1 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError("live: expected a contiguous bool tensor (rows,) on a GPU")
     return t
 
 
@@ -113,7 +114,8 @@ def fork_rows(buffers: Sequence, live: torch.Tensor, src: torch.Tensor, status: 
     -1 where src[i] is not a live row or no free row was left."""
     live = _live(live)
     arr, n_buf, rows, dev, tensors = _collect(buffers, live.shape[0])
-    _live(live, rows, dev)
+    if live.device != dev:
+        raise ValueError(f"live: expected a contiguous bool tensor ({rows},) on {dev}")
     src = _ids("src", src, dev)
     n, st = src.shape[0], _status(status, dev)
     ids = torch.empty(n, dtype=torch.int64, device=dev)
@@ -134,7 +136,7 @@ def free_rows(live: torch.Tensor, rows: torch.Tensor, status: Optional[torch.Ten
     live = _live(live)
     if live.shape[0] >= 1 << 31:
         raise ValueError(f"live: {live.shape[0]} rows")
-    dev = nat.require_gpu(live.device)
+    dev = live.device
     rows = _ids("rows", rows, dev)
     st = _status(status, dev)
     if rows.shape[0] == 0:
@@ -151,7 +153,8 @@ def compact_rows(buffers: Sequence, live: torch.Tensor) -> Tuple[torch.Tensor, t
     the row that holds what row r held, -1 for a free one; count is int64[1]."""
     live = _live(live)
     arr, n_buf, rows, dev, tensors = _collect(buffers, live.shape[0])
-    _live(live, rows, dev)
+    if live.device != dev:
+        raise ValueError(f"live: expected a contiguous bool tensor ({rows},) on {dev}")
     now = torch.empty(rows, dtype=torch.int64, device=dev)
     count = torch.empty(1, dtype=torch.int64, device=dev)
     L = nat.lib()
